@@ -47,6 +47,9 @@ enum le_type {
     LE_IQ2_S = 22
 };
 
+/* Types of activations, scales and logits where an entry takes more than fp32 (GGML ids as well). */
+enum le_dtype { LE_F32 = 0, LE_F16 = 1, LE_BF16 = 30 };
+
 enum le_status {
     LE_OK = 0,
     LE_ERR_ARG = -1,    /* null pointer / bad count */
@@ -278,6 +281,68 @@ int le_moe_layer_ptrs(le_ctx *ctx, int ty_gate, int ty_up, int ty_down, const vo
  * if a one-launch layer on ws gave up at its barrier since the last check, else LE_OK. Not for use
  * under graph capture. */
 int le_moe_check(le_ctx *ctx, const void *ws, le_stream_t stream);
+
+/* ---- matrix-vector products with 4-bit codes and group scales (no counterpart in the reference, whose 4-bit weights are
+ *      GGUF blocks; the form of checkpoints that keep codes, scales and zero points as tensors of their own) ----
+ * A stack of n_mat matrices of rows x cols weights
+ *     w[r][c] = scale[r][c / group] * (code[r][c] - zero[r][c / group]),
+ * all three row-major and contiguous, matrix after matrix: codes two to a byte, the even column in the low half; scales and
+ * zeros of scale_type (LE_F32, LE_F16, LE_BF16), cols / group of them a row; zeros NULL stands for 8 everywhere. cols is a
+ * multiple of 32; group is cols (one scale a row) or a power of two from 32 on that divides cols. codes 16-byte aligned,
+ * scales and zeros aligned to their type. */
+typedef struct le_g4 {
+    const void *codes, *scales, *zeros; /* device */
+    int n_mat, rows, cols, group, scale_type;
+} le_g4;
+/* For slot s < slots and token t < m: y[(s * m + t) * rows + r] = w_M[r,:] . a(s, t), with M = sel[s] (device array of `slots`
+ * ints, e.g. the experts that le_moe_route picked) or M = s where sel is NULL (then slots <= n_mat). A slot whose sel lies outside
+ * 0 .. n_mat - 1 gets zeros. `share` consecutive slots share their activations: a(s, t) is row (s / share) * m + t of x, rows
+ * xstride values apart (0: one row for all). x and y are of type xtype; with swiglu 0, a is x's row of cols values, with
+ * swiglu 1 a[c] = silu(row[c]) * row[cols + c] for a row of 2 * cols (gate | up), silu(g) = g / (1 + exp(-g)).
+ * Products are exact (activations enter in bf16 pieces that add up to them; the SwiGLU's as fp32), sums are fp32, and the result
+ * is rounded once to xtype. A row's activations, finite, may be of any magnitude whose sums fp32 holds; one that is not finite makes
+ * its token's outputs infinite or NaN. Limits: m <= 64, slots <= 65535; x 16-byte aligned, xstride a multiple of 16 bytes. y may not
+ * overlap an input. */
+int le_matvec_g4(le_ctx *ctx, const le_g4 *w, const int *sel, int slots, int share, int xtype, const void *x,
+                 long long xstride, int m, void *y, int swiglu, le_stream_t stream);
+
+/* ---- expert routing as single steps (the reference's router_topk, src/cuda/kernels.cu:437-456, its host grouping,
+ *      src/gpu/prefill.rs:153-168, and moe_combine, :470-475, as entries of their own, with their gradients; le_moe_layer
+ *      runs its own forms of them) ----
+ * A pair is p = t * k + s: selection s < k of token t < n_tok. k <= 16, n_exp <= 1024, n_tok * k < 2^31; n_tok may be 0.
+ *
+ * le_moe_route: idx[p], w[p] = the experts of token t's k largest logits (type ltype; ties keep the lower expert) in falling
+ * order, and their softmax over the selected, exp(l - top) / sum. An expert whose logit is -infinity or NaN is never
+ * selected: selections without an expert get idx -1 and weight 0. A logit of +infinity gives its token NaN weights.
+ * le_moe_route_bwd: dlogits[t * n_exp + e] (type ltype) = w[p] * (dw[p] - sum_j w_j dw_j) at e = idx[p], the sum over the token's
+ * selections; 0 at experts not selected. Pairs with idx outside 0 .. n_exp - 1 count nowhere. */
+int le_moe_route(le_ctx *ctx, int ltype, const void *logits, int n_tok, int n_exp, int k, int *idx, float *w,
+                 le_stream_t stream);
+int le_moe_route_bwd(le_ctx *ctx, int ltype, const int *idx, const float *w, const float *dw, int n_tok, int n_exp, int k,
+                     void *dlogits, le_stream_t stream);
+/* le_moe_sort: the pairs grouped by expert, in pair order within an expert, as le_mm_grouped takes them: off (n_exp + 1),
+ * in_idx[i] = the token and out_idx[i] = the pair of place i < off[n_exp], and pos[p] = the place of pair p. A pair whose
+ * idx lies outside 0 .. n_exp - 1 is dropped: pos[p] = -1, and no place is its own (in_idx and out_idx keep what they held
+ * from off[n_exp] on). Any of in_idx, out_idx and pos may be NULL. ws: le_moe_sort_workspace_size bytes, 16-byte aligned (NULL where
+ * that is 0); calls that may overlap need workspaces of their own. */
+size_t le_moe_sort_workspace_size(int n_tok, int k, int n_exp);
+int le_moe_sort(le_ctx *ctx, const int *idx, int n_tok, int k, int n_exp, int *off, int *in_idx, int *out_idx, int *pos,
+                void *ws, size_t ws_bytes, le_stream_t stream);
+/* Rows between token order and expert order. All rows have cols values of type ty, token rows ldt values apart, expert rows
+ * lde apart (each >= cols); pos[p] is the expert row of pair p, a pair with pos outside 0 .. n_row - 1 has none. pos NULL
+ * stands for pos[p] = p (rows in pair order, as le_mm_grouped leaves them under out_idx).
+ * le_moe_permute: e[pos[p]] = x[t]; rows of no pair keep what they held. Its gradient is le_moe_combine with w NULL.
+ * le_moe_combine: out[t] = sum over the token's pairs that have a row of w[p] * e[pos[p]], added in selection order in fp32
+ * and rounded once; w NULL stands for 1. A token without such pairs gets zeros.
+ * le_moe_combine_bwd: de[pos[p]] = w[p] * dout[t] (rows of no pair keep what they held) and dw[p] = dout[t] . e[pos[p]], summed in
+ * fp32 in an order that cols alone decides, 0 for a pair without a row. de or dw may be NULL; e may be NULL where dw is, and
+ * w NULL stands for 1. Rows of different pairs must differ, but for rows that are only read; outputs may not overlap inputs (de may be e). */
+int le_moe_permute(le_ctx *ctx, int ty, const void *x, long long ldt, const int *pos, int n_tok, int k, int cols, void *e,
+                   long long lde, int n_row, le_stream_t stream);
+int le_moe_combine(le_ctx *ctx, int ty, const void *e, long long lde, int n_row, const int *pos, const float *w, int n_tok,
+                   int k, int cols, void *out, long long ldt, le_stream_t stream);
+int le_moe_combine_bwd(le_ctx *ctx, int ty, const void *dout, long long ldt, const void *e, long long lde, int n_row,
+                       const int *pos, const float *w, int n_tok, int k, int cols, void *de, float *dw, le_stream_t stream);
 
 #ifdef __cplusplus
 }

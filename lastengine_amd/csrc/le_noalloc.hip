@@ -21,7 +21,7 @@
 
 #include <mutex>
 
-#include "../../include/le_qmm.h"
+#include "le_ctx.h"
 
 static __device__ __align__(256) unsigned char scratch[LE_GEMM_SCRATCH_BYTES];
 
@@ -46,10 +46,6 @@ int le_scratch_attach(int device) {
     g_ptr[device] = p;
     return LE_OK;
 }
-
-/* Host-side helpers of le_qmm.cpp (the context lives there). */
-int le_ctx_device(const le_ctx *ctx);
-int le_ctx_fail(le_ctx *ctx, int code, const char *msg);
 
 extern "C" int le_gemm_noalloc(le_ctx *ctx, int ty, const void *w, const float *x, int m, float *y, int rows,
                                int cols, le_stream_t stream) {

@@ -20,13 +20,14 @@
 #include <vector>
 
 #include "../../include/le_qmm.h"
+#include "le_ctx.h"
 #include "le_mt_layout.h"
 #include "le_formats.h"
 
 namespace {
 
 const char *kParts[] = {"le_qmm_deq", "le_qmm_moe", "le_qmm_mv8", "le_qmm_mv12", "le_qmm_mv14", "le_qmm_mv16", "le_qmm_mv18", "le_qmm_gm",
-                        "le_qmm_gq", "le_qmm_gq2", "le_qmm_mt", "le_qmm_mv2", "le_qmm_mv11", "le_qmm_mv13", "le_qmm_mv22"};
+                        "le_qmm_gq", "le_qmm_gq2", "le_qmm_mt", "le_qmm_mv2", "le_qmm_mv11", "le_qmm_mv13", "le_qmm_mv22", "le_qmm_g4", "le_qmm_rt"};
 
 /* Kernel argument block of le_mv_* (mirrors MvArgs in le_qmm_kernels.hip). */
 struct MvArgs {
@@ -1537,6 +1538,33 @@ int le_stream_read_sink_bytes(le_ctx *c) { return c ? c->cus * 16 * 4 : 0; }
 
 }  // extern "C"
 
-/* Context accessors for le_noalloc.hip. */
+/* Context accessors (le_ctx.h). */
 int le_ctx_device(const le_ctx *c) { return c ? c->device : -1; }
-int le_ctx_fail(le_ctx *c, int code, const char *msg) { return c ? c->fail(code, "%s", msg) : code; }
+int le_ctx_cus(const le_ctx *c) { return c ? c->cus : 0; }
+int le_ctx_fail(le_ctx *c, int code, const char *msg) { return le_ctx_failf(c, code, "%s", msg); }
+int le_ctx_failf(le_ctx *c, int code, const char *fmt, ...) {
+    char buf[512];
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(buf, sizeof buf, fmt, ap);
+    va_end(ap);
+    try {
+        if (c) c->err = buf;
+    } catch (...) { /* no memory for the text: the code alone */
+    }
+    return code;
+}
+int le_ctx_on_device(le_ctx *c) {
+    int dev = -1;
+    if (hipGetDevice(&dev) != hipSuccess) return le_ctx_failf(c, LE_ERR_HIP, "hipGetDevice failed");
+    if (dev != c->device)
+        return le_ctx_failf(c, LE_ERR_ARG, "the current device is %d, the context's is %d", dev, c->device);
+    return LE_OK;
+}
+int le_ctx_launch(le_ctx *c, const char *name, dim3 grid, int block, size_t lds, hipStream_t st, void **args) {
+    try {
+        return c->launch(name, grid, block, lds, st, args);
+    } catch (...) {
+        return LE_ERR_HIP;
+    }
+}

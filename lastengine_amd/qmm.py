@@ -23,6 +23,8 @@ Q4_0, Q8_0, Q3_K, Q4_K, Q5_K, Q6_K, IQ2_XXS, IQ3_XXS, IQ2_S = 2, 8, 11, 12, 13, 
 TYPES = {"Q8_0": Q8_0, "Q4_K": Q4_K, "Q6_K": Q6_K, "IQ2_XXS": IQ2_XXS, "IQ3_XXS": IQ3_XXS}
 # types that le_dequant_rows, le_matvec, le_matvec_q8 and le_gemm also accept
 MV_TYPES = dict(TYPES, Q4_0=Q4_0, Q3_K=Q3_K, Q5_K=Q5_K, IQ2_S=IQ2_S)
+# types of activations, scales and logits of the entries that take more than fp32 (GGML ids)
+F32, F16, BF16 = 0, 1, 30
 # (gate/up, down) type pairs of the decode-shaped MoE kernels; every other pair of MV_TYPES runs the
 # grouped form, whose workspace is le_moe_prefill_workspace_size at any token count
 MOE_DECODE_PAIRS = {(Q4_K, Q6_K), (Q4_K, Q4_K), (Q6_K, Q6_K), (Q8_0, Q8_0), (IQ2_XXS, IQ3_XXS), (IQ2_XXS, IQ2_XXS),
@@ -84,6 +86,14 @@ def lib():
         "le_moe_layer_ptrs": (I, [P, I, I, I, P, P, P, I, I, I, I, P, P, I, P, P, P, P, S, P]),
         "le_mm_grouped_workspace_size": (S, [I, I, I, I]),
         "le_mm_grouped": (I, [P, I, P, P, P, P, P, I, I, P, P, I, I, P, S, P]),
+        "le_matvec_g4": (I, [P, P, P, I, I, I, P, LL, I, P, I, P]),
+        "le_moe_route": (I, [P, I, P, I, I, I, P, P, P]),
+        "le_moe_route_bwd": (I, [P, I, P, P, P, I, I, I, P, P]),
+        "le_moe_sort_workspace_size": (S, [I, I, I]),
+        "le_moe_sort": (I, [P, P, I, I, I, P, P, P, P, P, S, P]),
+        "le_moe_permute": (I, [P, I, P, LL, P, I, I, I, P, LL, I, P]),
+        "le_moe_combine": (I, [P, I, P, LL, I, P, P, I, I, I, P, LL, P]),
+        "le_moe_combine_bwd": (I, [P, I, P, LL, P, LL, I, P, P, I, I, I, P, P, P]),
         "le_fill_normal": (None, [P, S, ctypes.c_uint64, ctypes.c_uint64, D, D, I]),
         "le_quantize_rows": (I, [I, P, P, S, S, I]),
         "le_f32_to_f16": (ctypes.c_uint16, [F]),
@@ -158,6 +168,39 @@ def _stream(stream):
     if isinstance(stream, int):
         return stream
     return stream.cuda_stream
+
+
+class _G4(ctypes.Structure):  # le_g4 of include/le_qmm.h
+    _fields_ = [("codes", ctypes.c_void_p), ("scales", ctypes.c_void_p), ("zeros", ctypes.c_void_p), ("n_mat", ctypes.c_int),
+                ("rows", ctypes.c_int), ("cols", ctypes.c_int), ("group", ctypes.c_int), ("scale_type", ctypes.c_int)]
+
+
+class G4:
+    """A stack of n_mat (rows, cols) matrices of 4-bit codes with a scale, and a zero point (None: 8), per `group` columns.
+
+    codes: uint8, two to a byte, the even column in the low half; scales, zeros: F32, F16 or BF16 (told by the tensor's
+    dtype, or scale_type for raw addresses). Holds the tensors as long as it lives; nothing is copied."""
+
+    def __init__(self, codes, scales, zeros, rows, cols, group, n_mat=1, scale_type=None):
+        if scale_type is None:
+            scale_type = dtype_id(scales)
+        if hasattr(zeros, "dtype") and hasattr(scales, "dtype") and zeros.dtype != scales.dtype:
+            raise LeError(-2, "scales and zeros of different types")
+        for t, n in ((codes, rows * cols // 2), (scales, rows * (cols // max(1, group))), (zeros, rows * (cols // max(1, group)))):
+            if hasattr(t, "numel") and (t.numel() != n * n_mat or not t.is_contiguous()):
+                raise LeError(-3, "a tensor of %d values where the %d matrices have %d, contiguous" % (t.numel(), n_mat, n * n_mat))
+        self.tensors = (codes, scales, zeros)
+        self.struct = _G4(_ptr(codes), _ptr(scales), _ptr(zeros), n_mat, rows, cols, group, scale_type)
+        self.ref = ctypes.addressof(self.struct)
+        self.cols = cols
+
+
+def dtype_id(t):
+    """F32, F16 or BF16 of a tensor."""
+    ids = {"torch.float32": F32, "torch.float16": F16, "torch.bfloat16": BF16}
+    if str(t.dtype) not in ids:
+        raise LeError(-2, str(t.dtype))
+    return ids[str(t.dtype)]
 
 
 class Engine:
@@ -274,6 +317,55 @@ class Engine:
         self._check(self._L.le_mm_grouped(self._ctx, ty, _ptr(ptrs), _ptr(w), _ptr(off), _ptr(in_idx), _ptr(out_idx),
                                           nslot, npair, _ptr(x), _ptr(y), rows, cols, _ptr(ws), ws_bytes,
                                           _stream(stream)))
+
+    def mv_g4(self, ty, w, x, out, m=1, slots=1, share=1, sel=None, xstride=None, swiglu=False, stream=None):
+        """Matrix-vector products with 4-bit codes and group scales (w: a G4): out[s][t] = W_sel[s] . x[s // share][t] for m
+        tokens of each slot, x and out of type ty. xstride: values between rows of x (default: rows back to back)."""
+        if xstride is None:
+            xstride = 2 * w.cols if swiglu else w.cols
+        self._check(self._L.le_matvec_g4(self._ctx, w.ref, _ptr(sel), slots, share, ty, _ptr(x), xstride, m, _ptr(out),
+                                         1 if swiglu else 0, _stream(stream)))
+
+    def moe_route(self, ty, logits, n_tok, n_exp, k, idx, w, stream=None):
+        """Top-k experts of each token and their softmax over the selected (ties keep the lower expert; experts at -inf or
+        NaN are never selected: idx -1, weight 0)."""
+        self._check(self._L.le_moe_route(self._ctx, ty, _ptr(logits), n_tok, n_exp, k, _ptr(idx), _ptr(w), _stream(stream)))
+
+    def moe_route_bwd(self, ty, idx, w, dw, n_tok, n_exp, k, dlogits, stream=None):
+        """Gradient of moe_route's weights with respect to all logits."""
+        self._check(self._L.le_moe_route_bwd(self._ctx, ty, _ptr(idx), _ptr(w), _ptr(dw), n_tok, n_exp, k, _ptr(dlogits),
+                                             _stream(stream)))
+
+    def moe_sort_workspace_size(self, n_tok, k, n_exp):
+        return int(self._L.le_moe_sort_workspace_size(n_tok, k, n_exp))
+
+    def moe_sort(self, idx, n_tok, k, n_exp, off, in_idx=None, out_idx=None, pos=None, ws=None, ws_bytes=None, stream=None):
+        """(token, expert) pairs grouped by expert, in pair order within one, as mm_grouped takes them; pos: the place of
+        each pair, -1 for one whose idx is no expert."""
+        if ws is None:
+            n = self.moe_sort_workspace_size(n_tok, k, n_exp)
+            if n:
+                import torch
+                ws = torch.empty(n, dtype=torch.uint8, device="cuda")
+        if ws_bytes is None:
+            ws_bytes = ws.numel() if hasattr(ws, "numel") else 0
+        self._check(self._L.le_moe_sort(self._ctx, _ptr(idx), n_tok, k, n_exp, _ptr(off), _ptr(in_idx), _ptr(out_idx), _ptr(pos),
+                                        _ptr(ws), ws_bytes, _stream(stream)))
+
+    def moe_permute(self, ty, x, pos, n_tok, k, cols, rows, n_row, ldt=None, lde=None, stream=None):
+        """rows[pos[p]] = x[p // k]: tokens copied to expert order. Its gradient is moe_combine without weights."""
+        self._check(self._L.le_moe_permute(self._ctx, ty, _ptr(x), ldt or cols, _ptr(pos), n_tok, k, cols, _ptr(rows), lde or cols,
+                                           n_row, _stream(stream)))
+
+    def moe_combine(self, ty, rows, pos, w, n_tok, k, cols, out, n_row, ldt=None, lde=None, stream=None):
+        """out[t] = sum of w[p] * rows[pos[p]] over the token's pairs (w None: 1; pos None: rows in pair order)."""
+        self._check(self._L.le_moe_combine(self._ctx, ty, _ptr(rows), lde or cols, n_row, _ptr(pos), _ptr(w), n_tok, k, cols,
+                                           _ptr(out), ldt or cols, _stream(stream)))
+
+    def moe_combine_bwd(self, ty, dout, rows, pos, w, n_tok, k, cols, drows, dw, n_row, ldt=None, lde=None, stream=None):
+        """Gradient of moe_combine: drows[pos[p]] = w[p] * dout[t] and dw[p] = dout[t] . rows[pos[p]] (either may be None)."""
+        self._check(self._L.le_moe_combine_bwd(self._ctx, ty, _ptr(dout), ldt or cols, _ptr(rows), lde or cols, n_row, _ptr(pos),
+                                               _ptr(w), n_tok, k, cols, _ptr(drows), _ptr(dw), _stream(stream)))
 
     def moe_check(self, ws, stream=None):
         """Raise LeError(-8) if a one-launch MoE layer on workspace ws gave up at its device-wide
