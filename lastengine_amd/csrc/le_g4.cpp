@@ -1,5 +1,6 @@
 /* Host side of the matrix-vector products with 4-bit codes and group scales (le_matvec_g4, include/le_qmm.h): argument
  * checks and launch shapes. */
+#include <algorithm>
 #include <cstdint>
 #include <cstdio>
 
@@ -11,22 +12,58 @@ namespace {
 int type_bytes(int ty) { return ty == LE_F32 ? 4 : ty == LE_F16 || ty == LE_BF16 ? 2 : 0; }
 bool aligned(const void *p, unsigned n) { return ((uintptr_t)p & (n - 1)) == 0; }
 
+/* One launch: bf16 pieces that hold an activation: 24 bits of fp32 in three, 11 of fp16 in two. SwiGLU's fp32 result: three, or the 16
+ * bits of two where the output is rounded to 11 or 8. */
+int pieces(int xtype, int swiglu) { return xtype == LE_F32 ? 3 : xtype == LE_F16 || swiglu ? 2 : 1; }
+/* ... and the tokens of a slot that it takes (le_g4q_*, four virtual rows). More need the activations laid out in the workspace, as ... */
+int most_tokens(int xtype, int swiglu) { return swiglu ? 1 : 4 / pieces(xtype, 0); }
+/* ... fp16 pieces (le_g4x_*, le_g4m_*). */
+int pieces16(int xtype, int swiglu) { return xtype == LE_F32 || swiglu ? 2 : 1; }
+/* Bytes of one set: fragments, powers of two. */
+size_t frag_bytes(int xtype, int swiglu, int m, int cols) { return (size_t)((cols + 127) / 128) * 256 * pieces16(xtype, swiglu) * m; }
+size_t tile_floats(int m, int cols) { return (size_t)((m + 15) / 16) * ((cols + 127) / 128) * 16; }
+size_t set_bytes(int xtype, int swiglu, int m, int cols) { return frag_bytes(xtype, swiglu, m, cols) + tile_floats(m, cols) * 4; }
+
+
+int scale_block(const le_g4 *w) { return w->group % 128 == 0 || w->group == w->cols ? 128 : w->group % 64 == 0 ? 64 : 32; }
+/* 128-column chunks that a wave of le_g4m_* keeps (two pieces' fragments of four and the sums over small scale blocks would not fit
+ * the registers), and the segments of K that blocks of eight waves make of them. */
+int chunks(const le_g4 *w, int xtype, int swiglu) { return pieces16(xtype, swiglu) == 2 && scale_block(w) == 32 ? 2 : 4; }
+int segments(const le_g4 *w, int xtype, int swiglu) {
+    const int most = 8 * chunks(w, xtype, swiglu);
+    return ((w->cols + 127) / 128 + most - 1) / most;
+}
+/* What is wrong with a shape, or null. */
+const char *shape_error(const le_g4 *w, int slots, int share, int m) {
+    if (w->n_mat <= 0 || w->rows <= 0 || w->cols <= 0 || slots <= 0 || share <= 0 || m <= 0) return "empty shape";
+    if (w->cols % 32) return "cols is not a multiple of 32";
+    if (w->group != w->cols && (w->group < 32 || (w->group & (w->group - 1)) || w->cols % w->group))
+        return "group is neither cols nor a power of two from 32 on that divides cols";
+    if (m > 64 || slots > 65535 || w->cols > 1 << 24) return "m above 64, slots above 65535 or cols above 2^24";
+    if ((long long)slots * m * w->rows > 1LL << 33) return "more than 2^33 results";
+    if ((long long)w->rows * (w->cols / 2) >= 1LL << 32 || (long long)w->rows * (w->cols / w->group) * type_bytes(w->scale_type) >= 1LL << 32)
+        return "a matrix with codes or scales of 4 GiB or more";
+    return nullptr;
+}
+
 }  // namespace
 
+extern "C" size_t le_matvec_g4_workspace_size(const le_g4 *w, int xtype, int m, int slots, int share, int swiglu) {
+    if (!w || !type_bytes(xtype) || !type_bytes(w->scale_type) || shape_error(w, slots, share, m) || m <= most_tokens(xtype, swiglu)) return 0;
+    const int segs = segments(w, xtype, swiglu);
+    return (size_t)((slots + share - 1) / share) * set_bytes(xtype, swiglu, m, w->cols) + (segs > 1 ? (size_t)segs * slots * m * w->rows * 4 : 0);
+}
+
 extern "C" int le_matvec_g4(le_ctx *c, const le_g4 *w, const int *sel, int slots, int share, int xtype, const void *x,
-                            long long xstride, int m, void *y, int swiglu, le_stream_t stream) {
+                            long long xstride, int m, void *y, int swiglu, void *ws, size_t ws_bytes,
+                            le_stream_t stream) {
     if (!c) return LE_ERR_ARG;
     if (!w || !w->codes || !w->scales || !x || !y) return le_ctx_fail(c, LE_ERR_ARG, "null pointer");
     const int xb = type_bytes(xtype), sb = type_bytes(w->scale_type);
     if (!xb) return le_ctx_failf(c, LE_ERR_TYPE, "activations of type %d", xtype);
     if (!sb) return le_ctx_failf(c, LE_ERR_TYPE, "scales of type %d", w->scale_type);
-    if (w->n_mat <= 0 || w->rows <= 0 || w->cols <= 0 || slots <= 0 || share <= 0 || m <= 0)
-        return le_ctx_fail(c, LE_ERR_SHAPE, "empty shape");
-    if (w->cols % 32) return le_ctx_failf(c, LE_ERR_SHAPE, "cols=%d is not a multiple of 32", w->cols);
-    if (w->group != w->cols && (w->group < 32 || (w->group & (w->group - 1)) || w->cols % w->group))
-        return le_ctx_failf(c, LE_ERR_SHAPE, "group=%d is neither cols nor a power of two from 32 on that divides cols=%d", w->group, w->cols);
-    if (m > 64 || slots > 65535) return le_ctx_failf(c, LE_ERR_SHAPE, "m=%d above 64 or slots=%d above 65535", m, slots);
-    if (w->rows > 1 << 27) return le_ctx_failf(c, LE_ERR_SHAPE, "rows=%d above 2^27", w->rows);
+    if (const char *e = shape_error(w, slots, share, m))
+        return le_ctx_failf(c, LE_ERR_SHAPE, "%s (%d matrices of %d x %d, group %d; %d slots, %d sharing, %d tokens)", e, w->n_mat, w->rows, w->cols, w->group, slots, share, m);
     if (!sel && slots > w->n_mat) return le_ctx_failf(c, LE_ERR_SHAPE, "%d slots of %d matrices without sel", slots, w->n_mat);
     const long long width = swiglu ? 2LL * w->cols : w->cols;
     if (xstride && xstride < width) return le_ctx_failf(c, LE_ERR_SHAPE, "xstride=%lld is less than a row of %lld", xstride, width);
@@ -34,6 +71,10 @@ extern "C" int le_matvec_g4(le_ctx *c, const le_g4 *w, const int *sel, int slots
         return le_ctx_fail(c, LE_ERR_ALIGN, "codes, x and its rows must be 16-byte aligned");
     if (!aligned(w->scales, sb) || !aligned(w->zeros, sb) || !aligned(y, xb) || !aligned(sel, 4))
         return le_ctx_fail(c, LE_ERR_ALIGN, "scales, zeros, sel and y must be aligned to their types");
+    const size_t need = le_matvec_g4_workspace_size(w, xtype, m, slots, share, swiglu);
+    if (need && (!ws || ws_bytes < need)) return le_ctx_failf(c, LE_ERR_WORKSPACE, "workspace needs %zu bytes", need);
+    if (need && !aligned(ws, 16)) return le_ctx_fail(c, LE_ERR_ALIGN, "ws must be 16-byte aligned");
+    if (need && (long long)((slots + share - 1) / share) * m > 65535) return le_ctx_fail(c, LE_ERR_SHAPE, "more than 65535 tokens");
     if (int rc = le_ctx_on_device(c)) return rc;
     G4Args a{};
     a.codes = (const unsigned char *)w->codes;
@@ -50,9 +91,53 @@ extern "C" int le_matvec_g4(le_ctx *c, const le_g4 *w, const int *sel, int slots
     a.ng = w->cols / w->group;
     a.share = share;
     a.m = m;
+    a.gshift = 31; /* one group a row */
+    if (w->group != w->cols)
+        for (a.gshift = 5; 1 << a.gshift < w->group;) a.gshift++;
+    a.xty = xtype;
+    a.sty = w->scale_type;
+    const int sub = scale_block(w), bpc = 128 / sub;
+    a.vec = bpc > 1 && a.ng % bpc == 0 && aligned(w->scales, bpc * sb) && aligned(w->zeros, bpc * sb);
+    const char *kind = xtype == LE_F32 ? "f32" : xtype == LE_F16 ? "f16" : "bf16";
+    const long long groups = (w->rows + 15) / 16;
+    const int most = most_tokens(xtype, swiglu), sb2 = sb == 4 ? 4 : 2, P = pieces(xtype, swiglu);
     char name[48];
-    snprintf(name, sizeof name, "le_g4_x%d_s%d_%s", xtype, w->scale_type, swiglu ? "swiglu" : "plain");
     void *args[] = {&a};
-    return le_ctx_launch(c, name, dim3((unsigned)((w->rows + 15) / 16), (unsigned)slots, (unsigned)m), 256, 0,
-                         (hipStream_t)stream, args);
+    /* Row groups a block: so many that blocks of nw waves fill the chip with `waves` a CU, and LDS holds their partial results (lds bytes
+     * a wave and group). */
+    auto share_out = [&](int nw, int waves, long long others, int lds) {
+        const long long target = (long long)le_ctx_cus(c) * std::max(1, waves / nw);
+        long long per = (groups * others + target - 1) / target;
+        per = std::max(1LL, std::min<long long>({per, groups, 64 * 1024 / ((long long)nw * lds)}));
+        const long long gx = (groups + per - 1) / per;
+        a.nw = nw;
+        a.gx = (int)gx;
+        a.per = (int)((groups + gx - 1) / gx);
+        a.full = (int)(groups - (a.per - 1) * gx);
+    };
+    if (m <= most) {
+        const int ns = (w->cols + 511) / 512, wmax = ns <= 8 || sub < 128 ? 8 : 16; /* slices of 512 columns */
+        const int passes = (ns + wmax - 1) / wmax, nw = (ns + passes - 1) / passes, T = m == 1 ? 1 : most;
+        const int quad = m == 1 && P > 1 ? nw * 4096 : 0;
+        share_out(nw, 16, slots, T * 256);
+        snprintf(name, sizeof name, "le_g4q_%s%s_s%d_b%d%s", kind, swiglu ? "w" : m == 1 ? "" : T == 2 ? "t2" : "t4", sb2, sub, passes > 1 || nw > 8 ? "_mp" : "");
+        return le_ctx_launch(c, name, dim3((unsigned)a.gx, (unsigned)slots), 64 * nw, (size_t)quad + (size_t)a.per * nw * T * 256, (hipStream_t)stream, args);
+    }
+    a.ws = (unsigned char *)ws;
+    a.ws_set = (long long)set_bytes(xtype, swiglu, m, w->cols);
+    a.ws_downs = (long long)frag_bytes(xtype, swiglu, m, w->cols);
+    a.segs = segments(w, xtype, swiglu);
+    const int sets = (slots + share - 1) / share, nc = (w->cols + 127) / 128, tiles = (m + 15) / 16, cs = chunks(w, xtype, swiglu);
+    a.part = (float *)(a.ws + sets * a.ws_set);
+    a.total = (long long)slots * m * w->rows;
+    snprintf(name, sizeof name, "le_g4x_%s%s_b%d", kind, swiglu ? "w" : "", sub);
+    int rc = le_ctx_launch(c, name, dim3((unsigned)((nc * 16 + 255) / 256), (unsigned)(sets * m)), 256, 0, (hipStream_t)stream, args);
+    if (rc) return rc;
+    /* waves: all of K's slices over the segments, evenly */
+    const int nw = ((nc + cs - 1) / cs + a.segs - 1) / a.segs;
+    share_out(nw, 8, (long long)slots * tiles * a.segs, 1024);
+    snprintf(name, sizeof name, "le_g4m_p%d_s%d_b%d", pieces16(xtype, swiglu), sb2, sub);
+    rc = le_ctx_launch(c, name, dim3((unsigned)a.gx, (unsigned)slots, (unsigned)(tiles * a.segs)), 64 * nw, (size_t)a.per * nw * 1024, (hipStream_t)stream, args);
+    if (rc || a.segs == 1) return rc;
+    return le_ctx_launch(c, "le_g4s", dim3((unsigned)((a.total + 1023) / 1024)), 256, 0, (hipStream_t)stream, args);
 }

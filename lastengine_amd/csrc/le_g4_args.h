@@ -1,4 +1,4 @@
-/* Kernel argument block of le_g4_*, shared by host (le_g4.cpp) and device (le_g4_kernels.hip). */
+/* Kernel argument block of le_g4*, shared by host (le_g4.cpp) and device (le_g4_kernels.hip). */
 #pragma once
 
 struct G4Args {
@@ -9,4 +9,13 @@ struct G4Args {
     void *y;
     long long xstride; /* values */
     int n_mat, rows, cols, group, ng /* groups a row */, share, m;
+    int gshift;        /* column >> gshift = group */
+    int xty, sty, vec;     /* types of x and y, of the scales; a 128-column part's scales and zeros can be loaded at once */
+    int nw, gx;        /* waves of a block, blocks of a slot (from here: the launch's own cost a load each) */
+    unsigned char *ws; /* le_g4x_*, le_g4m_*: fragments of a set of m tokens and their sums */
+    long long ws_set, ws_downs; /* bytes of a set, before its powers of two */
+    float *part;               /* [segment of K][value of y], where there are several segments */
+    long long total;           /* values of y */
+    int segs;
+    int per, full;     /* row groups of the blocks below `full`; the others have one less */
 };

@@ -86,7 +86,8 @@ def lib():
         "le_moe_layer_ptrs": (I, [P, I, I, I, P, P, P, I, I, I, I, P, P, I, P, P, P, P, S, P]),
         "le_mm_grouped_workspace_size": (S, [I, I, I, I]),
         "le_mm_grouped": (I, [P, I, P, P, P, P, P, I, I, P, P, I, I, P, S, P]),
-        "le_matvec_g4": (I, [P, P, P, I, I, I, P, LL, I, P, I, P]),
+        "le_matvec_g4": (I, [P, P, P, I, I, I, P, LL, I, P, I, P, S, P]),
+        "le_matvec_g4_workspace_size": (S, [P, I, I, I, I, I]),
         "le_moe_route": (I, [P, I, P, I, I, I, P, P, P]),
         "le_moe_route_bwd": (I, [P, I, P, P, P, I, I, I, P, P]),
         "le_moe_sort_workspace_size": (S, [I, I, I]),
@@ -168,6 +169,17 @@ def _stream(stream):
     if isinstance(stream, int):
         return stream
     return stream.cuda_stream
+
+
+def _workspace(n, stream):
+    """n bytes of device memory for one call on `stream` (None: none needed), not reused before that call is done."""
+    if not n:
+        return None
+    import torch
+    ws = torch.empty(n, dtype=torch.uint8, device="cuda")
+    if stream is not None:
+        ws.record_stream(torch.cuda.ExternalStream(stream) if isinstance(stream, int) else stream)
+    return ws
 
 
 class _G4(ctypes.Structure):  # le_g4 of include/le_qmm.h
@@ -318,13 +330,20 @@ class Engine:
                                           nslot, npair, _ptr(x), _ptr(y), rows, cols, _ptr(ws), ws_bytes,
                                           _stream(stream)))
 
-    def mv_g4(self, ty, w, x, out, m=1, slots=1, share=1, sel=None, xstride=None, swiglu=False, stream=None):
+    def mv_g4_workspace_size(self, ty, w, m, slots=1, share=1, swiglu=False):
+        return int(self._L.le_matvec_g4_workspace_size(w.ref, ty, m, slots, share, 1 if swiglu else 0))
+
+    def mv_g4(self, ty, w, x, out, m=1, slots=1, share=1, sel=None, xstride=None, swiglu=False, ws=None, ws_bytes=None, stream=None):
         """Matrix-vector products with 4-bit codes and group scales (w: a G4): out[s][t] = W_sel[s] . x[s // share][t] for m
         tokens of each slot, x and out of type ty. xstride: values between rows of x (default: rows back to back)."""
         if xstride is None:
             xstride = 2 * w.cols if swiglu else w.cols
+        if ws is None and m > 1:
+            ws = _workspace(self.mv_g4_workspace_size(ty, w, m, slots, share, swiglu), stream)
+        if ws_bytes is None:
+            ws_bytes = ws.numel() if hasattr(ws, "numel") else 0
         self._check(self._L.le_matvec_g4(self._ctx, w.ref, _ptr(sel), slots, share, ty, _ptr(x), xstride, m, _ptr(out),
-                                         1 if swiglu else 0, _stream(stream)))
+                                         1 if swiglu else 0, _ptr(ws), ws_bytes, _stream(stream)))
 
     def moe_route(self, ty, logits, n_tok, n_exp, k, idx, w, stream=None):
         """Top-k experts of each token and their softmax over the selected (ties keep the lower expert; experts at -inf or
@@ -343,10 +362,7 @@ class Engine:
         """(token, expert) pairs grouped by expert, in pair order within one, as mm_grouped takes them; pos: the place of
         each pair, -1 for one whose idx is no expert."""
         if ws is None:
-            n = self.moe_sort_workspace_size(n_tok, k, n_exp)
-            if n:
-                import torch
-                ws = torch.empty(n, dtype=torch.uint8, device="cuda")
+            ws = _workspace(self.moe_sort_workspace_size(n_tok, k, n_exp), stream)
         if ws_bytes is None:
             ws_bytes = ws.numel() if hasattr(ws, "numel") else 0
         self._check(self._L.le_moe_sort(self._ctx, _ptr(idx), n_tok, k, n_exp, _ptr(off), _ptr(in_idx), _ptr(out_idx), _ptr(pos),

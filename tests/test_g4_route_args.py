@@ -50,7 +50,7 @@ def lib(tmp_path_factory):
                     "-I" + os.path.join(REPO, "include"), str(d / "stub.cpp")] + [os.path.join(build.CSRC, f) for f in ("le_g4.cpp", "le_route.cpp")] +
                    ["-o", so], check=True)
     L, real = ctypes.CDLL(so), qmm.lib()
-    for name in ("le_matvec_g4", "le_moe_route", "le_moe_route_bwd", "le_moe_sort", "le_moe_sort_workspace_size", "le_moe_permute", "le_moe_combine",
+    for name in ("le_matvec_g4", "le_matvec_g4_workspace_size", "le_moe_route", "le_moe_route_bwd", "le_moe_sort", "le_moe_sort_workspace_size", "le_moe_permute", "le_moe_combine",
                  "le_moe_combine_bwd"):
         getattr(L, name).restype, getattr(L, name).argtypes = getattr(real, name).restype, getattr(real, name).argtypes
     return L
@@ -65,9 +65,9 @@ A = 0x10000  # an aligned address; nothing is read there
 
 
 def g4(L, c, codes=A, scales=A, zeros=A, n_mat=4, rows=64, cols=256, group=64, stype=1, sel=A, slots=2, share=1, xtype=0, x=A, xstride=256, m=1,
-       y=A, swiglu=0, w=True):
+       y=A, swiglu=0, w=True, ws=A, ws_bytes=1 << 40):
     s = qmm._G4(codes, scales, zeros, n_mat, rows, cols, group, stype)
-    return L.le_matvec_g4(ctypes.addressof(c), ctypes.addressof(s) if w else None, sel, slots, share, xtype, x, xstride, m, y, swiglu, None)
+    return L.le_matvec_g4(ctypes.addressof(c), ctypes.addressof(s) if w else None, sel, slots, share, xtype, x, xstride, m, y, swiglu, ws, ws_bytes, None)
 
 
 @pytest.mark.parametrize("bad,code", [
@@ -76,24 +76,42 @@ def g4(L, c, codes=A, scales=A, zeros=A, n_mat=4, rows=64, cols=256, group=64, s
     (dict(rows=0), -3), (dict(cols=0), -3), (dict(n_mat=0), -3), (dict(slots=0), -3), (dict(share=0), -3), (dict(m=0), -3), (dict(m=65), -3),
     (dict(rows=-5), -3), (dict(slots=65536), -3), (dict(cols=250, group=250), -3), (dict(cols=48, group=48), -3), (dict(group=16), -3),
     (dict(group=96, cols=192), -3), (dict(group=512), -3), (dict(group=0), -3), (dict(group=-64), -3), (dict(sel=None, slots=5), -3),
-    (dict(xstride=255), -3), (dict(xstride=-256), -3), (dict(swiglu=1, xstride=256), -3), (dict(rows=2**31 - 1, n_mat=1), -3),
+    (dict(xstride=255), -3), (dict(xstride=-256), -3), (dict(swiglu=1, xstride=256), -3), (dict(rows=2**31 - 1, n_mat=1), -3), (dict(rows=2**25, n_mat=1), -3), (dict(cols=2**25, group=2**25, xstride=2**25), -3),
+    (dict(rows=2**28, cols=32, group=32, stype=0), -3), (dict(rows=2**28, cols=32, group=32), -3), (dict(m=2, slots=40000, n_mat=40000, sel=None), -3),
+    (dict(m=2, ws=None), -7), (dict(m=2, ws_bytes=2 * 256 * 2), -7), (dict(m=5, xtype=30, ws=None), -7), (dict(m=2, swiglu=1, xstride=512, ws_bytes=99), -7),
+    (dict(m=2, ws=A + 8), -4),
     (dict(codes=A + 8), -4), (dict(x=A + 4), -4), (dict(xstride=258), -4), (dict(xtype=1, xstride=260), -4), (dict(scales=A + 1), -4),
     (dict(zeros=A + 1), -4), (dict(stype=0, scales=A + 2), -4), (dict(y=A + 2), -4), (dict(sel=A + 2), -4)])
 def test_g4_refusals(lib, ctx, bad, code):
     assert g4(lib, ctx, **bad) == code
     assert ctx.launches == 0 and ctx.err
-    assert lib.le_matvec_g4(None, None, None, 1, 1, 0, None, 0, 1, None, 0, None) == -1
+    assert lib.le_matvec_g4(None, None, None, 1, 1, 0, None, 0, 1, None, 0, None, 0, None) == -1
 
 
 @pytest.mark.parametrize("good", [
     dict(), dict(zeros=None), dict(sel=None), dict(xstride=0), dict(group=256), dict(cols=96, group=96), dict(cols=96, group=32), dict(cols=32, group=32),
-    dict(m=64), dict(slots=65535), dict(swiglu=1, xstride=512), dict(xtype=30, stype=30, y=A + 2, scales=A + 2), dict(rows=1), dict(rows=2**27, n_mat=1),
+    dict(m=64), dict(slots=65535), dict(swiglu=1, xstride=512), dict(xtype=30, stype=30, y=A + 2, scales=A + 2), dict(rows=1), dict(rows=2**24, n_mat=1), dict(m=4, xtype=30, ws=None), dict(m=2, xtype=1, ws=None), dict(m=64, cols=2**20, group=2**20, xstride=2**20), dict(m=17, slots=900, cols=14336, xstride=14336),
     dict(cols=2**20, group=2**20, xstride=2**20)])
 def test_g4_launches(lib, ctx, good):
     assert g4(lib, ctx, **good) == 0, ctx.err
-    assert 1 <= ctx.launches <= 2
+    assert 1 <= ctx.launches <= 3
     for name, g, block, lds in ctx.calls():
         assert g[0] * block < 2**32 and g[1] <= 65535 and g[2] <= 65535 and min(g) > 0 and lds <= 160 * 1024, (name, g, block, lds)
+
+
+def test_g4_workspace(lib):
+    def f(xtype, m, cols, slots, share, swiglu, rows=64, group=64, w=True):
+        s = qmm._G4(A, A, A, 4, rows, cols, group, 1)
+        return lib.le_matvec_g4_workspace_size(ctypes.addressof(s) if w else None, xtype, m, slots, share, swiglu)
+
+    assert f(0, 1, 4096, 8, 1, 1) == 0 and f(30, 4, 4096, 1, 1, 0) == 0 and f(1, 2, 4096, 1, 1, 0) == 0  # one launch
+    assert f(0, 2, 4096, 1, 1, 0) >= 2 * 4096 * 4 and f(30, 5, 4096, 1, 1, 0) >= 5 * 4096 * 2 and f(1, 3, 4096, 1, 1, 0) >= 3 * 4096 * 2
+    assert f(0, 2, 4096, 8, 2, 0) == 4 * f(0, 2, 4096, 1, 1, 0)  # sets of activations
+    assert f(0, 2, 14336, 3, 1, 0, rows=128) >= 3 * 2 * 14336 * 4 + 4 * 3 * 2 * 128 * 4  # and the partial results of K's segments
+    assert f(0, 2, 4096, 3, 1, 0, rows=128, group=32) >= 3 * 2 * 4096 * 4 + 2 * 3 * 2 * 128 * 4
+    for bad in ((8, 2, 4096, 1, 1, 0), (0, 0, 4096, 1, 1, 0), (0, 65, 4096, 1, 1, 0), (0, 2, 100, 1, 1, 0), (0, 2, 4096, 0, 1, 0), (0, 2, 4096, 1, 0, 0)):
+        assert f(*bad) == 0
+    assert f(0, 2, 4096, 1, 1, 0, w=False) == 0
 
 
 def test_other_device(lib, ctx):
