@@ -3,6 +3,7 @@
 #include <algorithm>
 #include <cstdint>
 #include <cstdio>
+#include <cstring>
 
 #include "le_ctx.h"
 #include "le_route_args.h"
@@ -31,6 +32,20 @@ int check_rows(le_ctx *c, int ty, long long ldt, long long lde, int n_tok, int k
     return LE_OK;
 }
 
+/* How le_rt_sort takes np pairs: one block up to 4096 of them, else at most 256 blocks of 16 waves. */
+struct SortShape {
+    int blocks = 1, waves, steps;
+    explicit SortShape(int np) {
+        waves = std::max(1, (int)std::min(16LL, (np + 63LL) / 64));
+        const int one = (int)((np + 1023LL) / 1024); /* steps of one block */
+        steps = std::max(1, one);
+        if (np > 4096) {
+            steps = (one + 255) / 256;
+            blocks = (int)((np + 1024LL * steps - 1) / (1024LL * steps));
+        }
+    }
+};
+
 }  // namespace
 
 extern "C" {
@@ -48,9 +63,11 @@ int le_moe_route(le_ctx *c, int ltype, const void *logits, int n_tok, int n_exp,
     if (int rc = le_ctx_on_device(c)) return rc;
     RouteArgs a{logits, idx, w, n_tok, n_exp, k};
     void *args[] = {&a};
-    char name[32];
-    snprintf(name, sizeof name, "le_rt_route_%d", ltype);
-    return le_ctx_launch(c, name, dim3((unsigned)std::min((n_tok + 3LL) / 4, 1LL << 20)), 256, 0, (hipStream_t)stream, args);
+    /* lanes a token and experts a lane: the fewest lanes that hold the experts in eight values each */
+    const int L = n_exp <= 128 ? 16 : n_exp <= 256 ? 32 : 64, V = n_exp <= 32 ? 2 : n_exp <= 64 ? 4 : n_exp <= 512 ? 8 : 16;
+    char name[40];
+    snprintf(name, sizeof name, "le_rt_route_%d_l%d_v%d", ltype, L, V);
+    return le_ctx_launch(c, name, dim3((unsigned)std::min((n_tok * (long long)L + 255) / 256, 1LL << 20)), 256, 0, (hipStream_t)stream, args);
 }
 
 int le_moe_route_bwd(le_ctx *c, int ltype, const int *idx, const float *w, const float *dw, int n_tok, int n_exp, int k,
@@ -69,12 +86,13 @@ int le_moe_route_bwd(le_ctx *c, int ltype, const int *idx, const float *w, const
     void *args[] = {&a};
     char name[32];
     snprintf(name, sizeof name, "le_rt_route_bwd_%d", ltype);
-    return le_ctx_launch(c, name, dim3((unsigned)std::min((n_tok + 3LL) / 4, 1LL << 20)), 256, 0, (hipStream_t)stream, args);
+    return le_ctx_launch(c, name, dim3((unsigned)std::min((n_tok + 15LL) / 16, 1LL << 20)), 256, 0, (hipStream_t)stream, args);
 }
 
 size_t le_moe_sort_workspace_size(int n_tok, int k, int n_exp) {
-    (void)n_tok, (void)k, (void)n_exp;
-    return 0;
+    if (n_tok < 0 || k <= 0 || k > 16 || (long long)n_tok * k > 0x7FFFFFFFLL || n_exp <= 0 || n_exp > 1024) return 0;
+    const SortShape s(n_tok * k);
+    return s.blocks > 1 ? (size_t)s.blocks * n_exp * 4 : 0;
 }
 
 int le_moe_sort(le_ctx *c, const int *idx, int n_tok, int k, int n_exp, int *off, int *in_idx, int *out_idx, int *pos,
@@ -88,18 +106,27 @@ int le_moe_sort(le_ctx *c, const int *idx, int n_tok, int k, int n_exp, int *off
     const size_t need = le_moe_sort_workspace_size(n_tok, k, n_exp);
     if (need && (!ws || ws_bytes < need)) return le_ctx_failf(c, LE_ERR_WORKSPACE, "workspace needs %zu bytes", need);
     if (int rc = le_ctx_on_device(c)) return rc;
-    SortArgs a{idx, off, in_idx, out_idx, pos, n_tok * k, k, n_exp};
+    const SortShape s(n_tok * k);
+    SortArgs a{idx, off, in_idx, out_idx, pos, n_tok * k, k, n_exp, s.blocks, s.waves, s.steps, (int *)ws};
     void *args[] = {&a};
-    return le_ctx_launch(c, "le_rt_sort", dim3((unsigned)n_exp + 1), 256, 0, (hipStream_t)stream, args);
+    if (s.blocks > 1)
+        if (int rc = le_ctx_launch(c, "le_rt_count", dim3((unsigned)s.blocks), 64 * s.waves, (size_t)n_exp * 4, (hipStream_t)stream, args)) return rc;
+    return le_ctx_launch(c, "le_rt_sort", dim3((unsigned)s.blocks), 64 * s.waves, ((size_t)(s.waves + 2) * n_exp + 16) * 4, (hipStream_t)stream, args);
 }
 
 static int rows_launch(le_ctx *c, const char *what, int ty, const RowsArgs &rows, le_stream_t stream) {
     if (int rc = le_ctx_on_device(c)) return rc;
     RowsArgs a = rows;
     void *args[] = {&a};
-    char name[32];
-    snprintf(name, sizeof name, "le_rt_%s_%d", what, ty);
-    return le_ctx_launch(c, name, dim3((unsigned)std::min(a.n_tok, 1 << 20)), 256, 0, (hipStream_t)stream, args);
+    /* lanes a token: as many as its row has 16-byte parts, of 16, 64 and 256; longer rows are cut over the grid's second axis where
+     * nothing is summed over a row */
+    const int n = ty == LE_F32 ? 4 : 8, parts = (a.cols + n - 1) / n, L = parts <= 16 ? 16 : parts <= 64 ? 64 : 256;
+    const bool whole = !strcmp(what, "combine_bwd");
+    if (!whole && (parts + L - 1) / L > 65535) return le_ctx_failf(c, LE_ERR_SHAPE, "cols=%d", a.cols);
+    char name[40];
+    snprintf(name, sizeof name, "le_rt_%s_%d_l%d", what, ty, L);
+    return le_ctx_launch(c, name, dim3((unsigned)std::min((a.n_tok * (long long)L + 255) / 256, 1LL << 20), whole ? 1u : (unsigned)((parts + L - 1) / L)), 256, 0,
+                         (hipStream_t)stream, args);
 }
 
 int le_moe_permute(le_ctx *c, int ty, const void *x, long long ldt, const int *pos, int n_tok, int k, int cols, void *e,

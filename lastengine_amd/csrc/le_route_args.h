@@ -17,6 +17,8 @@ struct SortArgs {
     const int *idx;
     int *off, *in_idx, *out_idx, *pos; /* all but off may be null */
     int np, k, n_exp;
+    int blocks, waves, steps; /* a wave takes 64 * steps pairs */
+    int *ws;                  /* [block][expert] counts, where there are several blocks */
 };
 struct RowsArgs {
     const void *src;  /* permute: x; combine: e; backward: dout */

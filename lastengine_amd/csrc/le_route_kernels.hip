@@ -4,178 +4,407 @@
 #include "le_f32_types.h"
 #include "le_route_args.h"
 
-static __device__ __forceinline__ float wave_sum(float v) {
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
-    return v;
+static __device__ __forceinline__ int as_int(float v) { return __builtin_bit_cast(int, v); }
+static __device__ __forceinline__ float as_float(int v) { return __builtin_bit_cast(float, v); }
+
+/* The value of the lane D away (1, 2), or of the mirrored lane of the 8 (4) or 16 (8) where all lanes of a 4 or 8 hold the same value by
+ * then, or of the row or half 16 or 32 away: the steps of a butterfly over up to 64 lanes without LDS. */
+template <int D> static __device__ __forceinline__ int across(int v) {
+    if constexpr (D == 1) return __builtin_amdgcn_mov_dpp(v, 0xB1, 0xf, 0xf, true);
+    else if constexpr (D == 2) return __builtin_amdgcn_mov_dpp(v, 0x4E, 0xf, 0xf, true);
+    else if constexpr (D == 4) return __builtin_amdgcn_mov_dpp(v, 0x141, 0xf, 0xf, true);
+    else if constexpr (D == 8) return __builtin_amdgcn_mov_dpp(v, 0x140, 0xf, 0xf, true);
+    else if constexpr (D == 16) {
+        const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+        return threadIdx.x & 16 ? r[0] : r[1];
+    } else {
+        const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+        return threadIdx.x & 32 ? r[0] : r[1];
+    }
+}
+/* Sum over groups of L lanes, in every lane of them. */
+template <int L, int D = 1> static __device__ __forceinline__ float group_sum(float v) {
+    if constexpr (D < L) {
+        v += as_float(across<D>(as_int(v)));
+        return group_sum<L, 2 * D>(v);
+    } else {
+        return v;
+    }
+}
+/* Largest value and, of equal ones, the lowest index over groups of L lanes. */
+template <int L, int D = 1> static __device__ __forceinline__ void group_argmax(float &v, int &i) {
+    if constexpr (D < L) {
+        const float ov = as_float(across<D>(as_int(v)));
+        const int oi = across<D>(i);
+        const bool take = ov > v || (ov == v && oi < i);
+        v = take ? ov : v;
+        i = take ? oi : i;
+        group_argmax<L, 2 * D>(v, i);
+    }
 }
 
-/* Top-k by one wave per token: lane l holds experts l, l + 64, ...; k rounds of a wave-wide maximum, the lowest expert of equal
- * ones first. Lane s < k keeps selection s. */
-template <int TY> __device__ __forceinline__ void route_body(const RouteArgs &a, int t) {
-    const int lane = threadIdx.x & 63;
-    const typename XT<TY>::raw *l = (const typename XT<TY>::raw *)a.logits + (size_t)t * a.n_exp;
-    float v[16];
+/* ---- router ----
+ * Top-k by groups of L lanes, a token each, lane l holding experts l, l + L, ... (V of them): k rounds of an argmax, first in the
+ * lane, then over the group by DPP. Lane s < k keeps selection s. Reads the logits once and is bound by the rounds' instructions:
+ * with 16 lanes a token a wave's rounds serve four tokens. */
+template <int TY, int L, int V> __device__ __forceinline__ void route_body(const RouteArgs &a) {
+    const int l = threadIdx.x & (L - 1);
+    for (long long t0 = (long long)blockIdx.x * (256 / L); t0 < a.n_tok; t0 += (long long)gridDim.x * (256 / L)) {
+        const long long t = t0 + threadIdx.x / L;
+        const bool there = t < a.n_tok; /* lanes of a token behind the last go along, and write nothing */
+        const typename XT<TY>::raw *lg = (const typename XT<TY>::raw *)a.logits + (there ? t : a.n_tok - 1) * a.n_exp;
+        float v[V];
 #pragma unroll
-    for (int j = 0; j < 16; j++) {
-        const int e = 64 * j + lane;
-        const float x = e < a.n_exp ? XT<TY>::up(l[e]) : -INFINITY;
-        v[j] = x == x ? x : -INFINITY;
+        for (int j = 0; j < V; j++) {
+            const int e = l + L * j;
+            const float x = e < a.n_exp ? XT<TY>::up(lg[e]) : -INFINITY;
+            v[j] = x == x ? x : -INFINITY;
+        }
+        int my_e = -1;
+        float my_v = -INFINITY;
+        for (int r = 0; r < a.k; r++) {
+            float mx = v[0];
+            int e = l;
+#pragma unroll
+            for (int j = 1; j < V; j++) {
+                e = v[j] > mx ? l + L * j : e;
+                mx = fmaxf(mx, v[j]);
+            }
+            group_argmax<L>(mx, e);
+            const bool found = mx > -INFINITY;
+#pragma unroll
+            for (int j = 0; j < V; j++) v[j] = e == l + L * j ? -INFINITY : v[j];
+            my_e = l == r && found ? e : my_e;
+            my_v = l == r && found ? mx : my_v;
+        }
+        const float top = as_float(__builtin_amdgcn_ds_bpermute((threadIdx.x & 63 & ~(L - 1)) * 4, as_int(my_v)));
+        const float ex = my_e >= 0 ? expf(my_v - top) : 0.f;
+        const float tot = group_sum<L>(ex);
+        if (there && l < a.k) {
+            a.idx[t * a.k + l] = my_e;
+            a.w[t * a.k + l] = my_e >= 0 ? ex / tot : 0.f;
+        }
     }
-    int my_e = -1;
-    float my_v = -INFINITY;
-    for (int r = 0; r < a.k; r++) {
-        float mx = v[0];
-#pragma unroll
-        for (int j = 1; j < 16; j++) mx = fmaxf(mx, v[j]);
-        for (int o = 32; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
-        if (!(mx > -INFINITY)) break; /* uniform */
+}
+
+/* Gradient: the token's selections in lanes s < k of a group of 16, each value then added where its expert is: no scatter, every logit written
+ * once. */
+template <int TY> __device__ __forceinline__ void route_bwd_body(const RouteBwdArgs &a) {
+    const int l = threadIdx.x & 15, base = threadIdx.x & 48;
+    for (long long t0 = (long long)blockIdx.x * 16; t0 < a.n_tok; t0 += (long long)gridDim.x * 16) {
+        const long long t = t0 + threadIdx.x / 16;
+        const bool there = t < a.n_tok;
         int e = -1;
+        float w = 0.f, dw = 0.f;
+        if (there && l < a.k) {
+            e = a.idx[t * a.k + l];
+            if (e < 0 || e >= a.n_exp) e = -1;
+            if (e >= 0) w = a.w[t * a.k + l], dw = a.dw[t * a.k + l];
+        }
+        const float g = w * (dw - group_sum<16>(w * dw));
+        typename XT<TY>::raw *d = (typename XT<TY>::raw *)a.dlogits + t * a.n_exp;
+        for (int e0 = 0; e0 < a.n_exp; e0 += 64) {
+            float v[4] = {0.f, 0.f, 0.f, 0.f};
+            for (int s = 0; s < a.k; s++) {
+                const int es = __builtin_amdgcn_ds_bpermute((base + s) * 4, e) - e0 - l;
+                const float gs = as_float(__builtin_amdgcn_ds_bpermute((base + s) * 4, as_int(g)));
 #pragma unroll
-        for (int j = 0; j < 16; j++) {
-            const unsigned long long b = __ballot(v[j] == mx);
-            if (e < 0 && b) {
-                const int wl = __ffsll((long long)b) - 1;
-                e = 64 * j + wl;
-                v[j] = lane == wl ? -INFINITY : v[j];
+                for (int j = 0; j < 4; j++) v[j] += es == 16 * j ? gs : 0.f;
+            }
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                if (there && e0 + l + 16 * j < a.n_exp) d[e0 + l + 16 * j] = XT<TY>::down(v[j]);
+        }
+    }
+}
+
+/* ---- sort ----
+ * A stable counting sort. A block takes a run of the pairs, each of its waves 64 J of them in a row (lane, then step), so that pair
+ * order is (block, wave, step, lane) order. Counts per wave and expert in LDS give every wave its first place for every expert; a
+ * pair's place is that, the wave's pairs of the expert in earlier steps, and those in lower lanes of the step, which ballots
+ * over the bits of the expert's number find. One block does all of up to 4096 pairs; more run as two launches, the first of which
+ * writes every block's counts to the workspace (at most 256 blocks, so that each can add up what all have). */
+static __device__ __forceinline__ int expert_of(const SortArgs &a, long long p) {
+    if (p >= a.np) return -2; /* no pair */
+    const int e = a.idx[p];
+    return e >= 0 && e < a.n_exp ? e : -1;
+}
+extern "C" __global__ void __launch_bounds__(1024) le_rt_count(SortArgs a) {
+    extern __shared__ int hist[];
+    for (int e = threadIdx.x; e < a.n_exp; e += blockDim.x) hist[e] = 0;
+    __syncthreads();
+    const long long p0 = ((long long)blockIdx.x * a.waves + (threadIdx.x >> 6)) * 64 * a.steps + (threadIdx.x & 63);
+#pragma unroll 4
+    for (int j = 0; j < a.steps; j++) {
+        const int e = expert_of(a, p0 + 64ll * j);
+        if (e >= 0) atomicAdd(&hist[e], 1);
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < a.n_exp; e += blockDim.x) a.ws[blockIdx.x * a.n_exp + e] = hist[e];
+}
+extern "C" __global__ void __launch_bounds__(1024) le_rt_sort(SortArgs a) {
+    extern __shared__ int hist[]; /* [wave][expert], then [expert] all pairs, [expert] those of earlier blocks, [16] */
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, nt = 64 * a.waves, ne = a.n_exp;
+    int *all = hist + a.waves * ne, *before = all + ne, *wsum = before + ne;
+    for (int i = threadIdx.x; i < a.waves * ne + 2 * ne; i += nt) hist[i] = 0;
+    const long long p0 = ((long long)blockIdx.x * a.waves + wave) * 64 * a.steps + lane;
+    int first = expert_of(a, p0); /* on its way while LDS is cleared */
+    __syncthreads();
+    if (first >= 0) atomicAdd(&hist[wave * ne + first], 1);
+#pragma unroll 4
+    for (int j = 1; j < a.steps; j++) {
+        const int e = expert_of(a, p0 + 64ll * j);
+        if (e >= 0) atomicAdd(&hist[wave * ne + e], 1);
+    }
+    if (a.blocks > 1) { /* integer sums: their order does not matter */
+        for (int i = threadIdx.x; i < a.blocks * ne; i += nt) {
+            const int c = a.ws[i], e = i % ne;
+            if (c) {
+                atomicAdd(&all[e], c);
+                if (i / ne < (int)blockIdx.x) atomicAdd(&before[e], c);
             }
         }
-        if (lane == r) my_e = e, my_v = mx;
     }
-    const float top = __shfl(my_v, 0);
-    const float ex = lane < a.k && my_e >= 0 ? expf(my_v - top) : 0.f;
-    const float tot = wave_sum(ex);
-    if (lane < a.k) {
-        a.idx[(size_t)t * a.k + lane] = my_e;
-        a.w[(size_t)t * a.k + lane] = my_e >= 0 ? ex / tot : 0.f;
-    }
-}
-
-template <int TY> __device__ __forceinline__ void route_bwd_body(const RouteBwdArgs &a, int t) {
-    const int lane = threadIdx.x & 63;
-    int e = -1;
-    float w = 0.f, dw = 0.f;
-    if (lane < a.k) {
-        e = a.idx[(size_t)t * a.k + lane];
-        if (e < 0 || e >= a.n_exp) e = -1;
-        if (e >= 0) w = a.w[(size_t)t * a.k + lane], dw = a.dw[(size_t)t * a.k + lane];
-    }
-    const float g = w * (dw - wave_sum(w * dw));
-    typename XT<TY>::raw *d = (typename XT<TY>::raw *)a.dlogits + (size_t)t * a.n_exp;
-    for (int e0 = 0; e0 < a.n_exp; e0 += 64) {
-        float v = 0.f;
-        for (int s = 0; s < a.k; s++) {
-            const int es = __shfl(e, s);
-            const float gs = __shfl(g, s);
-            if (es == e0 + lane) v += gs;
-        }
-        if (e0 + lane < a.n_exp) d[e0 + lane] = XT<TY>::down(v);
-    }
-}
-
-/* One block per expert: the pairs of lower experts counted, then its own placed in pair order (ranks by ballots). The
- * block after the last expert marks the dropped pairs and writes off[n_exp]. */
-extern "C" __global__ void __launch_bounds__(256) le_rt_sort(SortArgs a) {
-    __shared__ int wcnt[4];
-    const int e = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    int low = 0;
-    for (long long pl = threadIdx.x; pl < a.np; pl += 256) {
-        const int p = (int)pl;
-        const int v = a.idx[p];
-        low += v >= 0 && v < e;
-        if (e == a.n_exp && a.pos && (v < 0 || v >= e)) a.pos[p] = -1;
-    }
-    for (int o = 32; o > 0; o >>= 1) low += __shfl_xor(low, o);
-    if (lane == 0) wcnt[wave] = low;
     __syncthreads();
-    int at = wcnt[0] + wcnt[1] + wcnt[2] + wcnt[3];
-    if (threadIdx.x == 0) a.off[e] = at;
-    if (e == a.n_exp) return;
-    for (long long p0 = 0; p0 < a.np; p0 += 256) {
-        const bool in = p0 + threadIdx.x < a.np;
-        const int p = in ? (int)(p0 + threadIdx.x) : 0;
-        const bool hit = in && a.idx[p] == e;
-        const unsigned long long b = __ballot(hit);
-        __syncthreads();
-        if (lane == 0) wcnt[wave] = __popcll(b);
-        __syncthreads();
-        int q = at + __popcll(b & ((1ull << lane) - 1ull));
-        for (int w = 0; w < 4; w++) {
-            q += w < wave ? wcnt[w] : 0;
-            at += wcnt[w];
+    /* offsets: an exclusive scan over the experts, one a thread and round */
+    int carry = 0;
+    for (int e0 = 0; e0 < ne; e0 += nt) {
+        const int e = e0 + threadIdx.x;
+        int own = 0;
+        if (e < ne) {
+            if (a.blocks > 1) own = all[e];
+            else
+                for (int w = 0; w < a.waves; w++) own += hist[w * ne + e];
         }
-        if (hit) {
-            if (a.in_idx) a.in_idx[q] = p / a.k;
-            if (a.out_idx) a.out_idx[q] = p;
+        int incl = own;
+        for (int d = 1; d < 64; d <<= 1) {
+            const int y = __shfl_up(incl, d);
+            if (lane >= d) incl += y;
+        }
+        __syncthreads();
+        if (lane == 63) wsum[wave] = incl;
+        __syncthreads();
+        int at = carry + incl - own;
+        for (int w = 0; w < a.waves; w++) {
+            if (w < wave) at += wsum[w];
+            carry += wsum[w];
+        }
+        if (e < ne) {
+            if (blockIdx.x == 0) a.off[e] = at;
+            at += before[e];
+            for (int w = 0; w < a.waves; w++) { /* counts to places */
+                const int c = hist[w * ne + e];
+                hist[w * ne + e] = at;
+                at += c;
+            }
+        }
+    }
+    if (blockIdx.x == 0 && threadIdx.x == 0) a.off[ne] = carry;
+    __syncthreads();
+    const int bits = 32 - __clz(ne - 1);
+    const unsigned long long lower = (1ull << lane) - 1ull;
+    for (int j = 0; j < a.steps; j++) {
+        const long long p = p0 + 64ll * j;
+        const int e = j == 0 ? first : expert_of(a, p);
+        unsigned long long same = __ballot(e >= 0);
+        for (int b = 0; b < bits; b++) {
+            const unsigned long long m = __ballot(e >> b & 1);
+            same &= e >> b & 1 ? m : ~m;
+        }
+        if (e >= 0) {
+            int *next = &hist[wave * ne + e];
+            const int q = *next + __popcll(same & lower);
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            if ((same & ~lower) >> lane == 1ull) *next = q + 1; /* the step's last of this expert */
+            if (a.in_idx) a.in_idx[q] = (int)(p / a.k);
+            if (a.out_idx) a.out_idx[q] = (int)p;
             if (a.pos) a.pos[p] = q;
+        } else if (e == -1 && a.pos) {
+            a.pos[p] = -1;
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+
+/* ---- rows between token order and expert order ----
+ * Bound by memory: every row is read once and written once. A token is taken by a group of L lanes (16 to 256), 16 bytes a lane and step (rows
+ * need not be aligned: the unaligned forms of the loads and stores), the last values of a row one by one. The places and weights of a
+ * token's pairs are loaded by 16 lanes at once. */
+typedef unsigned v4 __attribute__((ext_vector_type(4)));
+typedef unsigned v4u __attribute__((ext_vector_type(4), aligned(2))); /* at any value's address */
+template <int TY> struct Oct { /* 16 bytes of values */
+    static constexpr int N = TY == 0 ? 4 : 8;
+    using raw = typename XT<TY>::raw;
+    raw v[N];
+    __device__ __forceinline__ void load(const raw *p, int n) { /* n values are there */
+        if (n >= N) {
+            const v4 w = *(const v4u *)p;
+            __builtin_memcpy(v, &w, 16);
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; i++) v[i] = i < n ? p[i] : (raw)0;
         }
     }
-}
-
-/* The expert row of pair p, or -1. */
-static __device__ __forceinline__ int row_of(const RowsArgs &a, int p) {
-    const int r = a.pos ? a.pos[p] : p;
-    return r >= 0 && r < a.n_row ? r : -1;
-}
-
-/* One block per token. */
-template <int TY> __device__ __forceinline__ void permute_body(const RowsArgs &a, int t) {
-    const typename XT<TY>::raw *x = (const typename XT<TY>::raw *)a.src + (size_t)t * a.ldt;
-    for (int s = 0; s < a.k; s++) {
-        const int r = row_of(a, t * a.k + s);
-        if (r < 0) continue;
-        typename XT<TY>::raw *e = (typename XT<TY>::raw *)a.dst + (size_t)r * a.lde;
-        for (int c = threadIdx.x; c < a.cols; c += 256) e[c] = x[c];
+    __device__ __forceinline__ void store(raw *p, int n) const {
+        if (n >= N) {
+            v4 w;
+            __builtin_memcpy(&w, v, 16);
+            *(v4u *)p = w;
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; i++)
+                if (i < n) p[i] = v[i];
+        }
     }
-}
+};
+/* The pairs of a token: lane i of each 16 holds pair i's row (-1: none) and weight. */
+template <int L> struct Pairs {
+    int row;
+    float w;
+    __device__ __forceinline__ void load(const RowsArgs &a, long long t) {
+        const int i = threadIdx.x & 15;
+        row = -1;
+        w = 1.f;
+        if (t < a.n_tok && i < a.k) {
+            const long long p = t * a.k + i;
+            row = a.pos ? a.pos[p] : (int)p;
+            if (row < 0 || row >= a.n_row) row = -1;
+            if (a.w) w = a.w[p];
+        }
+    }
+    template <class T> static __device__ __forceinline__ T of(T v, int s) {
+        const int b = __builtin_bit_cast(int, v);
+        if constexpr (L >= 64) return __builtin_bit_cast(T, __builtin_amdgcn_readlane(b, s)); /* one token a wave */
+        else return __builtin_bit_cast(T, __builtin_amdgcn_ds_bpermute((((int)threadIdx.x & 48) + s) * 4, b));
+    }
+};
+/* Group of L lanes, and the tokens it goes over. */
+#define GROUP_TOKENS(L) \
+    const int l = threadIdx.x & (L - 1); \
+    for (long long t0 = (long long)blockIdx.x * (256 / L), t; t = t0 + threadIdx.x / L, t0 < a.n_tok; t0 += (long long)gridDim.x * (256 / L))
 
-template <int TY> __device__ __forceinline__ void combine_body(const RowsArgs &a, int t) {
-    typename XT<TY>::raw *out = (typename XT<TY>::raw *)a.dst + (size_t)t * a.ldt;
-    for (int c = threadIdx.x; c < a.cols; c += 256) {
-        float sum = 0.f;
+/* e[row of pair] = x[t]; blockIdx.y: 16 L bytes of the columns. */
+template <int TY, int L> __device__ __forceinline__ void permute_body(const RowsArgs &a) {
+    using O = Oct<TY>;
+    GROUP_TOKENS(L) {
+        const int c = ((int)blockIdx.y * L + l) * O::N, n = t < a.n_tok ? a.cols - c : 0;
+        Pairs<L> pr;
+        pr.load(a, t);
+        O o;
+        if (n > 0) o.load((const typename O::raw *)a.src + t * a.ldt + c, n);
         for (int s = 0; s < a.k; s++) {
-            const int r = row_of(a, t * a.k + s);
-            if (r < 0) continue;
-            const float v = XT<TY>::up(((const typename XT<TY>::raw *)a.src)[(size_t)r * a.lde + c]);
-            sum += a.w ? a.w[t * a.k + s] * v : v;
+            const int r = Pairs<L>::of(pr.row, s);
+            if (r >= 0 && n > 0) o.store((typename O::raw *)a.dst + r * a.lde + c, n);
         }
-        out[c] = XT<TY>::down(sum);
     }
 }
 
-template <int TY> __device__ __forceinline__ void combine_bwd_body(const RowsArgs &a, int t) {
-    __shared__ float part[4];
-    const typename XT<TY>::raw *dout = (const typename XT<TY>::raw *)a.src + (size_t)t * a.ldt;
-    for (int s = 0; s < a.k; s++) {
-        const int p = t * a.k + s, r = row_of(a, p);
-        if (r < 0) {
-            if (a.dw && threadIdx.x == 0) a.dw[p] = 0.f;
-            continue;
+/* out[t] = sum of weight * e[row], in selection order; the rows' loads eight at a time. */
+template <int TY, int L> __device__ __forceinline__ void combine_body(const RowsArgs &a) {
+    using O = Oct<TY>;
+    GROUP_TOKENS(L) {
+        const int c = ((int)blockIdx.y * L + l) * O::N, n = t < a.n_tok ? a.cols - c : 0;
+        Pairs<L> pr;
+        pr.load(a, t);
+        float sum[O::N] = {};
+        for (int s0 = 0; s0 < a.k; s0 += 8) {
+            O o[8];
+            int r[8];
+#pragma unroll
+            for (int s = 0; s < 8; s++) {
+                r[s] = Pairs<L>::of(pr.row, s0 + s); /* -1 from k on */
+                if (r[s] >= 0 && n > 0) o[s].load((const typename O::raw *)a.src + r[s] * a.lde + c, n);
+            }
+#pragma unroll
+            for (int s = 0; s < 8; s++) {
+                const float w = Pairs<L>::of(pr.w, s0 + s);
+#pragma unroll
+                for (int i = 0; i < O::N; i++) sum[i] = r[s] >= 0 ? __builtin_fmaf(w, XT<TY>::up(o[s].v[i]), sum[i]) : sum[i];
+            }
         }
-        const float w = a.w ? a.w[p] : 1.f;
-        const typename XT<TY>::raw *e = (const typename XT<TY>::raw *)a.e + (size_t)r * a.lde;
-        typename XT<TY>::raw *de = (typename XT<TY>::raw *)a.dst + (size_t)r * a.lde;
-        float dot = 0.f;
-        for (int c = threadIdx.x; c < a.cols; c += 256) {
-            const float d = XT<TY>::up(dout[c]);
-            if (a.dw) dot += d * XT<TY>::up(e[c]);
-            if (a.dst) de[c] = XT<TY>::down(w * d);
+        if (n > 0) {
+            O o;
+#pragma unroll
+            for (int i = 0; i < O::N; i++) o.v[i] = XT<TY>::down(sum[i]);
+            o.store((typename O::raw *)a.dst + t * a.ldt + c, n);
         }
-        if (!a.dw) continue;
-        dot = wave_sum(dot);
-        __syncthreads();
-        if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = dot;
-        __syncthreads();
-        if (threadIdx.x == 0) a.dw[p] = part[0] + part[1] + part[2] + part[3];
     }
 }
 
-/* Tokens of a wave (four waves a block) and of a block; the grid may be smaller than the tokens. */
-#define WAVE_TOKENS for (long long t = blockIdx.x * 4ll + (threadIdx.x >> 6); t < a.n_tok; t += gridDim.x * 4ll)
-#define BLOCK_TOKENS for (long long t = blockIdx.x; t < a.n_tok; t += gridDim.x)
-#define LE_RT(TY)                                                                                                                      \
-    extern "C" __global__ void __launch_bounds__(256) le_rt_route_##TY(RouteArgs a) { WAVE_TOKENS route_body<TY>(a, (int)t); }             \
-    extern "C" __global__ void __launch_bounds__(256) le_rt_route_bwd_##TY(RouteBwdArgs a) { WAVE_TOKENS route_bwd_body<TY>(a, (int)t); }  \
-    extern "C" __global__ void __launch_bounds__(256) le_rt_permute_##TY(RowsArgs a) { BLOCK_TOKENS permute_body<TY>(a, (int)t); }         \
-    extern "C" __global__ void __launch_bounds__(256) le_rt_combine_##TY(RowsArgs a) { BLOCK_TOKENS combine_body<TY>(a, (int)t); }         \
-    extern "C" __global__ void __launch_bounds__(256) le_rt_combine_bwd_##TY(RowsArgs a) { BLOCK_TOKENS combine_bwd_body<TY>(a, (int)t); }
+/* de[row] = weight * dout[t], dw = dout[t] . e[row]: a lane's products over its columns, then the lanes', then the waves'. */
+template <int TY, int L> __device__ __forceinline__ void combine_bwd_body(const RowsArgs &a) {
+    using O = Oct<TY>;
+    __shared__ float part[4][8];
+    GROUP_TOKENS(L) {
+        Pairs<L> pr;
+        pr.load(a, t);
+        for (int s0 = 0; s0 < a.k; s0 += 8) {
+            int r[8];
+            float w[8], dot[8] = {};
+#pragma unroll
+            for (int s = 0; s < 8; s++) {
+                r[s] = Pairs<L>::of(pr.row, s0 + s);
+                w[s] = Pairs<L>::of(pr.w, s0 + s);
+            }
+            for (int c = l * O::N; c < (t < a.n_tok ? a.cols : 0); c += L * O::N) {
+                const int n = a.cols - c;
+                O d, e[8];
+                d.load((const typename O::raw *)a.src + t * a.ldt + c, n);
+                if (a.dw) {
+#pragma unroll
+                    for (int s = 0; s < 8; s++)
+                        if (r[s] >= 0) e[s].load((const typename O::raw *)a.e + r[s] * a.lde + c, n);
+                }
+#pragma unroll
+                for (int s = 0; s < 8; s++) {
+                    if (r[s] < 0) continue;
+                    if (a.dw) {
+#pragma unroll
+                        for (int i = 0; i < O::N; i++) dot[s] = __builtin_fmaf(XT<TY>::up(d.v[i]), XT<TY>::up(e[s].v[i]), dot[s]);
+                    }
+                    if (a.dst) {
+                        O o;
+#pragma unroll
+                        for (int i = 0; i < O::N; i++) o.v[i] = XT<TY>::down(w[s] * XT<TY>::up(d.v[i]));
+                        o.store((typename O::raw *)a.dst + r[s] * a.lde + c, n);
+                    }
+                }
+            }
+            if (!a.dw) continue;
+#pragma unroll
+            for (int s = 0; s < 8; s++) dot[s] = group_sum<(L < 64 ? L : 64)>(dot[s]);
+            if constexpr (L > 64) {
+                __syncthreads(); /* every thread of the block is here as often: L > 64 gives a block whole tokens, and k is one */
+                if ((threadIdx.x & 63) == 0)
+#pragma unroll
+                    for (int s = 0; s < 8; s++) part[threadIdx.x >> 6][s] = dot[s];
+                __syncthreads();
+                const int w0 = threadIdx.x / L * (L / 64);
+#pragma unroll
+                for (int s = 0; s < 8; s++) {
+                    dot[s] = part[w0][s];
+                    for (int i = 1; i < L / 64; i++) dot[s] += part[w0 + i][s];
+                }
+            }
+            if (t < a.n_tok && l < 8 && s0 + l < a.k) {
+                float v = 0.f;
+#pragma unroll
+                for (int s = 0; s < 8; s++) v = l == s && r[s] >= 0 ? dot[s] : v;
+                a.dw[t * a.k + s0 + l] = v;
+            }
+        }
+    }
+}
+
+#define LE_RT_ROUTE(TY, L, V) \
+    extern "C" __global__ void __launch_bounds__(256) le_rt_route_##TY##_l##L##_v##V(RouteArgs a) { route_body<TY, L, V>(a); }
+#define LE_RT_ROWS(TY, L) \
+    extern "C" __global__ void __launch_bounds__(256) le_rt_permute_##TY##_l##L(RowsArgs a) { permute_body<TY, L>(a); } \
+    extern "C" __global__ void __launch_bounds__(256) le_rt_combine_##TY##_l##L(RowsArgs a) { combine_body<TY, L>(a); } \
+    extern "C" __global__ void __launch_bounds__(256) le_rt_combine_bwd_##TY##_l##L(RowsArgs a) { combine_bwd_body<TY, L>(a); }
+#define LE_RT(TY) \
+    LE_RT_ROUTE(TY, 16, 2) LE_RT_ROUTE(TY, 16, 4) LE_RT_ROUTE(TY, 16, 8) LE_RT_ROUTE(TY, 32, 8) LE_RT_ROUTE(TY, 64, 8) LE_RT_ROUTE(TY, 64, 16) \
+    extern "C" __global__ void __launch_bounds__(256) le_rt_route_bwd_##TY(RouteBwdArgs a) { route_bwd_body<TY>(a); } \
+    LE_RT_ROWS(TY, 16) LE_RT_ROWS(TY, 64) LE_RT_ROWS(TY, 256)
 LE_RT(0) LE_RT(1) LE_RT(30)
