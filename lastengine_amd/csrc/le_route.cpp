@@ -63,8 +63,10 @@ int le_moe_route(le_ctx *c, int ltype, const void *logits, int n_tok, int n_exp,
     if (int rc = le_ctx_on_device(c)) return rc;
     RouteArgs a{logits, idx, w, n_tok, n_exp, k};
     void *args[] = {&a};
-    /* lanes a token and experts a lane: the fewest lanes that hold the experts in eight values each */
-    const int L = n_exp <= 128 ? 16 : n_exp <= 256 ? 32 : 64, V = n_exp <= 32 ? 2 : n_exp <= 64 ? 4 : n_exp <= 512 ? 8 : 16;
+    /* lanes a token and experts a lane: 64 lanes while the waves do not fill the chip (and for many experts), else the fewest
+     * that hold the experts in eight values each */
+    int L = n_exp <= 128 ? 16 : n_exp <= 256 ? 32 : 64, V = n_exp <= 32 ? 2 : n_exp <= 64 ? 4 : n_exp <= 512 ? 8 : 16;
+    if (L < 64 && n_tok <= 8 * le_ctx_cus(c)) L = 64, V = n_exp <= 64 ? 1 : n_exp <= 128 ? 2 : 4;
     char name[40];
     snprintf(name, sizeof name, "le_rt_route_%d_l%d_v%d", ltype, L, V);
     return le_ctx_launch(c, name, dim3((unsigned)std::min((n_tok * (long long)L + 255) / 256, 1LL << 20)), 256, 0, (hipStream_t)stream, args);
@@ -86,7 +88,7 @@ int le_moe_route_bwd(le_ctx *c, int ltype, const int *idx, const float *w, const
     void *args[] = {&a};
     char name[32];
     snprintf(name, sizeof name, "le_rt_route_bwd_%d", ltype);
-    return le_ctx_launch(c, name, dim3((unsigned)std::min((n_tok + 15LL) / 16, 1LL << 20)), 256, 0, (hipStream_t)stream, args);
+    return le_ctx_launch(c, name, dim3((unsigned)std::min((n_tok + 3LL) / 4, 1LL << 20)), 256, 0, (hipStream_t)stream, args);
 }
 
 size_t le_moe_sort_workspace_size(int n_tok, int k, int n_exp) {

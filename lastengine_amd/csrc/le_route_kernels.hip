@@ -31,54 +31,60 @@ template <int L, int D = 1> static __device__ __forceinline__ float group_sum(fl
         return v;
     }
 }
-/* Largest value and, of equal ones, the lowest index over groups of L lanes. */
-template <int L, int D = 1> static __device__ __forceinline__ void group_argmax(float &v, int &i) {
-    if constexpr (D < L) {
-        const float ov = as_float(across<D>(as_int(v)));
-        const int oi = across<D>(i);
-        const bool take = ov > v || (ov == v && oi < i);
-        v = take ? ov : v;
-        i = take ? oi : i;
-        group_argmax<L, 2 * D>(v, i);
-    }
+/* Largest and smallest over groups of L lanes, in every lane of them (one instruction a step up to 16 lanes). */
+template <int L, int D = 1> static __device__ __forceinline__ int group_max(int v) {
+    if constexpr (D < L) return group_max<L, 2 * D>(max(v, across<D>(v)));
+    else return v;
+}
+template <int L, int D = 1> static __device__ __forceinline__ int group_min(int v) {
+    if constexpr (D < L) return group_min<L, 2 * D>(min(v, across<D>(v)));
+    else return v;
 }
 
 /* ---- router ----
- * Top-k by groups of L lanes, a token each, lane l holding experts l, l + L, ... (V of them): k rounds of an argmax, first in the
- * lane, then over the group by DPP. Lane s < k keeps selection s. Reads the logits once and is bound by the rounds' instructions:
- * with 16 lanes a token a wave's rounds serve four tokens. */
+ * Top-k by groups of L lanes, a token each, lane l holding experts l, l + L, ... (V of them) as integers that order as the logits do (-0
+ * as 0; NaN and -infinity below all). k rounds of a maximum, then the lowest expert that has it. Lane s < k keeps selection s. Reads
+ * the logits once; bound by the rounds' instructions for many tokens (16384 of 128 experts, 8 of them: L = 16, whose wave serves
+ * four tokens with a round), by their latency for few (L = 64, ballots instead of the second reduction). */
+constexpr int kNone = (int)0x80000000;
+static __device__ __forceinline__ int order_key(float x) {
+    const int b = as_int(x + 0.f);
+    return x > -INFINITY ? b ^ ((b >> 31) & 0x7FFFFFFF) : kNone;
+}
+static __device__ __forceinline__ float key_value(int k) { return as_float(k ^ ((k >> 31) & 0x7FFFFFFF)); }
 template <int TY, int L, int V> __device__ __forceinline__ void route_body(const RouteArgs &a) {
     const int l = threadIdx.x & (L - 1);
     for (long long t0 = (long long)blockIdx.x * (256 / L); t0 < a.n_tok; t0 += (long long)gridDim.x * (256 / L)) {
         const long long t = t0 + threadIdx.x / L;
         const bool there = t < a.n_tok; /* lanes of a token behind the last go along, and write nothing */
         const typename XT<TY>::raw *lg = (const typename XT<TY>::raw *)a.logits + (there ? t : a.n_tok - 1) * a.n_exp;
-        float v[V];
+        int v[V];
 #pragma unroll
-        for (int j = 0; j < V; j++) {
-            const int e = l + L * j;
-            const float x = e < a.n_exp ? XT<TY>::up(lg[e]) : -INFINITY;
-            v[j] = x == x ? x : -INFINITY;
-        }
-        int my_e = -1;
-        float my_v = -INFINITY;
+        for (int j = 0; j < V; j++) v[j] = l + L * j < a.n_exp ? order_key(XT<TY>::up(lg[l + L * j])) : kNone;
+        int my_e = -1, my_v = kNone;
         for (int r = 0; r < a.k; r++) {
-            float mx = v[0];
-            int e = l;
+            int mx = v[0];
 #pragma unroll
-            for (int j = 1; j < V; j++) {
-                e = v[j] > mx ? l + L * j : e;
-                mx = fmaxf(mx, v[j]);
+            for (int j = 1; j < V; j++) mx = max(mx, v[j]);
+            mx = group_max<L>(mx);
+            int e = 0x7FFFFFFF;
+            if constexpr (L == 64) {
+#pragma unroll
+                for (int j = V - 1; j >= 0; j--) {
+                    const unsigned long long b = __ballot(v[j] == mx);
+                    e = b ? 64 * j + __ffsll((long long)b) - 1 : e;
+                }
+            } else {
+#pragma unroll
+                for (int j = V - 1; j >= 0; j--) e = v[j] == mx ? l + L * j : e;
+                e = group_min<L>(e);
             }
-            group_argmax<L>(mx, e);
-            const bool found = mx > -INFINITY;
 #pragma unroll
-            for (int j = 0; j < V; j++) v[j] = e == l + L * j ? -INFINITY : v[j];
-            my_e = l == r && found ? e : my_e;
-            my_v = l == r && found ? mx : my_v;
+            for (int j = 0; j < V; j++) v[j] = e == l + L * j ? kNone : v[j];
+            if (l == r && mx != kNone) my_e = e, my_v = mx;
         }
-        const float top = as_float(__builtin_amdgcn_ds_bpermute((threadIdx.x & 63 & ~(L - 1)) * 4, as_int(my_v)));
-        const float ex = my_e >= 0 ? expf(my_v - top) : 0.f;
+        const float top = key_value(__builtin_amdgcn_ds_bpermute((threadIdx.x & 63 & ~(L - 1)) * 4, my_v));
+        const float ex = my_e >= 0 ? expf(key_value(my_v) - top) : 0.f;
         const float tot = group_sum<L>(ex);
         if (there && l < a.k) {
             a.idx[t * a.k + l] = my_e;
@@ -87,33 +93,31 @@ template <int TY, int L, int V> __device__ __forceinline__ void route_body(const
     }
 }
 
-/* Gradient: the token's selections in lanes s < k of a group of 16, each value then added where its expert is: no scatter, every logit written
+/* Gradient: one wave a token, its selections in lanes s < k; each value is then added where its expert is: no scatter, every logit written
  * once. */
 template <int TY> __device__ __forceinline__ void route_bwd_body(const RouteBwdArgs &a) {
-    const int l = threadIdx.x & 15, base = threadIdx.x & 48;
-    for (long long t0 = (long long)blockIdx.x * 16; t0 < a.n_tok; t0 += (long long)gridDim.x * 16) {
-        const long long t = t0 + threadIdx.x / 16;
-        const bool there = t < a.n_tok;
+    const int l = threadIdx.x & 63;
+    for (long long t = (long long)blockIdx.x * 4 + (threadIdx.x >> 6); t < a.n_tok; t += (long long)gridDim.x * 4) {
         int e = -1;
         float w = 0.f, dw = 0.f;
-        if (there && l < a.k) {
+        if (l < a.k) {
             e = a.idx[t * a.k + l];
-            if (e < 0 || e >= a.n_exp) e = -1;
-            if (e >= 0) w = a.w[t * a.k + l], dw = a.dw[t * a.k + l];
+            w = a.w[t * a.k + l], dw = a.dw[t * a.k + l];
+            if (e < 0 || e >= a.n_exp) e = -1, w = 0.f, dw = 0.f;
         }
-        const float g = w * (dw - group_sum<16>(w * dw));
+        const float g = w * (dw - group_sum<16>(w * dw)); /* the selections lie in the first 16 lanes */
         typename XT<TY>::raw *d = (typename XT<TY>::raw *)a.dlogits + t * a.n_exp;
-        for (int e0 = 0; e0 < a.n_exp; e0 += 64) {
+        for (int e0 = 0; e0 < a.n_exp; e0 += 256) {
             float v[4] = {0.f, 0.f, 0.f, 0.f};
             for (int s = 0; s < a.k; s++) {
-                const int es = __builtin_amdgcn_ds_bpermute((base + s) * 4, e) - e0 - l;
-                const float gs = as_float(__builtin_amdgcn_ds_bpermute((base + s) * 4, as_int(g)));
+                const int es = __builtin_amdgcn_readlane(e, s) - e0 - l;
+                const float gs = as_float(__builtin_amdgcn_readlane(as_int(g), s));
 #pragma unroll
-                for (int j = 0; j < 4; j++) v[j] += es == 16 * j ? gs : 0.f;
+                for (int j = 0; j < 4; j++) v[j] += es == 64 * j ? gs : 0.f;
             }
 #pragma unroll
             for (int j = 0; j < 4; j++)
-                if (there && e0 + l + 16 * j < a.n_exp) d[e0 + l + 16 * j] = XT<TY>::down(v[j]);
+                if (e0 + l + 64 * j < a.n_exp) d[e0 + l + 64 * j] = XT<TY>::down(v[j]);
         }
     }
 }
@@ -131,24 +135,27 @@ static __device__ __forceinline__ int expert_of(const SortArgs &a, long long p) 
 }
 extern "C" __global__ void __launch_bounds__(1024) le_rt_count(SortArgs a) {
     extern __shared__ int hist[];
-    for (int e = threadIdx.x; e < a.n_exp; e += blockDim.x) hist[e] = 0;
-    __syncthreads();
     const long long p0 = ((long long)blockIdx.x * a.waves + (threadIdx.x >> 6)) * 64 * a.steps + (threadIdx.x & 63);
+    const int first = expert_of(a, p0); /* on its way while LDS is cleared */
+    for (int e = threadIdx.x; e < a.n_exp; e += 1024) hist[e] = 0;
+    __syncthreads();
+    if (first >= 0) atomicAdd(&hist[first], 1);
 #pragma unroll 4
-    for (int j = 0; j < a.steps; j++) {
+    for (int j = 1; j < a.steps; j++) {
         const int e = expert_of(a, p0 + 64ll * j);
         if (e >= 0) atomicAdd(&hist[e], 1);
     }
     __syncthreads();
-    for (int e = threadIdx.x; e < a.n_exp; e += blockDim.x) a.ws[blockIdx.x * a.n_exp + e] = hist[e];
+    for (int e = threadIdx.x; e < a.n_exp; e += 1024) a.ws[blockIdx.x * a.n_exp + e] = hist[e];
 }
 extern "C" __global__ void __launch_bounds__(1024) le_rt_sort(SortArgs a) {
     extern __shared__ int hist[]; /* [wave][expert], then [expert] all pairs, [expert] those of earlier blocks, [16] */
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, nt = 64 * a.waves, ne = a.n_exp;
     int *all = hist + a.waves * ne, *before = all + ne, *wsum = before + ne;
-    for (int i = threadIdx.x; i < a.waves * ne + 2 * ne; i += nt) hist[i] = 0;
     const long long p0 = ((long long)blockIdx.x * a.waves + wave) * 64 * a.steps + lane;
-    int first = expert_of(a, p0); /* on its way while LDS is cleared */
+    const int first = expert_of(a, p0); /* on its way while LDS is cleared; the other blocks' counts, too */
+    const int c0 = a.blocks > 1 && (int)threadIdx.x < a.blocks * ne ? a.ws[threadIdx.x] : 0;
+    for (int i = threadIdx.x; i < a.waves * ne + 2 * ne; i += nt) hist[i] = 0;
     __syncthreads();
     if (first >= 0) atomicAdd(&hist[wave * ne + first], 1);
 #pragma unroll 4
@@ -157,8 +164,9 @@ extern "C" __global__ void __launch_bounds__(1024) le_rt_sort(SortArgs a) {
         if (e >= 0) atomicAdd(&hist[wave * ne + e], 1);
     }
     if (a.blocks > 1) { /* integer sums: their order does not matter */
+#pragma unroll 4
         for (int i = threadIdx.x; i < a.blocks * ne; i += nt) {
-            const int c = a.ws[i], e = i % ne;
+            const int c = i == (int)threadIdx.x ? c0 : a.ws[i], e = i % ne;
             if (c) {
                 atomicAdd(&all[e], c);
                 if (i / ne < (int)blockIdx.x) atomicAdd(&before[e], c);
@@ -404,7 +412,8 @@ template <int TY, int L> __device__ __forceinline__ void combine_bwd_body(const 
     extern "C" __global__ void __launch_bounds__(256) le_rt_combine_##TY##_l##L(RowsArgs a) { combine_body<TY, L>(a); } \
     extern "C" __global__ void __launch_bounds__(256) le_rt_combine_bwd_##TY##_l##L(RowsArgs a) { combine_bwd_body<TY, L>(a); }
 #define LE_RT(TY) \
-    LE_RT_ROUTE(TY, 16, 2) LE_RT_ROUTE(TY, 16, 4) LE_RT_ROUTE(TY, 16, 8) LE_RT_ROUTE(TY, 32, 8) LE_RT_ROUTE(TY, 64, 8) LE_RT_ROUTE(TY, 64, 16) \
+    LE_RT_ROUTE(TY, 16, 2) LE_RT_ROUTE(TY, 16, 4) LE_RT_ROUTE(TY, 16, 8) LE_RT_ROUTE(TY, 32, 8) \
+    LE_RT_ROUTE(TY, 64, 1) LE_RT_ROUTE(TY, 64, 2) LE_RT_ROUTE(TY, 64, 4) LE_RT_ROUTE(TY, 64, 8) LE_RT_ROUTE(TY, 64, 16) \
     extern "C" __global__ void __launch_bounds__(256) le_rt_route_bwd_##TY(RouteBwdArgs a) { route_bwd_body<TY>(a); } \
     LE_RT_ROWS(TY, 16) LE_RT_ROWS(TY, 64) LE_RT_ROWS(TY, 256)
 LE_RT(0) LE_RT(1) LE_RT(30)
