@@ -126,7 +126,12 @@ static int rows_launch(le_ctx *c, const char *what, int ty, const RowsArgs &rows
     const bool whole = !strcmp(what, "combine_bwd");
     if (!whole && (parts + L - 1) / L > 65535) return le_ctx_failf(c, LE_ERR_SHAPE, "cols=%d", a.cols);
     char name[40];
-    snprintf(name, sizeof name, "le_rt_%s_%d_l%d", what, ty, L);
+    /* expert rows that are read and lie at 16-byte addresses: non-temporal from 8 MB on (4096 tokens of 8 pairs by 2048 bf16: sum 30.3 -> 26.6
+     * us, its gradient 62 -> 58, a sum behind that 90 -> 80; 64 tokens 3.6 -> 4.0, 301 by 1001 fp32, whose rows share lines, 5.3 -> 6.4) */
+    const void *e = whole ? a.e : a.src;
+    const int b = type_bytes(ty);
+    const bool nt = strcmp(what, "permute") && e && (long long)a.n_tok * a.k * a.cols * b >= 8 << 20 && aligned(e, 16) && a.lde * b % 16 == 0;
+    snprintf(name, sizeof name, "le_rt_%s_%d_l%d%s", what, ty, L, nt ? "_nt" : "");
     return le_ctx_launch(c, name, dim3((unsigned)std::min((a.n_tok * (long long)L + 255) / 256, 1LL << 20), whole ? 1u : (unsigned)((parts + L - 1) / L)), 256, 0,
                          (hipStream_t)stream, args);
 }

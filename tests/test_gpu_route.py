@@ -420,3 +420,34 @@ def test_refusals(engine):
         with pytest.raises(le.LeError) as e:
             call()
         assert e.value.code == code
+
+
+@pytest.mark.parametrize("ty", TYPES)
+def test_many_rows(engine, ty):
+    """Enough aligned rows for the non-temporal loads, with the last token's pairs and some others without a row."""
+    import torch
+    n_tok, k, cols = 1100, 8, 1024 if ty == le.F32 else 2048
+    n_row = n_tok * k
+    pos = positions(n_tok, k, n_row, 5, 0.05)
+    pos[-k:] = -1
+    g = torch.Generator().manual_seed(8)
+    e = torch.randn(n_row, cols, generator=g).to(torch_type(ty)).cuda()
+    dout = torch.randn(n_tok, cols, generator=g).to(torch_type(ty)).cuda()
+    w = torch.randn(n_tok * k, generator=g).cuda()
+    dpos = torch.from_numpy(pos).cuda()
+    out = torch.empty(n_tok, cols, dtype=torch_type(ty), device="cuda")
+    de, dw = torch.zeros_like(e), torch.empty(n_tok * k, device="cuda")
+    engine.moe_combine(ty, e, dpos, w, n_tok, k, cols, out, n_row)
+    engine.moe_combine_bwd(ty, dout, e, dpos, w, n_tok, k, cols, de, dw, n_row)
+    ok = ((dpos >= 0) & (dpos < n_row)).reshape(n_tok, k)
+    at = torch.where(ok, dpos.reshape(n_tok, k), 0).long()
+    ww = torch.where(ok, w.reshape(n_tok, k), 0.0).double()
+    rows = e.double()[at]
+    want, mag = (rows * ww[..., None]).sum(1), (rows * ww[..., None]).abs().sum(1)
+    assert ((out.double() - want).abs() <= half_step(ty) * want.abs() + 2 * (k + 1) * U * mag + tiny(ty)).all() and (out[-1] == 0).all()
+    terms = dout.double()[:, None] * rows
+    got = dw.double().reshape(n_tok, k)
+    assert ((got - terms.sum(-1)).abs() <= (cols + 1) * U * terms.abs().sum(-1))[ok].all() and (got[~ok] == 0).all()
+    grad = torch.zeros_like(e, dtype=torch.float64)
+    grad[at[ok]] = (dout.double()[:, None] * ww[..., None])[ok]
+    assert ((de.double() - grad).abs() <= (half_step(ty) + 2 * U) * grad.abs() + tiny(ty)).all()
