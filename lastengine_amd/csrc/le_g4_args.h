@@ -12,10 +12,10 @@ struct G4Args {
     int gshift;        /* column >> gshift = group */
     int xty, sty, vec;     /* types of x and y, of the scales; a 128-column part's scales and zeros can be loaded at once */
     int nw, gx;        /* waves of a block, blocks of a slot (from here: the launch's own cost a load each) */
-    unsigned char *ws; /* le_g4x_*, le_g4m_*: fragments of a set of m tokens and their sums */
+    unsigned char *ws; /* le_g4x_*, le_g4t_*, le_g4m_*: fragments of a set of m tokens */
     long long ws_set, ws_downs; /* bytes of a set, before its powers of two */
     float *part;               /* [segment of K][value of y], where there are several segments */
     long long total;           /* values of y */
-    int segs;
+    int segs, na;              /* na: le_g4t_*: sets of four virtual rows; 0: le_g4m_* */
     int per, full;     /* row groups of the blocks below `full`; the others have one less */
 };

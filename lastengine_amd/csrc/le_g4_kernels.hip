@@ -109,6 +109,31 @@ template <int XTY> struct XOct {
     }
 };
 
+/* A scale or zero point as loaded (SB bytes), and N consecutive ones at once (16-bit ones two to a word). */
+template <int SB> static __device__ __forceinline__ unsigned load_scale(__amdgpu_buffer_rsrc_t r, unsigned off) {
+    if constexpr (SB == 4) return __builtin_amdgcn_raw_buffer_load_b32(r, off, 0, 0);
+    else return __builtin_amdgcn_raw_buffer_load_b16(r, off, 0, 0);
+}
+template <int N, int SB> static __device__ __forceinline__ void load_scales(unsigned (&d)[N], __amdgpu_buffer_rsrc_t r, unsigned off) {
+    if constexpr (N * SB == 16) {
+        const auto v = __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0);
+        d[0] = v[0], d[1] = v[1], d[2] = v[2], d[3] = v[3];
+    } else if constexpr (N * SB == 8) {
+        const auto v = __builtin_amdgcn_raw_buffer_load_b64(r, off, 0, 0);
+        d[0] = v[0], d[1] = v[1];
+    } else if constexpr (N * SB == 4) {
+        d[0] = __builtin_amdgcn_raw_buffer_load_b32(r, off, 0, 0);
+    }
+}
+/* Value k of those; several: loaded at once where a.vec. */
+template <int SB, int N> static __device__ __forceinline__ float scale_at(const G4Args &a, const unsigned (&d)[N], int k, bool several) {
+    if constexpr (SB == 4) return flt(d[k]);
+    else {
+        const unsigned v = several && a.vec ? d[k / 2] >> 16 * (k & 1) : d[k];
+        return a.sty == 1 ? XT<1>::up((unsigned short)v) : XT<30>::up((unsigned short)v);
+    }
+}
+
 /* SB: bytes of a scale; T tokens (at most); P pieces; T * P <= 4; MP: more slices than waves */
 template <int XTY, bool SW, int T, int P, int SB, int SUB, bool MP> __device__ __forceinline__ void g4q_body(const G4Args &a) {
     constexpr int BPC = 128 / SUB, XB = XTY == 0 ? 4 : 2;
@@ -226,40 +251,20 @@ template <int XTY, bool SW, int T, int P, int SB, int SUB, bool MP> __device__ _
         const auto rq = rsrc(w0, there ? bytes : 0), rs = rsrc(s0, there ? sbytes : 0), rz = rsrc(z0, there && a.zeros ? sbytes : 0);
         if (BPC > 1 && a.vec) { /* one load for a part's blocks: a quarter of the requests (groups of 32) */
             const unsigned off = ((gr * 16 + myrow) * a.ng + min((sl * 4 + g) * BPC, a.ng - BPC)) * SB;
-            auto wide = [&](unsigned (&d)[BPC], __amdgpu_buffer_rsrc_t r) {
-                if constexpr (BPC * SB == 16) {
-                    const auto v = __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0);
-                    d[0] = v[0], d[1] = v[1], d[2] = v[2], d[3] = v[3];
-                } else if constexpr (BPC * SB == 8) {
-                    const auto v = __builtin_amdgcn_raw_buffer_load_b64(r, off, 0, 0);
-                    d[0] = v[0], d[1] = v[1];
-                } else if constexpr (BPC * SB == 4) {
-                    d[0] = __builtin_amdgcn_raw_buffer_load_b32(r, off, 0, 0);
-                }
-            };
-            wide(it.s, rs);
-            wide(it.z, rz);
+            load_scales<BPC, SB>(it.s, rs, off);
+            load_scales<BPC, SB>(it.z, rz, off);
         } else {
 #pragma unroll
             for (int b = 0; b < BPC; b++) {
                 const int col = (sl * 4 + g) * 128 + b * SUB;
                 const unsigned off = ((gr * 16 + myrow) * a.ng + (min(col, a.cols - 1) >> a.gshift)) * SB;
-                if constexpr (SB == 4) {
-                    it.s[b] = __builtin_amdgcn_raw_buffer_load_b32(rs, off, 0, 0);
-                    it.z[b] = __builtin_amdgcn_raw_buffer_load_b32(rz, off, 0, 0);
-                } else {
-                    it.s[b] = __builtin_amdgcn_raw_buffer_load_b16(rs, off, 0, 0);
-                    it.z[b] = __builtin_amdgcn_raw_buffer_load_b16(rz, off, 0, 0);
-                }
+                it.s[b] = load_scale<SB>(rs, off);
+                it.z[b] = load_scale<SB>(rz, off);
             }
         }
         const unsigned go = gr * 16 * rowb + sl * 256;
 #pragma unroll
         for (int u = 0; u < 4; u++) it.q[u] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rq, vo[u] + go, 0, 2 /* nt */));
-    };
-    auto up_scale = [&](unsigned v) {
-        if constexpr (SB == 4) return flt(v);
-        else return a.sty == 1 ? XT<1>::up((unsigned short)v) : XT<30>::up((unsigned short)v);
     };
     unsigned mask = 0x00780078u;
     asm volatile("" : "+v"(mask));
@@ -283,9 +288,7 @@ template <int XTY, bool SW, int T, int P, int SB, int SUB, bool MP> __device__ _
             float tot = 0.f;
 #pragma unroll
             for (int b = 0; b < BPC; b++) {
-                unsigned sr = it.s[b], zr = it.z[b];
-                if (BPC > 1 && SB == 2 && a.vec) sr = it.s[b / 2] >> 16 * (b & 1), zr = it.z[b / 2] >> 16 * (b & 1);
-                const float sc = up_scale(sr), zo = 16.f + (a.zeros ? up_scale(zr) : 8.f);
+                const float sc = scale_at<SB>(a, it.s, b, BPC > 1), zo = 16.f + (a.zeros ? scale_at<SB>(a, it.z, b, BPC > 1) : 8.f);
                 const bool in = (((MP ? pass * NW : 0) + wave) * 4 + g) * 128 + b * SUB < a.cols;
                 float d = keep[b][t * P];
 #pragma unroll
@@ -358,13 +361,15 @@ LE_G4Q(bf16, 30, false, 1, 1)
 LE_G4Q(f32w, 0, true, 1, 3)
 LE_G4Q(f16w, 1, true, 1, 2)
 LE_G4Q(bf16w, 30, true, 1, 2)
-LE_G4Q(f16t2, 1, false, 2, 2)
-LE_G4Q(bf16t4, 30, false, 4, 1)
+#define LE_G4Q_FEW(NAME, XTY, SW, T, P) LE_G4Q1(NAME, XTY, SW, T, P, 2, 64) LE_G4Q1(NAME, XTY, SW, T, P, 2, 128) LE_G4Q1(NAME, XTY, SW, T, P, 4, 64) LE_G4Q1(NAME, XTY, SW, T, P, 4, 128)
+LE_G4Q_FEW(f16t2, 1, false, 2, 2)
+LE_G4Q_FEW(bf16t4, 30, false, 4, 1)
 
 /* ---- more tokens: activations laid out by a launch of their own ----
  *
- * le_g4x_*: the activations of 16 tokens (a tile) as MFMA fragments in the workspace, [chunk of 128 columns][MFMA j][piece][lane
- * group][token], 16 bytes each; SwiGLU and the cut into pieces are thus done once a launch and not once a block. The pieces are
+ * le_g4x_*: the activations as MFMA fragments in the workspace, 16 bytes a lane: up to 16 virtual rows (tokens times pieces, a.na sets of
+ * four) as le_g4t_* takes them, [slice of 512 columns][MFMA j][set][lane]; more tokens as le_g4m_* does, tiles of 16,
+ * [chunk of 128 columns][MFMA j][piece][lane group][token]. SwiGLU and the cut into pieces are thus done once a launch and not once a block. The pieces are
  * fp16 here, of the chunk's activations times the power of two that brings the largest to [2^14, 2^15): one piece holds bf16 and fp16, two hold
  * 22 bits (fp32 and SwiGLU's result; what is cut off is below 2^-23 of the value, or 2^-39 of the chunk's largest), where bf16
  * would take three. Beside them the powers' reciprocals, [chunk][16 tokens]. A thread takes an octet of a token. */
@@ -406,6 +411,12 @@ template <int XTY, bool SW, int P, int SUB> __device__ __forceinline__ void g4x_
     const int hi = (oc >> 2) & 3, lo = oc & 3;
     const int j = SUB == 128 ? lo : SUB == 64 ? 2 * (hi >> 1) + (lo & 1) : hi, g = SUB == 128 ? hi : SUB == 64 ? (hi & 1) + 2 * (lo >> 1) : lo;
     uint4 *frag = (uint4 *)ws + (size_t)no * P * tile * 16 + ((size_t)((oc >> 4) * 4 + j) * P * 4 + g) * tm + (tok & 15);
+    int step = 4 * tm; /* from piece to piece */
+    if (a.na) {
+        const int v = tok * P; /* a token's pieces lie in one set: sets are four rows, P is 1 or 2 */
+        frag = (uint4 *)ws + ((size_t)((oc >> 6) * 4 + j) * a.na + (v >> 2)) * 64 + g * 16 + ((oc >> 4) & 3) * 4 + (v & 3);
+        step = 1;
+    }
 #pragma unroll
     for (int k = 0; k < 8; k++) f[k] *= up;
 #pragma unroll
@@ -417,13 +428,166 @@ template <int XTY, bool SW, int P, int SUB> __device__ __forceinline__ void g4x_
             f[k] -= (float)h[k];
         }
         auto two = [&](int k) { return __builtin_bit_cast(unsigned, (f16x2){h[k], h[k + 4]}); };
-        frag[p * 4 * tm] = make_uint4(two(0), two(1), two(2), two(3));
+        frag[p * step] = make_uint4(two(0), two(1), two(2), two(3));
     }
     if ((oc & 15) == 0) {
         float *downs = (float *)(ws + a.ws_downs) + ((size_t)tile * nc + (oc >> 4)) * 16;
         downs[tok & 15] = down;
         if (tok == a.m - 1)
             for (int t = tm; t < 16; t++) downs[t] = 0.f;
+    }
+}
+
+/* Eight codes as fp16 16 + code (k: 0x03C003C0, as in unpack). */
+static __device__ __forceinline__ f16x8 unpack16(unsigned q, unsigned k) {
+    const unsigned o = 0x4C004C00u; /* 16; a step of the last place is 2^-6 */
+    return __builtin_bit_cast(f16x8, make_uint4(((q << 6) & k) | o, ((q << 2) & k) | o, ((q >> 2) & k) | o, ((q >> 6) & k) | o));
+}
+static __device__ __forceinline__ f32x4 mfma16(const uint4 &a, const f16x8 &b, const f32x4 &c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), b, c, 0, 0, 0);
+}
+
+/* le_g4t_*: le_g4q_*'s layout with NA sets of four virtual rows, from the workspace; K in segments of a block's waves where it is
+ * longer than they hold, whose partial results le_g4s adds. Against the layout of le_g4m_* it has fewer vector instructions (a lane
+ * applies scale and zero point to one K part of one row, not to every one) and longer runs of a row's codes, for MFMAs that a few
+ * tokens leave idle. */
+template <int NA, int P, int SB, int SUB> __device__ __forceinline__ void g4t_body(const G4Args &a) {
+    constexpr int BPC = 128 / SUB, T = 4 / P, NT = NA * T;
+    struct Item {
+        uint4 q[4];
+        unsigned s[BPC], z[BPC];
+    };
+    extern __shared__ __align__(16) unsigned char lds[];
+    float *red = (float *)lds; /* [group][wave][token][64] */
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), NW = a.nw;
+    const int n = lane & 15, g = lane >> 4, s = blockIdx.y, seg = blockIdx.z, groups = (a.rows + 15) >> 4;
+    const int mat = a.sel ? a.sel[s] : s;
+    auto store = [&](int t, int r, float v) {
+        const size_t yo = ((size_t)s * a.m + t) * a.rows + r;
+        if (a.segs > 1) a.part[(size_t)seg * a.total + yo] = v;
+        else if (a.xty == 0) ((float *)a.y)[yo] = v;
+        else ((unsigned short *)a.y)[yo] = a.xty == 1 ? XT<1>::down(v) : XT<30>::down(v);
+    };
+    if (mat < 0 || mat >= a.n_mat) { /* uniform over the block */
+        for (int gr = blockIdx.x; gr < groups; gr += a.gx)
+            if (threadIdx.x < 16 && gr * 16 + (int)threadIdx.x < a.rows)
+                for (int t = 0; t < a.m; t++) store(t, gr * 16 + threadIdx.x, 0.f);
+        return;
+    }
+    const int nc = (a.cols + 127) >> 7, ns = (nc + 3) >> 2, G = a.per - ((int)blockIdx.x >= a.full ? 1 : 0);
+    const int sl = seg * NW + wave, slc = min(sl, ns - 1); /* a slice that is not there: no codes are read, and its result is left out */
+    const unsigned char *ws = (const unsigned char *)a.ws + (size_t)(s / a.share) * a.ws_set;
+    const uint4 *frag = (const uint4 *)ws + (size_t)slc * 4 * NA * 64 + lane;
+    const float *downs = (const float *)(ws + a.ws_downs) + (size_t)min(slc * 4 + g, nc - 1) * 16;
+    uint4 x[NA][4];
+    float down[NT];
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+#pragma unroll
+        for (int v = 0; v < NA; v++) x[v][j] = frag[(j * NA + v) * 64];
+#pragma unroll
+    for (int t = 0; t < NT; t++) down[t] = downs[t];
+    __builtin_amdgcn_sched_barrier(0); /* loads return in order: these first */
+
+    const unsigned rowb = a.cols >> 1, bytes = a.rows * rowb, sbytes = a.rows * a.ng * SB; /* of the matrix: below 4 GiB */
+    unsigned vo[4];
+#pragma unroll
+    for (int u = 0; u < 4; u++) vo[u] = (4 * u + (n >> 2)) * rowb + sl * 256 + ((n + u) & 3) * 64 + g * 16;
+    const int us = (g - n) & 3, myrow = 4 * us + (n >> 2); /* the step whose result this lane keeps, and its row */
+    const unsigned char *w0 = a.codes + (size_t)mat * bytes, *s0 = (const unsigned char *)a.scales + (size_t)mat * sbytes,
+                        *z0 = (const unsigned char *)a.zeros + (size_t)mat * sbytes;
+    auto load = [&](Item &it, int gi) {
+        const int gr = (int)blockIdx.x + gi * a.gx;
+        const bool there = gi < G && sl < ns;
+        const auto rq = rsrc(w0, there ? bytes : 0), rs = rsrc(s0, there ? sbytes : 0), rz = rsrc(z0, there && a.zeros ? sbytes : 0);
+        if (BPC > 1 && a.vec) {
+            const unsigned off = ((gr * 16 + myrow) * a.ng + min((sl * 4 + g) * BPC, a.ng - BPC)) * SB;
+            load_scales<BPC, SB>(it.s, rs, off);
+            load_scales<BPC, SB>(it.z, rz, off);
+        } else {
+#pragma unroll
+            for (int b = 0; b < BPC; b++) {
+                const unsigned off = ((gr * 16 + myrow) * a.ng + (min((sl * 4 + g) * 128 + b * SUB, a.cols - 1) >> a.gshift)) * SB;
+                it.s[b] = load_scale<SB>(rs, off);
+                it.z[b] = load_scale<SB>(rz, off);
+            }
+        }
+        const unsigned go = gr * 16 * rowb;
+#pragma unroll
+        for (int u = 0; u < 4; u++) it.q[u] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rq, vo[u] + go, 0, 2 /* nt */));
+    };
+    unsigned mask = 0x03C003C0u;
+    asm volatile("" : "+v"(mask));
+    auto work = [&](Item &it, int gi, const float (&xs)[BPC][NT]) {
+        float keep[BPC][NA * 4];
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            spread<SUB>(it.q[u]);
+            const unsigned qw[4] = {it.q[u].x, it.q[u].y, it.q[u].z, it.q[u].w};
+#pragma unroll
+            for (int b = 0; b < BPC; b++) {
+                f32x4 d[NA];
+#pragma unroll
+                for (int v = 0; v < NA; v++) d[v] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int j = b * (4 / BPC); j < (b + 1) * (4 / BPC); j++) {
+                    const f16x8 w = unpack16(qw[j], mask);
+#pragma unroll
+                    for (int v = 0; v < NA; v++) d[v] = mfma16(x[v][j], w, d[v]);
+                }
+#pragma unroll
+                for (int i = 0; i < NA * 4; i++) keep[b][i] = u == 0 || u == us ? d[i / 4][i % 4] : keep[b][i];
+            }
+        }
+        float tot[NT] = {};
+#pragma unroll
+        for (int b = 0; b < BPC; b++) {
+            const float sc = scale_at<SB>(a, it.s, b, BPC > 1), zo = 16.f + (a.zeros ? scale_at<SB>(a, it.z, b, BPC > 1) : 8.f);
+            const bool in = (sl * 4 + g) * 128 + b * SUB < a.cols;
+#pragma unroll
+            for (int t = 0; t < NT; t++) {
+                const float d = P == 2 ? keep[b][2 * t] + keep[b][2 * t + 1] : keep[b][t], v = sc * __builtin_fmaf(-zo, xs[b][t], d);
+                tot[t] += in ? v : 0.f;
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < NT; t++) red[((gi * NW + wave) * NT + t) * 64 + myrow * 4 + g] = tot[t] * down[t];
+    };
+    Item A, B;
+    load(A, 0);
+    load(B, 1);
+    float xs[BPC][NT]; /* sums of the activations over the scale blocks, where the results lie: the same MFMAs with codes of 1 */
+    {
+        const unsigned one = 0x3C003C00u;
+        const f16x8 ones = __builtin_bit_cast(f16x8, make_uint4(one, one, one, one));
+#pragma unroll
+        for (int b = 0; b < BPC; b++)
+#pragma unroll
+            for (int v = 0; v < NA; v++) {
+                f32x4 d = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int j = b * (4 / BPC); j < (b + 1) * (4 / BPC); j++) d = mfma16(x[v][j], ones, d);
+#pragma unroll
+                for (int t = 0; t < T; t++) xs[b][v * T + t] = P == 2 ? d[(2 * t) & 3] + d[(2 * t + 1) & 3] : d[t];
+            }
+    }
+    for (int gi = 0;; gi += 2) {
+        work(A, gi, xs);
+        if (gi + 1 >= G) break;
+        load(A, gi + 2);
+        work(B, gi + 1, xs);
+        if (gi + 2 >= G) break;
+        load(B, gi + 3);
+    }
+    __syncthreads();
+    for (int i = wave; i < G * NT; i += NW) { /* the waves' partial results, added in wave order */
+        const int gi = i / NT, t = i % NT, r = ((int)blockIdx.x + gi * a.gx) * 16 + (lane >> 2);
+        if (t >= a.m) continue;
+        float v = red[(gi * NW * NT + t) * 64 + lane];
+        for (int w = 1; w < NW; w++) v += red[((gi * NW + w) * NT + t) * 64 + lane];
+        v += flt(__builtin_amdgcn_mov_dpp(bits(v), 0xB1, 0xf, 0xf, true)); /* quad lanes 1 0 3 2 */
+        v += flt(__builtin_amdgcn_mov_dpp(bits(v), 0x4E, 0xf, 0xf, true)); /* quad lanes 2 3 0 1 */
+        if (r < a.rows && (lane & 3) == 0) store(t, r, v);
     }
 }
 
@@ -434,13 +598,6 @@ template <int XTY, bool SW, int P, int SUB> __device__ __forceinline__ void g4x_
  * rows, one pass's at a time (4096 x 14336, five tokens: 29 us). The scales of
  * an item are loaded once by the lane groups together and passed between them: loaded by each lane group they were a third of the
  * time (14336 x 4096 bf16, five tokens 18.4 us, 12.6 without those loads). */
-static __device__ __forceinline__ f16x8 unpack16(unsigned q, unsigned k) {
-    const unsigned o = 0x4C004C00u; /* 16; a step of the last place is 2^-6 */
-    return __builtin_bit_cast(f16x8, make_uint4(((q << 6) & k) | o, ((q << 2) & k) | o, ((q >> 2) & k) | o, ((q >> 6) & k) | o));
-}
-static __device__ __forceinline__ f32x4 mfma16(const uint4 &a, const f16x8 &b, const f32x4 &c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), b, c, 0, 0, 0);
-}
 template <int P, int SB, int SUB, int CS> __device__ __forceinline__ void g4m_body(const G4Args &a) {
     constexpr int BPC = 128 / SUB, NSUB = CS * BPC, NL = NSUB < 4 ? 1 : NSUB / 4; /* scale blocks of an item's row, of them a lane's to load */
     struct Item {
@@ -454,7 +611,7 @@ template <int P, int SB, int SUB, int CS> __device__ __forceinline__ void g4m_bo
     const int mat = a.sel ? a.sel[s] : s;
     auto store = [&](int t, int r, float v) {
         const size_t yo = ((size_t)s * a.m + t0 + t) * a.rows + r;
-        if (a.segs > 1) a.part[(size_t)seg * gridDim.y * a.m * a.rows + yo] = v;
+        if (a.segs > 1) a.part[(size_t)seg * a.total + yo] = v;
         else if (a.xty == 0) ((float *)a.y)[yo] = v;
         else ((unsigned short *)a.y)[yo] = a.xty == 1 ? XT<1>::down(v) : XT<30>::down(v);
     };
@@ -491,30 +648,14 @@ template <int P, int SB, int SUB, int CS> __device__ __forceinline__ void g4m_bo
         const int b0 = c0 * BPC + (NSUB < 4 ? g % NSUB : g * NL);
         if (NL > 1 && a.vec) {
             const unsigned off = ((gr * 16 + n) * a.ng + min(b0, a.ng - NL)) * SB;
-            auto wide = [&](unsigned (&d)[NL], __amdgpu_buffer_rsrc_t r) {
-                if constexpr (NL * SB == 16) {
-                    const auto v = __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0);
-                    d[0] = v[0], d[1] = v[1], d[2] = v[2], d[3] = v[3];
-                } else if constexpr (NL * SB == 8) {
-                    const auto v = __builtin_amdgcn_raw_buffer_load_b64(r, off, 0, 0);
-                    d[0] = v[0], d[1] = v[1];
-                } else if constexpr (NL * SB == 4) {
-                    d[0] = __builtin_amdgcn_raw_buffer_load_b32(r, off, 0, 0);
-                }
-            };
-            wide(it.s, rs);
-            wide(it.z, rz);
+            load_scales<NL, SB>(it.s, rs, off);
+            load_scales<NL, SB>(it.z, rz, off);
         } else {
 #pragma unroll
             for (int k = 0; k < NL; k++) {
                 const unsigned off = ((gr * 16 + n) * a.ng + (min((b0 + k) * SUB, a.cols - 1) >> a.gshift)) * SB;
-                if constexpr (SB == 4) {
-                    it.s[k] = __builtin_amdgcn_raw_buffer_load_b32(rs, off, 0, 0);
-                    it.z[k] = __builtin_amdgcn_raw_buffer_load_b32(rz, off, 0, 0);
-                } else {
-                    it.s[k] = __builtin_amdgcn_raw_buffer_load_b16(rs, off, 0, 0);
-                    it.z[k] = __builtin_amdgcn_raw_buffer_load_b16(rz, off, 0, 0);
-                }
+                it.s[k] = load_scale<SB>(rs, off);
+                it.z[k] = load_scale<SB>(rz, off);
             }
         }
         const unsigned go = gr * 16 * rowb + c0 * 64;
@@ -522,20 +663,14 @@ template <int P, int SB, int SUB, int CS> __device__ __forceinline__ void g4m_bo
         for (int c = 0; c < CS; c++)
             it.q[c] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rq, c0 + c < nc ? vo + go + c * 64 : 0xFFFFFFF0u, 0, 2 /* nt */));
     };
-    auto up_scale = [&](unsigned v) {
-        if constexpr (SB == 4) return flt(v);
-        else return a.sty == 1 ? XT<1>::up((unsigned short)v) : XT<30>::up((unsigned short)v);
-    };
     unsigned mask = 0x03C003C0u;
     asm volatile("" : "+v"(mask));
     auto work = [&](Item &it, int gi, const f32x4 (&sum)[CS][BPC]) {
         float sc[NL], zo[NL]; /* this lane's blocks, scale and 16 + zero point */
 #pragma unroll
         for (int k = 0; k < NL; k++) {
-            unsigned sr = it.s[k], zr = it.z[k];
-            if (NL > 1 && SB == 2 && a.vec) sr = it.s[k / 2] >> 16 * (k & 1), zr = it.z[k / 2] >> 16 * (k & 1);
-            sc[k] = up_scale(sr);
-            zo[k] = 16.f + (a.zeros ? up_scale(zr) : 8.f);
+            sc[k] = scale_at<SB>(a, it.s, k, NL > 1);
+            zo[k] = 16.f + (a.zeros ? scale_at<SB>(a, it.z, k, NL > 1) : 8.f);
         }
         f32x4 tot = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -609,33 +744,24 @@ template <int P, int SB, int SUB, int CS> __device__ __forceinline__ void g4m_bo
     extern "C" __global__ void __launch_bounds__(256) le_g4x_##NAME##_b64(G4Args a) { g4x_body<XTY, SW, P, 64>(a); }   \
     extern "C" __global__ void __launch_bounds__(256) le_g4x_##NAME##_b128(G4Args a) { g4x_body<XTY, SW, P, 128>(a); }
 LE_G4X(f32, 0, false, 2) LE_G4X(f16, 1, false, 1) LE_G4X(bf16, 30, false, 1) LE_G4X(f32w, 0, true, 2) LE_G4X(f16w, 1, true, 2) LE_G4X(bf16w, 30, true, 2)
+#define LE_G4T1(NA, P, SB, SUB) \
+    extern "C" __global__ void __launch_bounds__(512) le_g4t_n##NA##_p##P##_s##SB##_b##SUB(G4Args a) { g4t_body<NA, P, SB, SUB>(a); }
+#define LE_G4T(NA, P) \
+    LE_G4T1(NA, P, 2, 32) LE_G4T1(NA, P, 2, 64) LE_G4T1(NA, P, 2, 128) LE_G4T1(NA, P, 4, 32) LE_G4T1(NA, P, 4, 64) LE_G4T1(NA, P, 4, 128)
+LE_G4T(1, 1) LE_G4T(2, 1) LE_G4T(1, 2) LE_G4T(2, 2)
+LE_G4T1(3, 2, 2, 64) LE_G4T1(3, 2, 2, 128) LE_G4T1(3, 2, 4, 64) LE_G4T1(3, 2, 4, 128)
 #define LE_G4M1(P, SB, SUB, CS) \
     extern "C" __global__ void __launch_bounds__(512) le_g4m_p##P##_s##SB##_b##SUB(G4Args a) { g4m_body<P, SB, SUB, CS>(a); }
 LE_G4M1(1, 2, 32, 4) LE_G4M1(1, 2, 64, 4) LE_G4M1(1, 2, 128, 4) LE_G4M1(1, 4, 32, 4) LE_G4M1(1, 4, 64, 4) LE_G4M1(1, 4, 128, 4)
 LE_G4M1(2, 2, 32, 2) LE_G4M1(2, 2, 64, 4) LE_G4M1(2, 2, 128, 4) LE_G4M1(2, 4, 32, 2) LE_G4M1(2, 4, 64, 4) LE_G4M1(2, 4, 128, 4)
 
-/* le_g4s: the segments' partial results added in their order and rounded, four values a thread (the last ones one by one). */
+/* le_g4s: the segments' partial results added in their order and rounded, a value a thread. */
 extern "C" __global__ void __launch_bounds__(256) le_g4s(G4Args a) {
-    const size_t n = (size_t)a.total, i0 = ((size_t)blockIdx.x * 256 + threadIdx.x) * 4;
-    float v[4] = {0.f, 0.f, 0.f, 0.f};
-    const bool four = n % 4 == 0;
-    if (i0 >= n) return;
-    if (four) {
-        for (int s = 0; s < a.segs; s++) {
-            const f32x4 p = *(const f32x4 *)(a.part + (size_t)s * n + i0);
-#pragma unroll
-            for (int k = 0; k < 4; k++) v[k] += p[k];
-        }
-    } else {
-        for (int s = 0; s < a.segs; s++)
-#pragma unroll
-            for (int k = 0; k < 4; k++)
-                if (i0 + k < n) v[k] += a.part[(size_t)s * n + i0 + k];
-    }
-#pragma unroll
-    for (int k = 0; k < 4; k++)
-        if (i0 + k < n) {
-            if (a.xty == 0) ((float *)a.y)[i0 + k] = v[k];
-            else ((unsigned short *)a.y)[i0 + k] = a.xty == 1 ? XT<1>::down(v[k]) : XT<30>::down(v[k]);
-        }
+    const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x, n = (size_t)a.total;
+    if (i >= n) return;
+    float v = a.part[i];
+#pragma unroll 4
+    for (int s = 1; s < a.segs; s++) v += a.part[(size_t)s * n + i];
+    if (a.xty == 0) ((float *)a.y)[i] = v;
+    else ((unsigned short *)a.y)[i] = a.xty == 1 ? XT<1>::down(v) : XT<30>::down(v);
 }

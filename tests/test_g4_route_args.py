@@ -88,6 +88,40 @@ def test_g4_refusals(lib, ctx, bad, code):
     assert lib.le_matvec_g4(None, None, None, 1, 1, 0, None, 0, 1, None, 0, None, 0, None) == -1
 
 
+def test_every_launched_kernel_is_built(lib):
+    """The kernels that any type, group and number of tokens selects are in the code objects, within the launch limits."""
+    objects = b"".join(open(os.path.join(qmm.LIB_DIR, "le_qmm_%s.hsaco" % p), "rb").read() for p in ("g4", "rt"))
+    seen = set()
+
+    def collect(c):
+        for name, g, block, lds in c.calls():
+            assert g[0] * block < 2**32 and g[1] <= 65535 and g[2] <= 65535 and min(g) > 0 and block <= 1024 and lds <= 160 * 1024, (name, g, block, lds)
+            seen.add(name)
+
+    for xtype in (0, 1, 30):
+        for stype in (0, 1, 30):
+            for swiglu in (0, 1):
+                for cols, group in ((32, 32), (4096, 32), (9216, 32), (4160, 64), (9216, 64), (4096, 128), (12288 + 128, 128), (4000, 4000), (65536, 256)):
+                    for m in (1, 2, 3, 4, 5, 6, 7, 8, 9, 16, 17, 64):
+                        c = Ctx()
+                        assert g4(lib, c, xtype=xtype, stype=stype, swiglu=swiglu, cols=cols, group=group, xstride=cols * (1 + swiglu), m=m, rows=5000) == 0
+                        collect(c)
+        for n_tok in (1, 5000):
+            for n_exp in (1, 32, 64, 128, 256, 500, 1024):
+                c = Ctx()
+                assert lib.le_moe_route(ctypes.addressof(c), xtype, A, n_tok, n_exp, 1, A, A, None) == 0
+                assert lib.le_moe_route_bwd(ctypes.addressof(c), xtype, A, A, A, n_tok, n_exp, 1, A, None) == 0
+                assert lib.le_moe_sort(ctypes.addressof(c), A, n_tok, 4, n_exp, A, A, A, A, A, 1 << 30, None) == 0
+                collect(c)
+            for cols, ld in ((8, 8), (100, 104), (256, 256), (2048, 2048), (2047, 2047), (100000, 100000)):
+                c, k = Ctx(), 4
+                assert lib.le_moe_permute(ctypes.addressof(c), xtype, A, ld, A, n_tok, k, cols, A, ld, 9, None) == 0
+                assert lib.le_moe_combine(ctypes.addressof(c), xtype, A, ld, 9, A, A, n_tok, k, cols, A, ld, None) == 0
+                assert lib.le_moe_combine_bwd(ctypes.addressof(c), xtype, A, ld, A, ld, 9, A, A, n_tok, k, cols, A, A, None) == 0
+                collect(c)
+    assert len(seen) > 100 and not [n for n in seen if (n + ".kd").encode() not in objects]
+
+
 @pytest.mark.parametrize("good", [
     dict(), dict(zeros=None), dict(sel=None), dict(xstride=0), dict(group=256), dict(cols=96, group=96), dict(cols=96, group=32), dict(cols=32, group=32),
     dict(m=64), dict(slots=65535), dict(swiglu=1, xstride=512), dict(xtype=30, stype=30, y=A + 2, scales=A + 2), dict(rows=1), dict(rows=2**24, n_mat=1), dict(m=4, xtype=30, ws=None), dict(m=2, xtype=1, ws=None), dict(m=64, cols=2**20, group=2**20, xstride=2**20), dict(m=17, slots=900, cols=14336, xstride=14336),
@@ -104,7 +138,8 @@ def test_g4_workspace(lib):
         s = qmm._G4(A, A, A, 4, rows, cols, group, 1)
         return lib.le_matvec_g4_workspace_size(ctypes.addressof(s) if w else None, xtype, m, slots, share, swiglu)
 
-    assert f(0, 1, 4096, 8, 1, 1) == 0 and f(30, 4, 4096, 1, 1, 0) == 0 and f(1, 2, 4096, 1, 1, 0) == 0  # one launch
+    assert f(0, 1, 4096, 8, 1, 1) == 0 and f(30, 4, 4096, 1, 1, 0) == 0 and f(1, 2, 4096, 1, 1, 0) == 0 and f(30, 1, 4096, 1, 1, 0, group=32) == 0  # one launch
+    assert f(30, 2, 4096, 1, 1, 0, group=32) >= 2 * 4096 * 2
     assert f(0, 2, 4096, 1, 1, 0) >= 2 * 4096 * 4 and f(30, 5, 4096, 1, 1, 0) >= 5 * 4096 * 2 and f(1, 3, 4096, 1, 1, 0) >= 3 * 4096 * 2
     assert f(0, 2, 4096, 8, 2, 0) == 4 * f(0, 2, 4096, 1, 1, 0)  # sets of activations
     assert f(0, 2, 14336, 3, 1, 0, rows=128) >= 3 * 2 * 14336 * 4 + 4 * 3 * 2 * 128 * 4  # and the partial results of K's segments
