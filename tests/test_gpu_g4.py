@@ -258,3 +258,85 @@ def test_refusals(engine):
                 (codes, scales.double(), None, 16, 64, 32), (codes.transpose(1, 2), scales, z, 16, 64, 32)):
         with pytest.raises(le.LeError):
             le.G4(*bad)
+
+
+@pytest.mark.parametrize("ty,m,cols", [(le.F32, 5, 9216), (le.BF16, 20, 640), (le.F16, 3, 4352)])
+def test_streams_and_workspaces(engine, ty, m, cols):
+    """On streams given as torch streams and as raw handles, with a workspace of the call's own or the caller's, all at once."""
+    import torch
+    rows, group = 200, 64
+    codes, scales, z = make(1, rows, cols, group, le.F16, True, 560)
+    w = le.G4(codes.cuda(), scales.cuda(), z.cuda(), rows, cols, group)
+    wf, mag = dequant(codes, scales, z, group)
+    xs = [torch.randn(m, cols, generator=torch.Generator().manual_seed(i)).to(torch_type(ty)) for i in range(4)]
+    dx = [x.cuda() for x in xs]
+    outs = [torch.full((m, rows), float("nan"), dtype=torch_type(ty), device="cuda") for _ in xs]
+    streams = [torch.cuda.Stream() for _ in xs]
+    torch.cuda.synchronize()
+    need = engine.mv_g4_workspace_size(ty, w, m)
+    assert need > 0
+    for i, s in enumerate(streams):
+        ws = torch.empty(need, dtype=torch.uint8, device="cuda") if i == 3 else None
+        if ws is not None:
+            ws.record_stream(s)
+        engine.mv_g4(ty, w, dx[i], outs[i], m=m, ws=ws, stream=s if i != 1 else s.cuda_stream)
+    engine.mv_g4(ty, w, dx[0], outs[2], m=m, stream=streams[2])  # behind the first on its stream
+    torch.cuda.synchronize()
+    for i, x in enumerate(xs):
+        a = xs[0].double() if i == 2 else x.double()
+        check(outs[i], a @ wf[0].t(), a.abs() @ mag[0].t(), ty, cols)
+    with pytest.raises(le.LeError) as e:
+        engine.mv_g4(ty, w, dx[0], outs[0], m=m, ws=torch.empty(need - 1, dtype=torch.uint8, device="cuda"))
+    assert e.value.code == -7
+
+
+@pytest.mark.parametrize("ty,m", [(le.F32, 1), (le.F32, 6), (le.BF16, 33)])
+def test_graph(engine, ty, m):
+    """Captured and replayed with new activations and selections, eager calls between."""
+    import torch
+    from tests.test_gpu_graphs import capture
+    n_mat, rows, cols, group = 3, 90, 4736, 128
+    codes, scales, z = make(n_mat, rows, cols, group, le.F16, True, 570)
+    w = le.G4(codes.cuda(), scales.cuda(), z.cuda(), rows, cols, group, n_mat=n_mat)
+    wf, mag = dequant(codes, scales, z, group)
+    x = torch.zeros(m, cols, dtype=torch_type(ty), device="cuda")
+    sel = torch.zeros(2, dtype=torch.int32, device="cuda")
+    out = torch.zeros(2, m, rows, dtype=torch_type(ty), device="cuda")
+    ws = torch.empty(max(16, engine.mv_g4_workspace_size(ty, w, m, 2, 2)), dtype=torch.uint8, device="cuda")
+    call = lambda s: engine.mv_g4(ty, w, x, out, m=m, slots=2, share=2, sel=sel, ws=ws, stream=s)  # noqa: E731
+    graph = capture(call)
+    for rep in range(4):
+        h = torch.randn(m, cols, generator=torch.Generator().manual_seed(rep)).to(torch_type(ty))
+        x.copy_(h)
+        sel.copy_(torch.tensor([rep % 3, (rep + 2) % 3 if rep else -1], dtype=torch.int32))
+        out.fill_(float("nan"))
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        got = out.clone()
+        call(None)
+        torch.cuda.synchronize()
+        assert torch.equal(got, out)
+        for s, mat in enumerate(sel.tolist()):
+            if mat < 0:
+                assert (got[s] == 0).all()
+            else:
+                check(got[s], h.double() @ wf[mat].t(), h.double().abs() @ mag[mat].t(), ty, cols)
+
+
+@pytest.mark.parametrize("ty", TYPES)
+@pytest.mark.parametrize("m", [1, 3, 9])
+def test_scales_that_are_not_finite(engine, ty, m):
+    """An infinite or NaN scale or zero point reaches its own row alone."""
+    import torch
+    rows, cols, group = 40, 320, 32
+    codes, scales, z = make(1, rows, cols, group, le.F16, True, 580)
+    clean = le.G4(codes.cuda(), scales.cuda(), z.cuda(), rows, cols, group)
+    s2, z2 = scales.clone(), z.clone()
+    s2[0, 7, 3], s2[0, 39, 9], z2[0, 16, 0] = float("inf"), float("nan"), float("-inf")
+    x = torch.randn(m, cols).to(torch_type(ty)).cuda()
+    a, b = (torch.empty(m, rows, dtype=torch_type(ty), device="cuda") for _ in range(2))
+    engine.mv_g4(ty, clean, x, a, m=m)
+    engine.mv_g4(ty, le.G4(codes.cuda(), s2.cuda(), z2.cuda(), rows, cols, group), x, b, m=m)
+    keep = [r for r in range(rows) if r not in (7, 16, 39)]
+    assert torch.equal(a[:, keep], b[:, keep]) and not torch.isfinite(b[:, [7, 16, 39]]).any()

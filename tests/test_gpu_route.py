@@ -451,3 +451,41 @@ def test_many_rows(engine, ty):
     grad = torch.zeros_like(e, dtype=torch.float64)
     grad[at[ok]] = (dout.double()[:, None] * ww[..., None])[ok]
     assert ((de.double() - grad).abs() <= (half_step(ty) + 2 * U) * grad.abs() + tiny(ty)).all()
+
+
+def test_more_tokens_than_blocks(engine):
+    """Token counts past the grids' limits, where blocks take several."""
+    import torch
+    n = (1 << 24) + 37  # sixteen tokens a block, 2^20 blocks
+    l = torch.randn(n, 3, device="cuda")
+    idx, w = torch.empty(n, 2, dtype=torch.int32, device="cuda"), torch.empty(n, 2, device="cuda")
+    print("route", n, flush=True)
+    engine.moe_route(le.F32, l, n, 3, 2, idx, w)
+    top, order = torch.sort(l, dim=-1, descending=True, stable=True)
+    assert torch.equal(idx, order[:, :2].int())
+    assert float((w - torch.softmax(top[:, :2].double(), -1)).abs().max()) <= 1e-5
+    dl = torch.empty(n, 3, device="cuda")
+    dw = torch.randn(n, 2, device="cuda")
+    engine.moe_route_bwd(le.F32, idx, w, dw, n, 3, 2, dl)
+    g = w.double() * (dw.double() - (w.double() * dw.double()).sum(-1, keepdim=True))
+    assert float((dl.double() - torch.zeros(n, 3, dtype=torch.float64, device="cuda").scatter_(1, idx.long(), g)).abs().max()) <= 1e-5
+    del l, top, order, g, dl
+    n, cols = (1 << 20) + 5, 520  # a block each
+    x = torch.randn(n, cols, device="cuda", dtype=torch.float32)
+    pos = torch.randperm(n, device="cuda").int()
+    pos[3] = -1
+    e, out = torch.zeros(n, cols, device="cuda"), torch.empty(n, cols, device="cuda")
+    print("rows", n, flush=True)
+    engine.moe_permute(le.F32, x, pos, n, 1, cols, e, n)
+    engine.moe_combine(le.F32, e, pos, None, n, 1, cols, out, n)
+    want = x.clone()
+    want[3] = 0
+    assert torch.equal(out, want)
+    w = torch.randn(n, device="cuda")
+    dw, de = torch.empty(n, device="cuda"), torch.zeros_like(e)
+    engine.moe_combine_bwd(le.F32, x, e, pos, w, n, 1, cols, de, dw, n)
+    sq = x.double().square().sum(1)
+    sq[3] = 0
+    assert ((dw.double() - sq).abs() <= (cols + 1) * U * sq).all()
+    engine.moe_combine(le.F32, de, pos, None, n, 1, cols, out, n)
+    assert ((out - want * w[:, None]).abs() <= 2 * U * (want * w[:, None]).abs() + 2.0 ** -126).all()
