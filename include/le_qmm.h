@@ -304,8 +304,8 @@ typedef struct le_g4 {
  * its token's outputs infinite or NaN. Limits: m <= 64, slots <= 65535, cols <= 2^24, slots * m * rows <= 2^31,
  * a matrix's codes and its scales each below 4 GiB; x 16-byte aligned, xstride a multiple of 16 bytes. y may not overlap an
  * input.
- * ws: le_matvec_g4_workspace_size bytes (16-byte aligned; NULL where that is 0: one token, and with groups of 64 or more
- * two in fp16 and up to four in bf16), which every call writes anew; calls that may overlap need workspaces of their own. */
+ * ws: le_matvec_g4_workspace_size bytes (16-byte aligned; NULL where that is 0: one token, and without SwiGLU two in fp16
+ * and up to four in bf16), which every call writes anew; calls that may overlap need workspaces of their own. */
 size_t le_matvec_g4_workspace_size(const le_g4 *w, int xtype, int m, int slots, int share, int swiglu);
 int le_matvec_g4(le_ctx *ctx, const le_g4 *w, const int *sel, int slots, int share, int xtype, const void *x,
                  long long xstride, int m, void *y, int swiglu, void *ws, size_t ws_bytes, le_stream_t stream);

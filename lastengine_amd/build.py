@@ -24,12 +24,13 @@ for _ty in (2, 8, 11, 12, 13, 14, 16, 18, 22):
     PARTS["mv%d" % _ty] = ["-DLE_PART_MV=%d" % _ty]
 PARTS["gm"] = []
 PARTS["mt"] = []
-PARTS["g4"] = []
+for _ty in (0, 1, 30):
+    PARTS["g4s%d" % _ty] = ["-DLE_G4_STY=%d" % _ty]
 PARTS["rt"] = []
 PARTS["gq"] = ["-DLE_GQ_SET=1"]
 PARTS["gq2"] = ["-DLE_GQ_SET=2"]
 SOURCES = {"gm": "le_gemm_kernels.hip", "mt": "le_mt_kernels.hip", "gq": "le_gq_kernels.hip", "gq2": "le_gq_kernels.hip",
-           "g4": "le_g4_kernels.hip", "rt": "le_route_kernels.hip"}  # parts not listed here compile le_qmm_kernels.hip
+           "g4s0": "le_g4_kernels.hip", "g4s1": "le_g4_kernels.hip", "g4s30": "le_g4_kernels.hip", "rt": "le_route_kernels.hip"}  # parts not listed here compile le_qmm_kernels.hip
 
 HOST_SOURCES = ["le_qmm.cpp", "le_g4.cpp", "le_route.cpp", "le_quant.cpp", "le_gguf.cpp"]
 # Host sources that declare device memory (hipcc, host and device passes), linked into the library.

@@ -17,31 +17,29 @@ bool aligned(const void *p, unsigned n) { return ((uintptr_t)p & (n - 1)) == 0; 
 int pieces(int xtype, int swiglu) { return xtype == LE_F32 ? 3 : xtype == LE_F16 || swiglu ? 2 : 1; }
 /* Columns that a scale is applied to at a time. */
 int scale_block(const le_g4 *w) { return w->group % 128 == 0 || w->group == w->cols ? 128 : w->group % 64 == 0 ? 64 : 32; }
-/* ... and the tokens of a slot that it takes (le_g4q_*, four virtual rows; with scale blocks of 32 columns two or more tokens' sums are
- * too many for it: 14336 x 4096 bf16, two to four tokens 21 us, in two launches 17.6). More need the activations laid out in the
- * workspace, as ... */
-int most_tokens(const le_g4 *w, int xtype, int swiglu) { return swiglu || scale_block(w) == 32 ? 1 : 4 / pieces(xtype, 0); }
+/* ... and the tokens of a slot that it takes (le_g4q_*, four virtual rows). More need the activations laid out in the workspace, as ... */
+int most_tokens(int xtype, int swiglu) { return swiglu ? 1 : 4 / pieces(xtype, 0); }
 /* ... fp16 pieces (le_g4x_*, le_g4m_*). */
 int pieces16(int xtype, int swiglu) { return xtype == LE_F32 || swiglu ? 2 : 1; }
-/* le_g4t_*: sets of four virtual rows, up to two, or three of two pieces a token and larger scale blocks; 0: le_g4m_*, whose rows are 16
- * tokens. 14336 x 4096 fp32, groups of 128, le_g4t_* / le_g4m_*: 2 tokens (one set) 11.5 / 15.7 us, 4 (two) 13.1 / 15.8, 5 (three)
- * 15.8 / 16.0, 8 (four) 17.1 / 16.0; bf16 8 (two) 13.9 / 14.5, 16 (four) 21.1 / 14.8; 4096 x 14336 SwiGLU, groups of 64: 5 tokens
- * 20.7 / 22.2, 8 25.4 / 22.5. */
-int row_sets(const le_g4 *w, int xtype, int swiglu, int m) {
+/* le_g4t_*: sets of four virtual rows, up to two, or three of two pieces a token; 0: le_g4m_*, whose rows are 16 tokens. 14336 x 4096,
+ * le_g4t_* / le_g4m_* in us, fp32, groups of 32, 64, 128: 2 tokens (one set) 12.5 / 18.9, 11.9 / 18.3, 11.1 / 15.8; 4 (two) 15.2 / 19.1,
+ * 13.8 / 18.1, 13.3 / 16.2; 5 (three) 18.0 / 19.4, 16.1 / 18.1, 15.7 / 16.1; 8 (four) 20.6 / 19.7, 18.4 / 18.1, 17.2 / 16.2; bf16, 8
+ * tokens (two) 16.5 / 17.9, 14.9 / 16.5, 14.2 / 14.6, 9 (three) 22.3 / 18.0, 19.5 / 16.6, 18.3 / 14.7. */
+int row_sets(int xtype, int swiglu, int m) {
     const int p = pieces16(xtype, swiglu), na = (m * p + 3) / 4;
-    return na <= 2 || (na == 3 && p == 2 && scale_block(w) > 32) ? na : 0;
+    return na <= 2 || (na == 3 && p == 2) ? na : 0;
 }
 /* Bytes of one set of activations: fragments, powers of two. */
-size_t frag_bytes(const le_g4 *w, int xtype, int swiglu, int m) {
-    const size_t nc = (size_t)(w->cols + 127) / 128;
-    if (const int na = row_sets(w, xtype, swiglu, m)) return (nc + 3) / 4 * 4096 * na;
+size_t frag_bytes(int xtype, int swiglu, int m, int cols) {
+    const size_t nc = (size_t)(cols + 127) / 128;
+    if (const int na = row_sets(xtype, swiglu, m)) return (nc + 3) / 4 * 4096 * na;
     return nc * 256 * pieces16(xtype, swiglu) * m;
 }
 size_t tile_floats(int m, int cols) { return (size_t)((m + 15) / 16) * ((cols + 127) / 128) * 16; }
-size_t set_bytes(const le_g4 *w, int xtype, int swiglu, int m) { return frag_bytes(w, xtype, swiglu, m) + tile_floats(m, w->cols) * 4; }
+size_t set_bytes(int xtype, int swiglu, int m, int cols) { return frag_bytes(xtype, swiglu, m, cols) + tile_floats(m, cols) * 4; }
 /* 128-column chunks that a wave keeps (le_g4m_*: two pieces' fragments of four and the sums over small scale blocks would not fit the
  * registers), and the segments of K that blocks of eight waves make of them. */
-int chunks(const le_g4 *w, int xtype, int swiglu, int m) { return !row_sets(w, xtype, swiglu, m) && pieces16(xtype, swiglu) == 2 && scale_block(w) == 32 ? 2 : 4; }
+int chunks(const le_g4 *w, int xtype, int swiglu, int m) { return !row_sets(xtype, swiglu, m) && pieces16(xtype, swiglu) == 2 && scale_block(w) == 32 ? 2 : 4; }
 int segments(const le_g4 *w, int xtype, int swiglu, int m) {
     const int most = 8 * chunks(w, xtype, swiglu, m);
     return ((w->cols + 127) / 128 + most - 1) / most;
@@ -62,9 +60,9 @@ const char *shape_error(const le_g4 *w, int slots, int share, int m) {
 }  // namespace
 
 extern "C" size_t le_matvec_g4_workspace_size(const le_g4 *w, int xtype, int m, int slots, int share, int swiglu) {
-    if (!w || !type_bytes(xtype) || !type_bytes(w->scale_type) || shape_error(w, slots, share, m) || m <= most_tokens(w, xtype, swiglu)) return 0;
+    if (!w || !type_bytes(xtype) || !type_bytes(w->scale_type) || shape_error(w, slots, share, m) || m <= most_tokens(xtype, swiglu)) return 0;
     const int segs = segments(w, xtype, swiglu, m);
-    return (size_t)((slots + share - 1) / share) * set_bytes(w, xtype, swiglu, m) + (segs > 1 ? (size_t)segs * slots * m * w->rows * 4 : 0);
+    return (size_t)((slots + share - 1) / share) * set_bytes(xtype, swiglu, m, w->cols) + (segs > 1 ? (size_t)segs * slots * m * w->rows * 4 : 0);
 }
 
 extern "C" int le_matvec_g4(le_ctx *c, const le_g4 *w, const int *sel, int slots, int share, int xtype, const void *x,
@@ -108,12 +106,14 @@ extern "C" int le_matvec_g4(le_ctx *c, const le_g4 *w, const int *sel, int slots
     if (w->group != w->cols)
         for (a.gshift = 5; 1 << a.gshift < w->group;) a.gshift++;
     a.xty = xtype;
-    a.sty = w->scale_type;
     const int sub = scale_block(w), bpc = 128 / sub;
-    a.vec = bpc > 1 && a.ng % bpc == 0 && aligned(w->scales, bpc * sb) && aligned(w->zeros, bpc * sb);
+    /* a 128-column part's scales and its zero points can be loaded at once */
+    const bool vec = bpc > 1 && a.ng % bpc == 0 && aligned(w->scales, bpc * sb) && aligned(w->zeros, bpc * sb);
+    char tail[16];
+    snprintf(tail, sizeof tail, "b%d%s", sub, vec ? "v" : "");
     const char *kind = xtype == LE_F32 ? "f32" : xtype == LE_F16 ? "f16" : "bf16";
     const long long groups = (w->rows + 15) / 16;
-    const int most = most_tokens(w, xtype, swiglu), sb2 = sb == 4 ? 4 : 2, P = pieces(xtype, swiglu);
+    const int most = most_tokens(xtype, swiglu), sty = w->scale_type, P = pieces(xtype, swiglu);
     char name[48];
     void *args[] = {&a};
     /* Row groups a block: so many that blocks of nw waves fill the chip with `waves` a CU, and LDS holds their partial results (lds bytes
@@ -132,14 +132,16 @@ extern "C" int le_matvec_g4(le_ctx *c, const le_g4 *w, const int *sel, int slots
         const int ns = (w->cols + 511) / 512, wmax = ns <= 8 || sub < 128 ? 8 : 16; /* slices of 512 columns */
         const int passes = (ns + wmax - 1) / wmax, nw = (ns + passes - 1) / passes, T = m == 1 ? 1 : most;
         const int quad = m == 1 && P > 1 ? nw * 4096 : 0;
-        share_out(nw, 16, slots, T * 256);
-        snprintf(name, sizeof name, "le_g4q_%s%s_s%d_b%d%s", kind, swiglu ? "w" : m == 1 ? "" : T == 2 ? "t2" : "t4", sb2, sub, passes > 1 || nw > 8 ? "_mp" : "");
+        /* 32 experts of 1536 x 2048 (four waves a block), 16 / 24 waves a CU: groups of 32 15.0 / 14.4 us, 128 12.1 / 11.7; 28672 x
+         * 4096 (eight) 13.1 / 14.6 */
+        share_out(nw, nw <= 4 ? 24 : 16, slots, T * 256);
+        snprintf(name, sizeof name, "le_g4q_%s%s_%s%s_s%d", kind, swiglu ? "w" : m == 1 ? "" : T == 2 ? "t2" : "t4", tail, passes > 1 || nw > 8 ? "_mp" : "", sty);
         return le_ctx_launch(c, name, dim3((unsigned)a.gx, (unsigned)slots), 64 * nw, (size_t)quad + (size_t)a.per * nw * T * 256, (hipStream_t)stream, args);
     }
     a.ws = (unsigned char *)ws;
-    a.ws_set = (long long)set_bytes(w, xtype, swiglu, m);
-    a.ws_downs = (long long)frag_bytes(w, xtype, swiglu, m);
-    a.na = row_sets(w, xtype, swiglu, m);
+    a.ws_set = (long long)set_bytes(xtype, swiglu, m, w->cols);
+    a.ws_downs = (long long)frag_bytes(xtype, swiglu, m, w->cols);
+    a.na = row_sets(xtype, swiglu, m);
     a.segs = segments(w, xtype, swiglu, m);
     const int sets = (slots + share - 1) / share, nc = (w->cols + 127) / 128, tiles = a.na ? 1 : (m + 15) / 16, cs = chunks(w, xtype, swiglu, m);
     a.part = (float *)(a.ws + sets * a.ws_set);
@@ -150,8 +152,8 @@ extern "C" int le_matvec_g4(le_ctx *c, const le_g4 *w, const int *sel, int slots
     /* waves: all of K's slices over the segments, evenly */
     const int nw = ((nc + cs - 1) / cs + a.segs - 1) / a.segs, p16 = pieces16(xtype, swiglu), lds = a.na ? a.na * 4 / p16 * 256 : 1024;
     share_out(nw, 8, (long long)slots * tiles * a.segs, lds);
-    if (a.na) snprintf(name, sizeof name, "le_g4t_n%d_p%d_s%d_b%d", a.na, p16, sb2, sub);
-    else snprintf(name, sizeof name, "le_g4m_p%d_s%d_b%d", p16, sb2, sub);
+    if (a.na) snprintf(name, sizeof name, "le_g4t_n%d_p%d_%s_s%d", a.na, p16, tail, sty);
+    else snprintf(name, sizeof name, "le_g4m_p%d_%s_s%d", p16, tail, sty);
     rc = le_ctx_launch(c, name, dim3((unsigned)a.gx, (unsigned)slots, (unsigned)(tiles * a.segs)), 64 * nw, (size_t)a.per * nw * lds, (hipStream_t)stream, args);
     if (rc || a.segs == 1) return rc;
     return le_ctx_launch(c, "le_g4s", dim3((unsigned)((a.total + 255) / 256)), 256, 0, (hipStream_t)stream, args);

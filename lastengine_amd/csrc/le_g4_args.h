@@ -10,7 +10,7 @@ struct G4Args {
     long long xstride; /* values */
     int n_mat, rows, cols, group, ng /* groups a row */, share, m;
     int gshift;        /* column >> gshift = group */
-    int xty, sty, vec;     /* types of x and y, of the scales; a 128-column part's scales and zeros can be loaded at once */
+    int xty;           /* type of x and y */
     int nw, gx;        /* waves of a block, blocks of a slot (from here: the launch's own cost a load each) */
     unsigned char *ws; /* le_g4x_*, le_g4t_*, le_g4m_*: fragments of a set of m tokens */
     long long ws_set, ws_downs; /* bytes of a set, before its powers of two */

@@ -30,7 +30,12 @@
  * The waves of a block split K, in passes where they are fewer than the slices, and go over the same row groups, each at its own
  * pace: partial results are kept in LDS, every lane's in a place of its own, and meet after one barrier, added in wave order.
  * Codes of the next two items are on their way while one is multiplied; loads of items that do not exist and of rows past the end
- * are cut off by the buffer's size and fetch nothing. */
+ * are cut off by the buffer's size and fetch nothing.
+ *
+ * One token, weights from HBM (a streaming read of as many bytes at this size): 28672 x 4096 bf16, groups of 128, 62 MB 13.1 us (11.8),
+ * 14336 x 4096 fp32 31 MB 8.2 (6.9), groups of 32 37 MB 9.4, 4096 x 4096 4.7 (3.5), 1024 x 2048 3.15 (2.7), 4096 x 14336 SwiGLU
+ * fp32, groups of 64, 33 MB 13.6 (7.3): there each of 256 blocks reads all of x, forms SwiGLU and goes over K twice for its
+ * 16 rows. What the types and groups choose is compiled in: as branches on arguments it cost 14336 x 4096 in groups of 32 5.6 us. */
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
@@ -109,37 +114,45 @@ template <int XTY> struct XOct {
     }
 };
 
-/* A scale or zero point as loaded (SB bytes), and N consecutive ones at once (16-bit ones two to a word). */
-template <int SB> static __device__ __forceinline__ unsigned load_scale(__amdgpu_buffer_rsrc_t r, unsigned off) {
-    if constexpr (SB == 4) return __builtin_amdgcn_raw_buffer_load_b32(r, off, 0, 0);
-    else return __builtin_amdgcn_raw_buffer_load_b16(r, off, 0, 0);
-}
-template <int N, int SB> static __device__ __forceinline__ void load_scales(unsigned (&d)[N], __amdgpu_buffer_rsrc_t r, unsigned off) {
-    if constexpr (N * SB == 16) {
-        const auto v = __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0);
-        d[0] = v[0], d[1] = v[1], d[2] = v[2], d[3] = v[3];
-    } else if constexpr (N * SB == 8) {
-        const auto v = __builtin_amdgcn_raw_buffer_load_b64(r, off, 0, 0);
-        d[0] = v[0], d[1] = v[1];
-    } else if constexpr (N * SB == 4) {
-        d[0] = __builtin_amdgcn_raw_buffer_load_b32(r, off, 0, 0);
+/* N scales or zero points of type STY as loaded: one by one, or at once from an address of that alignment (VEC; 16-bit ones then two to a
+ * word). Where there are no zero points the buffer is empty and 0 comes back. */
+template <int STY, int N, bool VEC> struct Scales {
+    static constexpr int SB = STY == 0 ? 4 : 2;
+    unsigned d[N];
+    /* of blocks b .. b + N - 1 (of `sub` columns) of the matrix row that begins at value `row` */
+    __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t r, unsigned row, int b, int sub, int cols, int gshift, int ng) {
+        if constexpr (VEC) {
+            const unsigned off = (row + min(b, ng - N)) * SB;
+            if constexpr (N * SB == 16) {
+                const auto v = __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0);
+                d[0] = v[0], d[1] = v[1], d[2] = v[2], d[3] = v[3];
+            } else if constexpr (N * SB == 8) {
+                const auto v = __builtin_amdgcn_raw_buffer_load_b64(r, off, 0, 0);
+                d[0] = v[0], d[1] = v[1];
+            } else {
+                d[0] = __builtin_amdgcn_raw_buffer_load_b32(r, off, 0, 0);
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < N; k++) {
+                const unsigned off = (row + (min((b + k) * sub, cols - 1) >> gshift)) * SB;
+                if constexpr (SB == 4) d[k] = __builtin_amdgcn_raw_buffer_load_b32(r, off, 0, 0);
+                else d[k] = __builtin_amdgcn_raw_buffer_load_b16(r, off, 0, 0);
+            }
+        }
     }
-}
-/* Value k of those; several: loaded at once where a.vec. */
-template <int SB, int N> static __device__ __forceinline__ float scale_at(const G4Args &a, const unsigned (&d)[N], int k, bool several) {
-    if constexpr (SB == 4) return flt(d[k]);
-    else {
-        const unsigned v = several && a.vec ? d[k / 2] >> 16 * (k & 1) : d[k];
-        return a.sty == 1 ? XT<1>::up((unsigned short)v) : XT<30>::up((unsigned short)v);
+    __device__ __forceinline__ float at(int k) const {
+        if constexpr (STY == 0) return flt(d[k]);
+        else return XT<STY>::up((unsigned short)(VEC && N > 1 ? d[k / 2] >> 16 * (k & 1) : d[k]));
     }
-}
+};
 
-/* SB: bytes of a scale; T tokens (at most); P pieces; T * P <= 4; MP: more slices than waves */
-template <int XTY, bool SW, int T, int P, int SB, int SUB, bool MP> __device__ __forceinline__ void g4q_body(const G4Args &a) {
-    constexpr int BPC = 128 / SUB, XB = XTY == 0 ? 4 : 2;
+/* STY: type of the scales; T tokens (at most); P pieces; T * P <= 4; MP: more slices than waves */
+template <int XTY, bool SW, int T, int P, int STY, int SUB, bool VEC, bool MP> __device__ __forceinline__ void g4q_body(const G4Args &a) {
+    constexpr int BPC = 128 / SUB, XB = XTY == 0 ? 4 : 2, SB = STY == 0 ? 4 : 2;
     struct Item {
         uint4 q[4];
-        unsigned s[BPC], z[BPC]; /* 16-bit ones of a part loaded at once: two to a word */
+        Scales<STY, BPC, VEC> s, z;
     };
     constexpr bool QUAD = T == 1 && P > 1;  /* lane i of four takes octet i for all of them, exchanged through LDS */
     extern __shared__ __align__(16) unsigned char lds[]; /* QUAD: [wave][octet][kappa][g][piece] octets; then [group][wave][token][64] sums */
@@ -237,6 +250,7 @@ template <int XTY, bool SW, int T, int P, int SB, int SUB, bool MP> __device__ _
         }
     };
 
+    const float zbase = a.zeros ? 16.f : 24.f;
     const unsigned rowb = a.cols >> 1;
     unsigned vo[4];
 #pragma unroll
@@ -249,19 +263,9 @@ template <int XTY, bool SW, int T, int P, int SB, int SUB, bool MP> __device__ _
         const int gr = (int)blockIdx.x + gi * a.gx, sl = (MP ? pass * NW : 0) + wave;
         there = there && sl < ns;
         const auto rq = rsrc(w0, there ? bytes : 0), rs = rsrc(s0, there ? sbytes : 0), rz = rsrc(z0, there && a.zeros ? sbytes : 0);
-        if (BPC > 1 && a.vec) { /* one load for a part's blocks: a quarter of the requests (groups of 32) */
-            const unsigned off = ((gr * 16 + myrow) * a.ng + min((sl * 4 + g) * BPC, a.ng - BPC)) * SB;
-            load_scales<BPC, SB>(it.s, rs, off);
-            load_scales<BPC, SB>(it.z, rz, off);
-        } else {
-#pragma unroll
-            for (int b = 0; b < BPC; b++) {
-                const int col = (sl * 4 + g) * 128 + b * SUB;
-                const unsigned off = ((gr * 16 + myrow) * a.ng + (min(col, a.cols - 1) >> a.gshift)) * SB;
-                it.s[b] = load_scale<SB>(rs, off);
-                it.z[b] = load_scale<SB>(rz, off);
-            }
-        }
+        const unsigned row = (gr * 16 + myrow) * a.ng;
+        it.s.load(rs, row, (sl * 4 + g) * BPC, SUB, a.cols, a.gshift, a.ng);
+        it.z.load(rz, row, (sl * 4 + g) * BPC, SUB, a.cols, a.gshift, a.ng);
         const unsigned go = gr * 16 * rowb + sl * 256;
 #pragma unroll
         for (int u = 0; u < 4; u++) it.q[u] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rq, vo[u] + go, 0, 2 /* nt */));
@@ -288,7 +292,7 @@ template <int XTY, bool SW, int T, int P, int SB, int SUB, bool MP> __device__ _
             float tot = 0.f;
 #pragma unroll
             for (int b = 0; b < BPC; b++) {
-                const float sc = scale_at<SB>(a, it.s, b, BPC > 1), zo = 16.f + (a.zeros ? scale_at<SB>(a, it.z, b, BPC > 1) : 8.f);
+                const float sc = it.s.at(b), zo = zbase + it.z.at(b);
                 const bool in = (((MP ? pass * NW : 0) + wave) * 4 + g) * 128 + b * SUB < a.cols;
                 float d = keep[b][t * P];
 #pragma unroll
@@ -349,21 +353,27 @@ template <int XTY, bool SW, int T, int P, int SB, int SUB, bool MP> __device__ _
     }
 }
 
-#define LE_G4Q1(NAME, XTY, SW, T, P, SB, SUB) \
-    extern "C" __global__ void __launch_bounds__(512) le_g4q_##NAME##_s##SB##_b##SUB(G4Args a) { g4q_body<XTY, SW, T, P, SB, SUB, false>(a); } \
-    extern "C" __global__ void __launch_bounds__(SUB == 128 ? 1024 : 512) le_g4q_##NAME##_s##SB##_b##SUB##_mp(G4Args a) { g4q_body<XTY, SW, T, P, SB, SUB, true>(a); }
-#define LE_G4Q(NAME, XTY, SW, T, P) \
-    LE_G4Q1(NAME, XTY, SW, T, P, 2, 32) LE_G4Q1(NAME, XTY, SW, T, P, 2, 64) LE_G4Q1(NAME, XTY, SW, T, P, 2, 128) \
-    LE_G4Q1(NAME, XTY, SW, T, P, 4, 32) LE_G4Q1(NAME, XTY, SW, T, P, 4, 64) LE_G4Q1(NAME, XTY, SW, T, P, 4, 128)
-LE_G4Q(f32, 0, false, 1, 3)
-LE_G4Q(f16, 1, false, 1, 2)
-LE_G4Q(bf16, 30, false, 1, 1)
-LE_G4Q(f32w, 0, true, 1, 3)
-LE_G4Q(f16w, 1, true, 1, 2)
-LE_G4Q(bf16w, 30, true, 1, 2)
-#define LE_G4Q_FEW(NAME, XTY, SW, T, P) LE_G4Q1(NAME, XTY, SW, T, P, 2, 64) LE_G4Q1(NAME, XTY, SW, T, P, 2, 128) LE_G4Q1(NAME, XTY, SW, T, P, 4, 64) LE_G4Q1(NAME, XTY, SW, T, P, 4, 128)
-LE_G4Q_FEW(f16t2, 1, false, 2, 2)
-LE_G4Q_FEW(bf16t4, 30, false, 4, 1)
+#ifndef LE_G4_STY
+#define LE_G4_STY 1 /* a code object for each type of scales */
+#endif
+#define LE_G4_CAT2(a, b) a##b
+#define LE_G4_CAT(a, b) LE_G4_CAT2(a, b)
+#define LE_G4_S LE_G4_CAT(_s, LE_G4_STY)
+#define LE_G4_KERNEL(BLOCK, NAME, BODY) extern "C" __global__ void __launch_bounds__(BLOCK) LE_G4_CAT(NAME, LE_G4_S)(G4Args a) { BODY(a); }
+/* F(suffix, SUB, VEC, ...) for all scale blocks */
+#define LE_G4_SUBS(F, ...) F(b32, 32, false, __VA_ARGS__) F(b32v, 32, true, __VA_ARGS__) F(b64, 64, false, __VA_ARGS__) F(b64v, 64, true, __VA_ARGS__) \
+    F(b128, 128, false, __VA_ARGS__)
+#define LE_G4Q1(B, SUB, VEC, NAME, XTY, SW, T, P) \
+    LE_G4_KERNEL(512, le_g4q_##NAME##_##B, (g4q_body<XTY, SW, T, P, LE_G4_STY, SUB, VEC, false>)) \
+    LE_G4_KERNEL((SUB == 128 ? 1024 : 512), le_g4q_##NAME##_##B##_mp, (g4q_body<XTY, SW, T, P, LE_G4_STY, SUB, VEC, true>))
+LE_G4_SUBS(LE_G4Q1, f32, 0, false, 1, 3)
+LE_G4_SUBS(LE_G4Q1, f16, 1, false, 1, 2)
+LE_G4_SUBS(LE_G4Q1, bf16, 30, false, 1, 1)
+LE_G4_SUBS(LE_G4Q1, f32w, 0, true, 1, 3)
+LE_G4_SUBS(LE_G4Q1, f16w, 1, true, 1, 2)
+LE_G4_SUBS(LE_G4Q1, bf16w, 30, true, 1, 2)
+LE_G4_SUBS(LE_G4Q1, f16t2, 1, false, 2, 2)
+LE_G4_SUBS(LE_G4Q1, bf16t4, 30, false, 4, 1)
 
 /* ---- more tokens: activations laid out by a launch of their own ----
  *
@@ -451,11 +461,11 @@ static __device__ __forceinline__ f32x4 mfma16(const uint4 &a, const f16x8 &b, c
  * longer than they hold, whose partial results le_g4s adds. Against the layout of le_g4m_* it has fewer vector instructions (a lane
  * applies scale and zero point to one K part of one row, not to every one) and longer runs of a row's codes, for MFMAs that a few
  * tokens leave idle. */
-template <int NA, int P, int SB, int SUB> __device__ __forceinline__ void g4t_body(const G4Args &a) {
-    constexpr int BPC = 128 / SUB, T = 4 / P, NT = NA * T;
+template <int NA, int P, int STY, int SUB, bool VEC> __device__ __forceinline__ void g4t_body(const G4Args &a) {
+    constexpr int BPC = 128 / SUB, T = 4 / P, NT = NA * T, SB = STY == 0 ? 4 : 2;
     struct Item {
         uint4 q[4];
-        unsigned s[BPC], z[BPC];
+        Scales<STY, BPC, VEC> s, z;
     };
     extern __shared__ __align__(16) unsigned char lds[];
     float *red = (float *)lds; /* [group][wave][token][64] */
@@ -489,6 +499,7 @@ template <int NA, int P, int SB, int SUB> __device__ __forceinline__ void g4t_bo
     for (int t = 0; t < NT; t++) down[t] = downs[t];
     __builtin_amdgcn_sched_barrier(0); /* loads return in order: these first */
 
+    const float zbase = a.zeros ? 16.f : 24.f;
     const unsigned rowb = a.cols >> 1, bytes = a.rows * rowb, sbytes = a.rows * a.ng * SB; /* of the matrix: below 4 GiB */
     unsigned vo[4];
 #pragma unroll
@@ -500,18 +511,9 @@ template <int NA, int P, int SB, int SUB> __device__ __forceinline__ void g4t_bo
         const int gr = (int)blockIdx.x + gi * a.gx;
         const bool there = gi < G && sl < ns;
         const auto rq = rsrc(w0, there ? bytes : 0), rs = rsrc(s0, there ? sbytes : 0), rz = rsrc(z0, there && a.zeros ? sbytes : 0);
-        if (BPC > 1 && a.vec) {
-            const unsigned off = ((gr * 16 + myrow) * a.ng + min((sl * 4 + g) * BPC, a.ng - BPC)) * SB;
-            load_scales<BPC, SB>(it.s, rs, off);
-            load_scales<BPC, SB>(it.z, rz, off);
-        } else {
-#pragma unroll
-            for (int b = 0; b < BPC; b++) {
-                const unsigned off = ((gr * 16 + myrow) * a.ng + (min((sl * 4 + g) * 128 + b * SUB, a.cols - 1) >> a.gshift)) * SB;
-                it.s[b] = load_scale<SB>(rs, off);
-                it.z[b] = load_scale<SB>(rz, off);
-            }
-        }
+        const unsigned row = (gr * 16 + myrow) * a.ng;
+        it.s.load(rs, row, (sl * 4 + g) * BPC, SUB, a.cols, a.gshift, a.ng);
+        it.z.load(rz, row, (sl * 4 + g) * BPC, SUB, a.cols, a.gshift, a.ng);
         const unsigned go = gr * 16 * rowb;
 #pragma unroll
         for (int u = 0; u < 4; u++) it.q[u] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rq, vo[u] + go, 0, 2 /* nt */));
@@ -542,7 +544,7 @@ template <int NA, int P, int SB, int SUB> __device__ __forceinline__ void g4t_bo
         float tot[NT] = {};
 #pragma unroll
         for (int b = 0; b < BPC; b++) {
-            const float sc = scale_at<SB>(a, it.s, b, BPC > 1), zo = 16.f + (a.zeros ? scale_at<SB>(a, it.z, b, BPC > 1) : 8.f);
+            const float sc = it.s.at(b), zo = zbase + it.z.at(b);
             const bool in = (sl * 4 + g) * 128 + b * SUB < a.cols;
 #pragma unroll
             for (int t = 0; t < NT; t++) {
@@ -597,12 +599,12 @@ template <int NA, int P, int SB, int SUB> __device__ __forceinline__ void g4t_bo
  * partial results le_g4s_* adds: with passes instead (as le_g4q_*), every block of a long K reads all fragments for its few
  * rows, one pass's at a time (4096 x 14336, five tokens: 29 us). The scales of
  * an item are loaded once by the lane groups together and passed between them: loaded by each lane group they were a third of the
- * time (14336 x 4096 bf16, five tokens 18.4 us, 12.6 without those loads). */
-template <int P, int SB, int SUB, int CS> __device__ __forceinline__ void g4m_body(const G4Args &a) {
-    constexpr int BPC = 128 / SUB, NSUB = CS * BPC, NL = NSUB < 4 ? 1 : NSUB / 4; /* scale blocks of an item's row, of them a lane's to load */
+ * time (14336 x 4096 bf16, five tokens 18.4 us, 12.6 without those loads). 14336 x 4096 fp32, groups of 128: 16 tokens 17.0 us, 64 42. */
+template <int P, int STY, int SUB, bool VEC, int CS> __device__ __forceinline__ void g4m_body(const G4Args &a) {
+    constexpr int SB = STY == 0 ? 4 : 2, BPC = 128 / SUB, NSUB = CS * BPC, NL = NSUB < 4 ? 1 : NSUB / 4; /* scale blocks of an item's row, of them a lane's to load */
     struct Item {
         uint4 q[CS];
-        unsigned s[NL], z[NL];
+        Scales<STY, NL, VEC && (NL > 1)> s, z;
     };
     extern __shared__ __align__(16) unsigned char lds[];
     f32x4 *red = (f32x4 *)lds; /* [group][wave][64] */
@@ -637,6 +639,7 @@ template <int P, int SB, int SUB, int CS> __device__ __forceinline__ void g4m_bo
         down[c] = downs[cc * 4];
     }
     __builtin_amdgcn_sched_barrier(0); /* loads return in order: these first */
+    const float zbase = a.zeros ? 16.f : 24.f;
     const unsigned rowb = a.cols >> 1, bytes = a.rows * rowb, sbytes = a.rows * a.ng * SB; /* of the matrix: below 4 GiB */
     const unsigned char *w0 = a.codes + (size_t)mat * bytes, *s0 = (const unsigned char *)a.scales + (size_t)mat * sbytes,
                         *z0 = (const unsigned char *)a.zeros + (size_t)mat * sbytes;
@@ -646,18 +649,9 @@ template <int P, int SB, int SUB, int CS> __device__ __forceinline__ void g4m_bo
         const bool there = gi < G;
         const auto rq = rsrc(w0, there ? bytes : 0), rs = rsrc(s0, there ? sbytes : 0), rz = rsrc(z0, there && a.zeros ? sbytes : 0);
         const int b0 = c0 * BPC + (NSUB < 4 ? g % NSUB : g * NL);
-        if (NL > 1 && a.vec) {
-            const unsigned off = ((gr * 16 + n) * a.ng + min(b0, a.ng - NL)) * SB;
-            load_scales<NL, SB>(it.s, rs, off);
-            load_scales<NL, SB>(it.z, rz, off);
-        } else {
-#pragma unroll
-            for (int k = 0; k < NL; k++) {
-                const unsigned off = ((gr * 16 + n) * a.ng + (min((b0 + k) * SUB, a.cols - 1) >> a.gshift)) * SB;
-                it.s[k] = load_scale<SB>(rs, off);
-                it.z[k] = load_scale<SB>(rz, off);
-            }
-        }
+        const unsigned row = (gr * 16 + n) * a.ng;
+        it.s.load(rs, row, b0, SUB, a.cols, a.gshift, a.ng);
+        it.z.load(rz, row, b0, SUB, a.cols, a.gshift, a.ng);
         const unsigned go = gr * 16 * rowb + c0 * 64;
 #pragma unroll
         for (int c = 0; c < CS; c++)
@@ -669,8 +663,8 @@ template <int P, int SB, int SUB, int CS> __device__ __forceinline__ void g4m_bo
         float sc[NL], zo[NL]; /* this lane's blocks, scale and 16 + zero point */
 #pragma unroll
         for (int k = 0; k < NL; k++) {
-            sc[k] = scale_at<SB>(a, it.s, k, NL > 1);
-            zo[k] = 16.f + (a.zeros ? scale_at<SB>(a, it.z, k, NL > 1) : 8.f);
+            sc[k] = it.s.at(k);
+            zo[k] = zbase + it.z.at(k);
         }
         f32x4 tot = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -739,21 +733,17 @@ template <int P, int SB, int SUB, int CS> __device__ __forceinline__ void g4m_bo
     }
 }
 
-#define LE_G4X(NAME, XTY, SW, P)                                                                                                              \
-    extern "C" __global__ void __launch_bounds__(256) le_g4x_##NAME##_b32(G4Args a) { g4x_body<XTY, SW, P, 32>(a); }   \
-    extern "C" __global__ void __launch_bounds__(256) le_g4x_##NAME##_b64(G4Args a) { g4x_body<XTY, SW, P, 64>(a); }   \
+#define LE_G4T1(B, SUB, VEC, NA, P) LE_G4_KERNEL(512, le_g4t_n##NA##_p##P##_##B, (g4t_body<NA, P, LE_G4_STY, SUB, VEC>))
+LE_G4_SUBS(LE_G4T1, 1, 1) LE_G4_SUBS(LE_G4T1, 2, 1) LE_G4_SUBS(LE_G4T1, 1, 2) LE_G4_SUBS(LE_G4T1, 2, 2) LE_G4_SUBS(LE_G4T1, 3, 2)
+#define LE_G4M1(B, SUB, VEC, P) LE_G4_KERNEL(512, le_g4m_p##P##_##B, (g4m_body<P, LE_G4_STY, SUB, VEC, (P == 2 && SUB == 32 ? 2 : 4)>))
+LE_G4_SUBS(LE_G4M1, 1) LE_G4_SUBS(LE_G4M1, 2)
+
+#if LE_G4_STY == 1 /* once */
+#define LE_G4X(NAME, XTY, SW, P)                                                                                     \
+    extern "C" __global__ void __launch_bounds__(256) le_g4x_##NAME##_b32(G4Args a) { g4x_body<XTY, SW, P, 32>(a); } \
+    extern "C" __global__ void __launch_bounds__(256) le_g4x_##NAME##_b64(G4Args a) { g4x_body<XTY, SW, P, 64>(a); } \
     extern "C" __global__ void __launch_bounds__(256) le_g4x_##NAME##_b128(G4Args a) { g4x_body<XTY, SW, P, 128>(a); }
 LE_G4X(f32, 0, false, 2) LE_G4X(f16, 1, false, 1) LE_G4X(bf16, 30, false, 1) LE_G4X(f32w, 0, true, 2) LE_G4X(f16w, 1, true, 2) LE_G4X(bf16w, 30, true, 2)
-#define LE_G4T1(NA, P, SB, SUB) \
-    extern "C" __global__ void __launch_bounds__(512) le_g4t_n##NA##_p##P##_s##SB##_b##SUB(G4Args a) { g4t_body<NA, P, SB, SUB>(a); }
-#define LE_G4T(NA, P) \
-    LE_G4T1(NA, P, 2, 32) LE_G4T1(NA, P, 2, 64) LE_G4T1(NA, P, 2, 128) LE_G4T1(NA, P, 4, 32) LE_G4T1(NA, P, 4, 64) LE_G4T1(NA, P, 4, 128)
-LE_G4T(1, 1) LE_G4T(2, 1) LE_G4T(1, 2) LE_G4T(2, 2)
-LE_G4T1(3, 2, 2, 64) LE_G4T1(3, 2, 2, 128) LE_G4T1(3, 2, 4, 64) LE_G4T1(3, 2, 4, 128)
-#define LE_G4M1(P, SB, SUB, CS) \
-    extern "C" __global__ void __launch_bounds__(512) le_g4m_p##P##_s##SB##_b##SUB(G4Args a) { g4m_body<P, SB, SUB, CS>(a); }
-LE_G4M1(1, 2, 32, 4) LE_G4M1(1, 2, 64, 4) LE_G4M1(1, 2, 128, 4) LE_G4M1(1, 4, 32, 4) LE_G4M1(1, 4, 64, 4) LE_G4M1(1, 4, 128, 4)
-LE_G4M1(2, 2, 32, 2) LE_G4M1(2, 2, 64, 4) LE_G4M1(2, 2, 128, 4) LE_G4M1(2, 4, 32, 2) LE_G4M1(2, 4, 64, 4) LE_G4M1(2, 4, 128, 4)
 
 /* le_g4s: the segments' partial results added in their order and rounded, a value a thread. */
 extern "C" __global__ void __launch_bounds__(256) le_g4s(G4Args a) {
@@ -765,3 +755,4 @@ extern "C" __global__ void __launch_bounds__(256) le_g4s(G4Args a) {
     if (a.xty == 0) ((float *)a.y)[i] = v;
     else ((unsigned short *)a.y)[i] = a.xty == 1 ? XT<1>::down(v) : XT<30>::down(v);
 }
+#endif
