@@ -299,8 +299,9 @@ typedef struct le_g4 {
  * 0 .. n_mat - 1 gets zeros. `share` consecutive slots share their activations: a(s, t) is row (s / share) * m + t of x, rows
  * xstride values apart (0: one row for all). x and y are of type xtype; with swiglu 0, a is x's row of cols values, with
  * swiglu 1 a[c] = silu(row[c]) * row[cols + c] for a row of 2 * cols (gate | up), silu(g) = g / (1 + exp(-g)).
- * Products are exact (activations enter in bf16 pieces that add up to them; the SwiGLU's as fp32), sums are fp32, and the result
- * is rounded once to xtype. A row's activations, finite, may be of any magnitude whose sums fp32 holds; one that is not finite makes
+ * Activations are held to 2^-22 of their value (fp16 and bf16 without SwiGLU exactly, SwiGLU's of 16-bit types to 2^-16) or to 2^-39 of
+ * the largest of their 128 columns, whichever is more; products with codes are exact, sums are fp32, and the result is rounded
+ * once to xtype. A row's activations, finite, may be of any magnitude whose sums fp32 holds; one that is not finite makes
  * its token's outputs infinite or NaN. Limits: m <= 64, slots <= 65535, cols <= 2^24, slots * m * rows <= 2^31,
  * a matrix's codes and its scales each below 4 GiB; x 16-byte aligned, xstride a multiple of 16 bytes. y may not overlap an
  * input.
@@ -333,7 +334,7 @@ size_t le_moe_sort_workspace_size(int n_tok, int k, int n_exp);
 int le_moe_sort(le_ctx *ctx, const int *idx, int n_tok, int k, int n_exp, int *off, int *in_idx, int *out_idx, int *pos,
                 void *ws, size_t ws_bytes, le_stream_t stream);
 /* Rows between token order and expert order. All rows have cols values of type ty, token rows ldt values apart, expert rows
- * lde apart (each >= cols); pos[p] is the expert row of pair p, a pair with pos outside 0 .. n_row - 1 has none. pos NULL
+ * lde apart (each >= cols, and cols <= 2^25); pos[p] is the expert row of pair p, a pair with pos outside 0 .. n_row - 1 has none. pos NULL
  * stands for pos[p] = p (rows in pair order, as le_mm_grouped leaves them under out_idx).
  * le_moe_permute: e[pos[p]] = x[t]; rows of no pair keep what they held. Its gradient is le_moe_combine with w NULL.
  * le_moe_combine: out[t] = sum over the token's pairs that have a row of w[p] * e[pos[p]], added in selection order in fp32

@@ -77,12 +77,14 @@ static __device__ __forceinline__ f32x4 mfma(const uint4 &a, const bf16x8 &b, co
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), b, c, 0, 0, 0);
 }
 /* silu(g) * u = g u / (1 + 2^t), t = -g log2 e held as t + lo; the exponential and the reciprocal are the hardware's (1 ulp each). t stops
- * at 126, where the result is below 2^-118 |u| already. */
+ * at 126, where the result is below 2^-118 |u| already, and 0 is given beyond (not for NaN and infinities: 0 g is NaN). Below -126 there
+ * is no lo to add, and t0, which g of 2^127 and more make infinite, gives none. */
 static __device__ __forceinline__ float silu_mul(float g, float u) {
     const float l2e = 1.44269502f, t0 = -g * l2e, t = fminf(t0, 126.f);
-    const float lo = t0 <= 126.f ? __builtin_fmaf(-g, l2e, -t0) - g * 1.92596299e-8f : 0.f;
+    const float lo = fabsf(t0) <= 126.f ? __builtin_fmaf(-g, l2e, -t0) - g * 1.92596299e-8f : 0.f;
     const float e0 = __builtin_amdgcn_exp2f(t), e = __builtin_fmaf(e0 * 0.693147181f, lo, e0);
-    return g * __builtin_amdgcn_rcpf(1.f + e) * u;
+    const float q = t0 > 126.f ? 0.f : __builtin_amdgcn_rcpf(1.f + e);
+    return g * q * u;
 }
 static __device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc(const void *p, unsigned n) { return __builtin_amdgcn_make_buffer_rsrc((void *)p, 0, n, 0x00027000); }
 /* LDS writes of this wave's lanes are seen by its later reads (no other wave touches them). */

@@ -27,8 +27,8 @@ int check_experts(le_ctx *c, int n_exp, int k_most) {
 int check_rows(le_ctx *c, int ty, long long ldt, long long lde, int n_tok, int k, int cols, int n_row) {
     if (!type_bytes(ty)) return le_ctx_failf(c, LE_ERR_TYPE, "rows of type %d", ty);
     if (int rc = check_pairs(c, n_tok, k)) return rc;
-    if (cols <= 0 || n_row < 0 || ldt < cols || lde < cols)
-        return le_ctx_failf(c, LE_ERR_SHAPE, "cols=%d, n_row=%d, row strides %lld and %lld", cols, n_row, ldt, lde);
+    if (cols <= 0 || cols > 1 << 25 || n_row < 0 || ldt < cols || lde < cols)
+        return le_ctx_failf(c, LE_ERR_SHAPE, "cols=%d (1..2^25), n_row=%d, row strides %lld and %lld", cols, n_row, ldt, lde);
     return LE_OK;
 }
 
@@ -124,7 +124,6 @@ static int rows_launch(le_ctx *c, const char *what, int ty, const RowsArgs &rows
      * nothing is summed over a row */
     const int n = ty == LE_F32 ? 4 : 8, parts = (a.cols + n - 1) / n, L = parts <= 16 ? 16 : parts <= 64 ? 64 : 256;
     const bool whole = !strcmp(what, "combine_bwd");
-    if (!whole && (parts + L - 1) / L > 65535) return le_ctx_failf(c, LE_ERR_SHAPE, "cols=%d", a.cols);
     char name[40];
     /* expert rows that are read and lie at 16-byte addresses: non-temporal from 8 MB on (4096 tokens of 8 pairs by 2048 bf16: sum 30.3 -> 26.6
      * us, its gradient 62 -> 58, a sum behind that 90 -> 80; 64 tokens 3.6 -> 4.0, 301 by 1001 fp32, whose rows share lines, 5.3 -> 6.4) */

@@ -172,14 +172,15 @@ def _stream(stream):
 
 
 def _workspace(n, stream):
-    """n bytes of device memory for one call on `stream` (None: none needed), not reused before that call is done."""
+    """n bytes of device memory for one call on `stream` (None: none needed), from that stream's own memory: nothing that another
+    stream still uses, and given to no other stream's call before this one is done."""
     if not n:
         return None
     import torch
-    ws = torch.empty(n, dtype=torch.uint8, device="cuda")
-    if stream is not None:
-        ws.record_stream(torch.cuda.ExternalStream(stream) if isinstance(stream, int) else stream)
-    return ws
+    if stream is None:
+        return torch.empty(n, dtype=torch.uint8, device="cuda")
+    with torch.cuda.stream(torch.cuda.ExternalStream(stream) if isinstance(stream, int) else stream):
+        return torch.empty(n, dtype=torch.uint8, device="cuda")
 
 
 class _G4(ctypes.Structure):  # le_g4 of include/le_qmm.h

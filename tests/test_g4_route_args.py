@@ -220,7 +220,7 @@ def test_rows_refusals(lib, ctx):
 
     for f in (permute, combine, bwd):
         assert f(ty=8) == -2
-        for bad in (dict(n_tok=-1), dict(k=0), dict(k=17), dict(cols=0), dict(n_row=-1), dict(ldt=7), dict(lde=7), dict(n_tok=2**31 - 1)):
+        for bad in (dict(n_tok=-1), dict(k=0), dict(k=17), dict(cols=0), dict(cols=2**25 + 1, ldt=2**26, lde=2**26), dict(cols=2**31 - 1, ldt=2**31, lde=2**31), dict(n_row=-1), dict(ldt=7), dict(lde=7), dict(n_tok=2**31 - 1)):
             assert f(**bad) == -3, bad
         assert f(x=None) == -1 and f(e=None) == -1
         assert f(x=A + 2) == -4 and f(e=A + 2) == -4 and f(ty=1, x=A + 1) == -4 and f(pos=A + 2) == -4
@@ -229,7 +229,7 @@ def test_rows_refusals(lib, ctx):
     assert permute(n_row=0) == 0 and bwd(de=None, dw=None) == 0
     assert ctx.launches == 0
     for f in (permute, combine, bwd):
-        assert f() == 0 and f(pos=None) == 0 and f(ty=30, x=A + 2, e=A + 2) == 0 and f(n_tok=2**27, k=1) == 0
+        assert f() == 0 and f(pos=None) == 0 and f(cols=2**25, ldt=2**25, lde=2**25) == 0 and f(ty=30, x=A + 2, e=A + 2) == 0 and f(n_tok=2**27, k=1) == 0
     assert bwd(dw=None, e=None) == 0 and bwd(de=None) == 0 and combine(w=None) == 0 and combine(e=None, n_row=0) == 0
     for name, g, block, lds in ctx.calls():
         assert g[0] * block < 2**32 and g[1] <= 65535 and min(g) > 0 and lds <= 160 * 1024, (name, g, block)

@@ -208,6 +208,36 @@ def test_not_finite(engine, ty, bad, m):
     assert torch.equal(out[keep], ref[keep])
 
 
+@pytest.mark.parametrize("ty", [le.F32, le.BF16])
+@pytest.mark.parametrize("m", [1, 3, 20])
+def test_far_gates(engine, ty, m):
+    """Gates whose exponential, or whose product with log2 e, no fp32 holds, next to ordinary ones: SwiGLU is gate * up, or 0.
+
+    The ups are at 2^-118 so that the products stay in range; the ordinary gates' products are below the tolerance then, and
+    normal (|g| > 2^-8 nearly always, and what is flushed otherwise is 2^-126 of 1024 columns, below the bound's U * terms)."""
+    import torch
+    gen = torch.Generator().manual_seed(540)
+    gates = torch.tensor([3e38, -3e38, 1e37, -1e37, -1000.0, 2.5e38, -88.5, -2e30])
+    g = gates[torch.randint(0, 8, (m, 1024), generator=gen)]
+    g[:, ::3] = torch.randn(m, 342, generator=gen)
+    x = torch.cat([g, torch.randn(m, 1024, generator=gen) * 2.0 ** -118], 1).to(torch_type(ty))
+    run(engine, ty, le.F16, 1, 40, 1024, 64, m, 1, 1, None, True, True, 541, x=x, rms=False)
+
+
+@pytest.mark.parametrize("ty", TYPES)
+def test_gates_that_are_not_finite(engine, ty):
+    import torch
+    codes, scales, z = make(1, 32, 512, 64, le.F16, True, 545)
+    w = le.G4(codes.cuda(), scales.cuda(), z.cuda(), 32, 512, 64)
+    for m in (1, 3):
+        for bad in (float("inf"), float("-inf"), float("nan")):
+            x = torch.randn(m, 1024).to(torch_type(ty))
+            x[0, 100] = bad
+            out = torch.zeros(m, 32, dtype=torch_type(ty), device="cuda")
+            engine.mv_g4(ty, w, x.cuda(), out, m=m, swiglu=True)
+            assert not torch.isfinite(out[0]).any() and torch.isfinite(out[1:]).all()
+
+
 def test_same_bits_again(engine):
     """Sums in a fixed order: the same bits from call to call, and in a batch of another size class or not."""
     import torch
@@ -288,6 +318,19 @@ def test_streams_and_workspaces(engine, ty, m, cols):
     with pytest.raises(le.LeError) as e:
         engine.mv_g4(ty, w, dx[0], outs[0], m=m, ws=torch.empty(need - 1, dtype=torch.uint8, device="cuda"))
     assert e.value.code == -7
+
+
+def test_workspace_of_another_stream(engine):
+    """A call on another stream takes no memory that the current stream's work may still use."""
+    import torch
+    from lastengine_amd import qmm
+    s = torch.cuda.Stream()
+    for stream in (s, s.cuda_stream):
+        used = torch.empty(37 << 20, dtype=torch.uint8, device="cuda")
+        at = used.data_ptr()
+        del used  # free for the current stream at once, for others when its work is done
+        assert qmm._workspace(37 << 20, stream).data_ptr() != at
+    assert qmm._workspace(37 << 20, None).data_ptr() == at and qmm._workspace(0, s) is None
 
 
 @pytest.mark.parametrize("ty,m", [(le.F32, 1), (le.F32, 6), (le.BF16, 33)])
