@@ -21,7 +21,8 @@
  *   - No entry allocates device memory; entries that need scratch take a caller-sized workspace.
  *   - Activations are fp32; results are fp32 with fp32 accumulation. Inside the kernels each
  *     32-value activation block is held as a 15-bit integer split into two int8 planes with an
- *     fp32 scale (error <= 3.1e-5 of the block maximum per value); weight codes are exact.
+ *     fp32 scale (error <= 3.1e-5 of the block maximum per value); weight codes are exact. (le_matvec_g4 and the
+ *     entries behind it take the types of enum le_dtype and say what they hold.)
  *
  * Supported types (GGML ids, src/quant.rs:13-20): Q8_0=8, Q4_K=12, Q6_K=14, IQ2_XXS=16, IQ3_XXS=18,
  * and Q4_0=2, Q3_K=11, Q5_K=13, IQ2_S=22 (src/quant.rs:64-67,83-95,113-126,155-167; the reference's
