@@ -329,14 +329,16 @@ int le_moe_route_bwd(le_ctx *ctx, int ltype, const int *idx, const float *w, con
 /* le_moe_sort: the pairs grouped by expert, in pair order within an expert, as le_mm_grouped takes them: off (n_exp + 1),
  * in_idx[i] = the token and out_idx[i] = the pair of place i < off[n_exp], and pos[p] = the place of pair p. A pair whose
  * idx lies outside 0 .. n_exp - 1 is dropped: pos[p] = -1, and no place is its own (in_idx and out_idx keep what they held
- * from off[n_exp] on). Any of in_idx, out_idx and pos may be NULL. ws: le_moe_sort_workspace_size bytes, 16-byte aligned (NULL where
+ * from off[n_exp] on; le_mm_grouped, with n_tok * k as npair, goes by none of those). Any of in_idx, out_idx and pos may be NULL. ws: le_moe_sort_workspace_size bytes, 16-byte aligned (NULL where
  * that is 0); calls that may overlap need workspaces of their own. */
 size_t le_moe_sort_workspace_size(int n_tok, int k, int n_exp);
 int le_moe_sort(le_ctx *ctx, const int *idx, int n_tok, int k, int n_exp, int *off, int *in_idx, int *out_idx, int *pos,
                 void *ws, size_t ws_bytes, le_stream_t stream);
 /* Rows between token order and expert order. All rows have cols values of type ty, token rows ldt values apart, expert rows
  * lde apart (each >= cols, and cols <= 2^25); pos[p] is the expert row of pair p, a pair with pos outside 0 .. n_row - 1 has none. pos NULL
- * stands for pos[p] = p (rows in pair order, as le_mm_grouped leaves them under out_idx).
+ * stands for pos[p] = p (rows in pair order, as le_mm_grouped leaves them under out_idx): then every pair has a row, also one that
+ * le_moe_sort dropped and no product wrote, which has to hold finite values for its weight 0 to drop it. With rows in place order
+ * (le_mm_grouped with places 0, 1, .. as out_idx) and pos such a pair has none.
  * le_moe_permute: e[pos[p]] = x[t]; rows of no pair keep what they held. Its gradient is le_moe_combine with w NULL.
  * le_moe_combine: out[t] = sum over the token's pairs that have a row of w[p] * e[pos[p]], added in selection order in fp32
  * and rounded once; w NULL stands for 1. A token without such pairs gets zeros.

@@ -55,6 +55,39 @@ def test_steps_make_the_layer(engine, n_tok):
     assert torch.equal(out2, out)
 
 
+@pytest.mark.parametrize("n_tok,pads", [(1, 1), (20, 3), (300, 40), (64, 64)])
+def test_steps_with_padding(engine, n_tok, pads):
+    """Padding tokens have no pairs: rows in place order and pos give them zeros whatever the rows' buffer held, and the others
+    what the layer gives for them alone (twice the layer's parity bar)."""
+    import torch
+    tg, td, n_exp, k, hidden, ff = le.Q4_K, le.Q6_K, 16, 4, 256, 256
+    g, u, d = (dev(weights(ty, n_exp * r, c, 80 + i)[0]) for i, (ty, r, c) in enumerate(((tg, ff, hidden), (tg, ff, hidden), (td, hidden, ff))))
+    h = dev(acts(n_tok * hidden, 90).reshape(n_tok, hidden))
+    logits = dev(acts(n_tok * n_exp, 91).reshape(n_tok, n_exp))
+    live = n_tok - pads
+    logits[live:] = -torch.inf
+    n = n_tok * k
+    idx, w = torch.empty(n_tok, k, dtype=torch.int32, device="cuda"), torch.empty(n_tok, k, device="cuda")
+    off = torch.empty(n_exp + 1, dtype=torch.int32, device="cuda")
+    i, o, pos = (torch.zeros(n, dtype=torch.int32, device="cuda") for _ in range(3))
+    engine.moe_route(le.F32, logits, n_tok, n_exp, k, idx, w)
+    engine.moe_sort(idx, n_tok, k, n_exp, off, i, o, pos)
+    assert int(off[-1]) == live * k
+    gate, up, down = (torch.full((n, c), float("nan"), device="cuda") for c in (ff, ff, hidden))
+    place = torch.arange(n, dtype=torch.int32, device="cuda")
+    engine.mm_grouped(tg, off, i, place, n_exp, n, h, gate, ff, hidden, w=g)
+    engine.mm_grouped(tg, off, i, place, n_exp, n, h, up, ff, hidden, w=u)
+    engine.mm_grouped(td, off, place, place, n_exp, n, gate * torch.sigmoid(gate) * up, down, hidden, ff, w=d)
+    assert torch.isnan(down[live * k:]).all()
+    out = torch.full((n_tok, hidden), float("nan"), device="cuda")
+    engine.moe_combine(le.F32, down, pos, w, n_tok, k, hidden, out, n)
+    assert (out[live:] == 0).all()
+    if live:
+        want = torch.empty(live, hidden, device="cuda")
+        engine.moe(tg, tg, td, g, u, d, n_exp, k, hidden, ff, logits[:live], h[:live], live, want)
+        assert float((out[:live] - want).abs().max()) <= 2e-3 * float(want.abs().max())
+
+
 def g4_stack(n_mat, rows, cols, group, seed):
     codes, scales, z = make(n_mat, rows, cols, group, le.F16, True, seed)
     return le.G4(codes.cuda(), scales.cuda(), z.cuda(), rows, cols, group, n_mat=n_mat), dequant(codes, scales, z, group)[0]
