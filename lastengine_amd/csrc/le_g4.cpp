@@ -116,16 +116,20 @@ extern "C" int le_matvec_g4(le_ctx *c, const le_g4 *w, const int *sel, int slots
     const int most = most_tokens(xtype, swiglu), sty = w->scale_type, P = pieces(xtype, swiglu);
     char name[48];
     void *args[] = {&a};
-    /* Row groups a block: so many that blocks of nw waves fill the chip with `waves` a CU, and LDS holds their partial results (lds bytes
-     * a wave and group). */
-    auto share_out = [&](int nw, int waves, long long others, int lds) {
-        const long long target = (long long)le_ctx_cus(c) * std::max(1, waves / nw);
-        long long per = (groups * others + target - 1) / target;
-        per = std::max(1LL, std::min<long long>({per, groups, 64 * 1024 / ((long long)nw * lds)}));
-        const long long gx = (groups + per - 1) / per;
+    /* Row groups a block: so many that blocks of nw waves, for each of the `others` (slots, token tiles, segments), fill the chip with
+     * `waves` a CU once or, where a block's LDS (lds bytes a wave and row group, `fixed` beside them) cannot hold its groups'
+     * partial results then, R times; then the fewest blocks that need no more groups (14336 x 4096 fp32, four tokens: 224 blocks 12.8 us,
+     * 256 with 3 or 4 groups 13.5). Rounds that end short are what this avoids: the same matrix with 64 tokens, in blocks of 8 groups
+     * for 64 KB 41.8 us, now 34.7; 40 tokens in groups of 32 47.7, now 44.4; 32000 x 4096, 5 tokens 31.4, now 25.8 (bf16, whose kernel fits a CU
+     * twice, 21.1, now 22.2). */
+    auto share_out = [&](int nw, int waves, long long others, int lds, int fixed) {
+        const int blocks = std::max(1, waves / nw); /* a CU */
+        const long long target = (long long)le_ctx_cus(c) * blocks, cap = std::max(1, (144 * 1024 / blocks - fixed) / (nw * lds));
+        const long long least = (groups + cap - 1) / cap, R = (least * others + target - 1) / target;
+        const long long most_gx = std::min(groups, target * R / others), per = (groups + most_gx - 1) / most_gx, gx = (groups + per - 1) / per;
         a.nw = nw;
         a.gx = (int)gx;
-        a.per = (int)((groups + gx - 1) / gx);
+        a.per = (int)per;
         a.full = (int)(groups - (a.per - 1) * gx);
     };
     if (m <= most) {
@@ -134,7 +138,7 @@ extern "C" int le_matvec_g4(le_ctx *c, const le_g4 *w, const int *sel, int slots
         const int quad = m == 1 && P > 1 ? nw * 4096 : 0;
         /* 32 experts of 1536 x 2048 (four waves a block), 16 / 24 waves a CU: groups of 32 15.0 / 14.4 us, 128 12.1 / 11.7; 28672 x
          * 4096 (eight) 13.1 / 14.6 */
-        share_out(nw, nw <= 4 ? 24 : 16, slots, T * 256);
+        share_out(nw, nw <= 4 ? 24 : 16, slots, T * 256, quad);
         snprintf(name, sizeof name, "le_g4q_%s%s_%s%s_s%d", kind, swiglu ? "w" : m == 1 ? "" : T == 2 ? "t2" : "t4", tail, passes > 1 || nw > 8 ? "_mp" : "", sty);
         return le_ctx_launch(c, name, dim3((unsigned)a.gx, (unsigned)slots), 64 * nw, (size_t)quad + (size_t)a.per * nw * T * 256, (hipStream_t)stream, args);
     }
@@ -151,7 +155,7 @@ extern "C" int le_matvec_g4(le_ctx *c, const le_g4 *w, const int *sel, int slots
     if (rc) return rc;
     /* waves: all of K's slices over the segments, evenly */
     const int nw = ((nc + cs - 1) / cs + a.segs - 1) / a.segs, p16 = pieces16(xtype, swiglu), lds = a.na ? a.na * 4 / p16 * 256 : 1024;
-    share_out(nw, 8, (long long)slots * tiles * a.segs, lds);
+    share_out(nw, 8, (long long)slots * tiles * a.segs, lds, 0);
     if (a.na) snprintf(name, sizeof name, "le_g4t_n%d_p%d_%s_s%d", a.na, p16, tail, sty);
     else snprintf(name, sizeof name, "le_g4m_p%d_%s_s%d", p16, tail, sty);
     rc = le_ctx_launch(c, name, dim3((unsigned)a.gx, (unsigned)slots, (unsigned)(tiles * a.segs)), 64 * nw, (size_t)a.per * nw * lds, (hipStream_t)stream, args);

@@ -601,7 +601,7 @@ template <int NA, int P, int STY, int SUB, bool VEC> __device__ __forceinline__ 
  * partial results le_g4s_* adds: with passes instead (as le_g4q_*), every block of a long K reads all fragments for its few
  * rows, one pass's at a time (4096 x 14336, five tokens: 29 us). The scales of
  * an item are loaded once by the lane groups together and passed between them: loaded by each lane group they were a third of the
- * time (14336 x 4096 bf16, five tokens 18.4 us, 12.6 without those loads). 14336 x 4096 fp32, groups of 128: 16 tokens 17.0 us, 64 42. */
+ * time (14336 x 4096 bf16, five tokens 18.4 us, 12.6 without those loads). 14336 x 4096 fp32, groups of 128: 16 tokens 17.0 us, 32 22.8, 64 34.7. */
 template <int P, int STY, int SUB, bool VEC, int CS> __device__ __forceinline__ void g4m_body(const G4Args &a) {
     constexpr int SB = STY == 0 ? 4 : 2, BPC = 128 / SUB, NSUB = CS * BPC, NL = NSUB < 4 ? 1 : NSUB / 4; /* scale blocks of an item's row, of them a lane's to load */
     struct Item {
