@@ -38,10 +38,13 @@ size_t frag_bytes(int xtype, int swiglu, int m, int cols) {
 size_t tile_floats(int m, int cols) { return (size_t)((m + 15) / 16) * ((cols + 127) / 128) * 16; }
 size_t set_bytes(int xtype, int swiglu, int m, int cols) { return frag_bytes(xtype, swiglu, m, cols) + tile_floats(m, cols) * 4; }
 /* 128-column chunks that a wave keeps (le_g4m_*: two pieces' fragments of four and the sums over small scale blocks would not fit the
- * registers), and the segments of K that blocks of eight waves make of them. */
+ * registers), and the segments of K that blocks make of them: of 16 waves where the kernels' registers allow it (le_g4t_* with one set,
+ * or two at scale blocks of 64 and more), else of eight. With 16 against 8, two tokens fp32 in groups of 64: 5120 x 5120 (one
+ * segment against two) 9.4 / 12.2 us, 4096 x 14336 (two against four) 14.7 / 15.3, 28672 x 8192 32.2 / 32.2. */
 int chunks(const le_g4 *w, int xtype, int swiglu, int m) { return !row_sets(xtype, swiglu, m) && pieces16(xtype, swiglu) == 2 && scale_block(w) == 32 ? 2 : 4; }
 int segments(const le_g4 *w, int xtype, int swiglu, int m) {
-    const int most = 8 * chunks(w, xtype, swiglu, m);
+    const int na = row_sets(xtype, swiglu, m);
+    const int most = (na == 1 || (na == 2 && scale_block(w) >= 64) ? 16 : 8) * chunks(w, xtype, swiglu, m);
     return ((w->cols + 127) / 128 + most - 1) / most;
 }
 /* What is wrong with a shape, or null. */
@@ -133,7 +136,10 @@ extern "C" int le_matvec_g4(le_ctx *c, const le_g4 *w, const int *sel, int slots
         a.full = (int)(groups - (a.per - 1) * gx);
     };
     if (m <= most) {
-        const int ns = (w->cols + 511) / 512, wmax = ns <= 8 || sub < 128 ? 8 : 16; /* slices of 512 columns */
+        /* slices of 512 columns; 16 waves a block for more than eight of them (but for several tokens at scale blocks of 32, which take
+         * more than the 128 registers that leaves): 4096 x 14336 in groups of 64, 16 / 8 waves, fp32 11.3 / 12.3 us, SwiGLU 13.0 /
+         * 13.7, bf16, 4 tokens 14.6 / 15.1; 2048 x 6144 SwiGLU 6.75 / 7.8 */
+        const int ns = (w->cols + 511) / 512, wmax = ns <= 8 || (sub < 64 && m > 1) ? 8 : 16;
         const int passes = (ns + wmax - 1) / wmax, nw = (ns + passes - 1) / passes, T = m == 1 ? 1 : most;
         const int quad = m == 1 && P > 1 ? nw * 4096 : 0;
         /* 32 experts of 1536 x 2048 (four waves a block), 16 / 24 waves a CU: groups of 32 15.0 / 14.4 us, 128 12.1 / 11.7; 28672 x
@@ -156,7 +162,7 @@ extern "C" int le_matvec_g4(le_ctx *c, const le_g4 *w, const int *sel, int slots
     /* waves: all of K's slices over the segments, evenly */
     const int nw = ((nc + cs - 1) / cs + a.segs - 1) / a.segs, p16 = pieces16(xtype, swiglu), lds = a.na ? a.na * 4 / p16 * 256 : 1024;
     share_out(nw, 8, (long long)slots * tiles * a.segs, lds, 0);
-    if (a.na) snprintf(name, sizeof name, "le_g4t_n%d_p%d_%s_s%d", a.na, p16, tail, sty);
+    if (a.na) snprintf(name, sizeof name, "le_g4t_n%d_p%d_%s%s_s%d", a.na, p16, tail, nw > 8 && a.na == 2 && p16 == 1 && sub == 64 ? "_w" : "", sty);
     else snprintf(name, sizeof name, "le_g4m_p%d_%s_s%d", p16, tail, sty);
     rc = le_ctx_launch(c, name, dim3((unsigned)a.gx, (unsigned)slots, (unsigned)(tiles * a.segs)), 64 * nw, (size_t)a.per * nw * lds, (hipStream_t)stream, args);
     if (rc || a.segs == 1) return rc;

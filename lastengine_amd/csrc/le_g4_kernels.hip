@@ -34,7 +34,7 @@
  *
  * One token, weights from HBM (a streaming read of as many bytes at this size): 28672 x 4096 bf16, groups of 128, 62 MB 13.1 us (11.8),
  * 14336 x 4096 fp32 31 MB 8.2 (6.9), groups of 32 37 MB 9.4, 4096 x 4096 4.7 (3.5), 1024 x 2048 3.15 (2.7), 4096 x 14336 SwiGLU
- * fp32, groups of 64, 33 MB 13.6 (7.3): there each of 256 blocks reads all of x, forms SwiGLU and goes over K twice for its
+ * fp32, groups of 64, 33 MB 13.0 (7.3): there each of 256 blocks reads all of x, forms SwiGLU and goes over K twice for its
  * 16 rows. What the types and groups choose is compiled in: as branches on arguments it cost 14336 x 4096 in groups of 32 5.6 us. */
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -367,7 +367,7 @@ template <int XTY, bool SW, int T, int P, int STY, int SUB, bool VEC, bool MP> _
     F(b128, 128, false, __VA_ARGS__)
 #define LE_G4Q1(B, SUB, VEC, NAME, XTY, SW, T, P) \
     LE_G4_KERNEL(512, le_g4q_##NAME##_##B, (g4q_body<XTY, SW, T, P, LE_G4_STY, SUB, VEC, false>)) \
-    LE_G4_KERNEL((SUB == 128 ? 1024 : 512), le_g4q_##NAME##_##B##_mp, (g4q_body<XTY, SW, T, P, LE_G4_STY, SUB, VEC, true>))
+    LE_G4_KERNEL((T == 1 || SUB >= 64 ? 1024 : 512), le_g4q_##NAME##_##B##_mp, (g4q_body<XTY, SW, T, P, LE_G4_STY, SUB, VEC, true>))
 LE_G4_SUBS(LE_G4Q1, f32, 0, false, 1, 3)
 LE_G4_SUBS(LE_G4Q1, f16, 1, false, 1, 2)
 LE_G4_SUBS(LE_G4Q1, bf16, 30, false, 1, 1)
@@ -735,7 +735,12 @@ template <int P, int STY, int SUB, bool VEC, int CS> __device__ __forceinline__ 
     }
 }
 
-#define LE_G4T1(B, SUB, VEC, NA, P) LE_G4_KERNEL(512, le_g4t_n##NA##_p##P##_##B, (g4t_body<NA, P, LE_G4_STY, SUB, VEC>))
+/* 16 waves, which leave each 128 registers: one set, and two at scale blocks of 64 and more; two sets of one piece at 64 (143 registers)
+ * as a kernel of its own for long rows, which spills a few (14336 x 4096 bf16, 8 tokens 14.8 us, with spills 16.2; 5120 x 5120, 6
+ * tokens, in two segments of eight waves 15.0, in one of ten 11.4) */
+#define LE_G4T1(B, SUB, VEC, NA, P) \
+    LE_G4_KERNEL((NA == 1 || (NA == 2 && (SUB == 128 || (SUB == 64 && P == 2))) ? 1024 : 512), le_g4t_n##NA##_p##P##_##B, (g4t_body<NA, P, LE_G4_STY, SUB, VEC>))
+LE_G4_KERNEL(1024, le_g4t_n2_p1_b64_w, (g4t_body<2, 1, LE_G4_STY, 64, false>)) LE_G4_KERNEL(1024, le_g4t_n2_p1_b64v_w, (g4t_body<2, 1, LE_G4_STY, 64, true>))
 LE_G4_SUBS(LE_G4T1, 1, 1) LE_G4_SUBS(LE_G4T1, 2, 1) LE_G4_SUBS(LE_G4T1, 1, 2) LE_G4_SUBS(LE_G4T1, 2, 2) LE_G4_SUBS(LE_G4T1, 3, 2)
 #define LE_G4M1(B, SUB, VEC, P) LE_G4_KERNEL(512, le_g4m_p##P##_##B, (g4m_body<P, LE_G4_STY, SUB, VEC, (P == 2 && SUB == 32 ? 2 : 4)>))
 LE_G4_SUBS(LE_G4M1, 1) LE_G4_SUBS(LE_G4M1, 2)
