@@ -38,14 +38,17 @@ size_t frag_bytes(int xtype, int swiglu, int m, int cols) {
 size_t tile_floats(int m, int cols) { return (size_t)((m + 15) / 16) * ((cols + 127) / 128) * 16; }
 size_t set_bytes(int xtype, int swiglu, int m, int cols) { return frag_bytes(xtype, swiglu, m, cols) + tile_floats(m, cols) * 4; }
 /* 128-column chunks that a wave keeps (le_g4m_*: two pieces' fragments of four and the sums over small scale blocks would not fit the
- * registers), and the segments of K that blocks make of them: of 16 waves where the kernels' registers allow it (le_g4t_* with one set,
- * or two at scale blocks of 64 and more), else of eight. With 16 against 8, two tokens fp32 in groups of 64: 5120 x 5120 (one
- * segment against two) 9.4 / 12.2 us, 4096 x 14336 (two against four) 14.7 / 15.3, 28672 x 8192 32.2 / 32.2. */
+ * registers), and the segments of K that blocks make of them, of as many waves as the kernels' registers allow: le_g4t_* 16 with one set, or
+ * with two at scale blocks of 64 and more (16 / 8 waves, two tokens fp32 in groups of 64: 5120 x 5120, one segment against two, 9.4 /
+ * 12.2 us, 4096 x 14336, two against four, 14.7 / 15.3, 28672 x 8192 32.2 / 32.2); 12 with two sets of two pieces at 32 or three at 64 and
+ * more, where that makes one segment (12 / 8, five tokens: 5120 x 5120 12.3 / 15.1 us; but 4096 x 14336, three against four, 21.4 / 18.8);
+ * else, and le_g4m_*, eight. */
 int chunks(const le_g4 *w, int xtype, int swiglu, int m) { return !row_sets(xtype, swiglu, m) && pieces16(xtype, swiglu) == 2 && scale_block(w) == 32 ? 2 : 4; }
 int segments(const le_g4 *w, int xtype, int swiglu, int m) {
-    const int na = row_sets(xtype, swiglu, m);
-    const int most = (na == 1 || (na == 2 && scale_block(w) >= 64) ? 16 : 8) * chunks(w, xtype, swiglu, m);
-    return ((w->cols + 127) / 128 + most - 1) / most;
+    const int na = row_sets(xtype, swiglu, m), sub = scale_block(w), nc = (w->cols + 127) / 128;
+    const bool w16 = na == 1 || (na == 2 && sub >= 64), w12 = (na == 3 && sub >= 64) || (na == 2 && pieces16(xtype, swiglu) == 2);
+    const int most = (w16 ? 16 : w12 && nc <= 12 * 4 ? 12 : 8) * chunks(w, xtype, swiglu, m);
+    return (nc + most - 1) / most;
 }
 /* What is wrong with a shape, or null. */
 const char *shape_error(const le_g4 *w, int slots, int share, int m) {

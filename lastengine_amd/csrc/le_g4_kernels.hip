@@ -735,11 +735,12 @@ template <int P, int STY, int SUB, bool VEC, int CS> __device__ __forceinline__ 
     }
 }
 
-/* 16 waves, which leave each 128 registers: one set, and two at scale blocks of 64 and more; two sets of one piece at 64 (143 registers)
+/* 16 waves, which leave each 128 registers: one set, and two at scale blocks of 64 and more; 12 waves (168): two sets of two pieces at 32, three
+ * at 64 and more; two sets of one piece at 64 (143 registers)
  * as a kernel of its own for long rows, which spills a few (14336 x 4096 bf16, 8 tokens 14.8 us, with spills 16.2; 5120 x 5120, 6
  * tokens, in two segments of eight waves 15.0, in one of ten 11.4) */
 #define LE_G4T1(B, SUB, VEC, NA, P) \
-    LE_G4_KERNEL((NA == 1 || (NA == 2 && (SUB == 128 || (SUB == 64 && P == 2))) ? 1024 : 512), le_g4t_n##NA##_p##P##_##B, (g4t_body<NA, P, LE_G4_STY, SUB, VEC>))
+    LE_G4_KERNEL((NA == 1 || (NA == 2 && (SUB == 128 || (SUB == 64 && P == 2))) ? 1024 : (NA == 3 && SUB >= 64) || (NA == 2 && P == 2) ? 768 : 512), le_g4t_n##NA##_p##P##_##B, (g4t_body<NA, P, LE_G4_STY, SUB, VEC>))
 LE_G4_KERNEL(1024, le_g4t_n2_p1_b64_w, (g4t_body<2, 1, LE_G4_STY, 64, false>)) LE_G4_KERNEL(1024, le_g4t_n2_p1_b64v_w, (g4t_body<2, 1, LE_G4_STY, 64, true>))
 LE_G4_SUBS(LE_G4T1, 1, 1) LE_G4_SUBS(LE_G4T1, 2, 1) LE_G4_SUBS(LE_G4T1, 1, 2) LE_G4_SUBS(LE_G4T1, 2, 2) LE_G4_SUBS(LE_G4T1, 3, 2)
 #define LE_G4M1(B, SUB, VEC, P) LE_G4_KERNEL(512, le_g4m_p##P##_##B, (g4m_body<P, LE_G4_STY, SUB, VEC, (P == 2 && SUB == 32 ? 2 : 4)>))

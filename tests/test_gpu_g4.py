@@ -111,6 +111,14 @@ def test_tokens(engine, ty, m, cols, group):
 
 
 @pytest.mark.parametrize("ty", TYPES)
+@pytest.mark.parametrize("m", [1, 2, 3, 4, 5, 6, 8, 9, 17])
+@pytest.mark.parametrize("cols,group", [(4608, 32), (5120, 64), (6272, 128), (8224, 32), (12352, 64), (16512, 128)])
+def test_long_rows(engine, ty, m, cols, group):
+    """Rows that one block's waves hold, in one go or several, and rows that several blocks share."""
+    run(engine, ty, le.BF16, 1, 37, cols, group, m, 1, 1, None, m % 2 == 0, m == 3, 150 + m)
+
+
+@pytest.mark.parametrize("ty", TYPES)
 @pytest.mark.parametrize("stype", TYPES)
 @pytest.mark.parametrize("zeros,swiglu", [(False, False), (True, False), (True, True)])
 @pytest.mark.parametrize("m", [1, 6])
