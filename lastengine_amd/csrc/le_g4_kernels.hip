@@ -37,6 +37,7 @@
  * fp32, groups of 64, 33 MB 13.0 (7.3): there each of 256 blocks reads all of x, forms SwiGLU and goes over K twice for its
  * 16 rows. What the types and groups choose is compiled in: as branches on arguments it cost 14336 x 4096 in groups of 32 5.6 us. */
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 static __device__ __forceinline__ unsigned bits(float v) { return __builtin_bit_cast(unsigned, v); }
@@ -47,6 +48,11 @@ static __device__ __forceinline__ unsigned pack_hi16(float lo, float hi) { retur
 /* Eight values, cut to bf16, in a word's order of columns. */
 static __device__ __forceinline__ uint4 pack_octet(const float (&f)[8]) {
     return make_uint4(pack_hi16(f[0], f[4]), pack_hi16(f[1], f[5]), pack_hi16(f[2], f[6]), pack_hi16(f[3], f[7]));
+}
+/* The same, rounded to nearest. */
+static __device__ __forceinline__ uint4 pack_octet_near(const float (&f)[8]) {
+    auto two = [&](int k) { return __builtin_bit_cast(unsigned, (bf16x2){(__bf16)f[k], (__bf16)f[k + 4]}); };
+    return make_uint4(two(0), two(1), two(2), two(3));
 }
 /* First column, of a part of 128, of the octet that MFMA j takes from lane group g. */
 template <int SUB> static __device__ __forceinline__ int octet_col(int j, int g) {
@@ -210,12 +216,15 @@ template <int XTY, bool SW, int T, int P, int STY, int SUB, bool VEC, bool MP> _
 #pragma unroll
             for (int k = 0; k < 8; k++) f[k] = in ? f[k] : 0.f;
             uint4 *xl = (uint4 *)(lds + wave * 4096) + (kappa * 4 + g) * 4;
+            /* cut, so that no piece exceeds the value; the last, of what is left, to nearest: exact but for SwiGLU's 24 bits in two
+             * pieces, whose rest is below 2^-7 of the value's power of two and is held to 2^-16 of it */
 #pragma unroll 1
-            for (int p = 0; p < P; p++) {
+            for (int p = 0; p < P - 1; p++) {
                 xl[vi * 64 + p] = pack_octet(f);
 #pragma unroll
                 for (int k = 0; k < 8; k++) f[k] -= cut16(f[k]);
             }
+            xl[vi * 64 + P - 1] = pack_octet_near(f);
 #pragma unroll
             for (int p = P; p < 4; p++) xl[vi * 64 + p] = make_uint4(0, 0, 0, 0);
             wave_lds_fence();
