@@ -301,7 +301,7 @@ typedef struct le_g4 {
  * xstride values apart (0: one row for all). x and y are of type xtype; with swiglu 0, a is x's row of cols values, with
  * swiglu 1 a[c] = silu(row[c]) * row[cols + c] for a row of 2 * cols (gate | up), silu(g) = g / (1 + exp(-g)).
  * Activations are held to 2^-22 of their value (fp16 and bf16 without SwiGLU exactly, SwiGLU's of 16-bit types to 2^-16) or to 2^-39 of
- * the largest of their 128 columns, whichever is more; products with codes are exact, sums are fp32, and the result is rounded
+ * the largest of their 128 columns, whichever is more, SwiGLU's beside the 2^-21 (or fp32's least values) to which it is formed; products with codes are exact, sums are fp32, and the result is rounded
  * once to xtype. A row's activations, finite, may be of any magnitude whose sums fp32 holds; one that is not finite makes
  * its token's outputs infinite or NaN. Limits: m <= 64, slots <= 65535, cols <= 2^24, slots * m * rows <= 2^31,
  * a matrix's codes and its scales each below 4 GiB; x 16-byte aligned, xstride a multiple of 16 bytes. y may not overlap an

@@ -82,15 +82,35 @@ static __device__ __forceinline__ bf16x8 unpack(unsigned q, unsigned k) {
 static __device__ __forceinline__ f32x4 mfma(const uint4 &a, const bf16x8 &b, const f32x4 &c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), b, c, 0, 0, 0);
 }
-/* silu(g) * u = g u / (1 + 2^t), t = -g log2 e held as t + lo; the exponential and the reciprocal are the hardware's (1 ulp each). t stops
- * at 126, where the result is below 2^-118 |u| already, and 0 is given beyond (not for NaN and infinities: 0 g is NaN). Below -126 there
- * is no lo to add, and t0, which g of 2^127 and more make infinite, gives none. */
-static __device__ __forceinline__ float silu_mul(float g, float u) {
-    const float l2e = 1.44269502f, t0 = -g * l2e, t = fminf(t0, 126.f);
-    const float lo = fabsf(t0) <= 126.f ? __builtin_fmaf(-g, l2e, -t0) - g * 1.92596299e-8f : 0.f;
-    const float e0 = __builtin_amdgcn_exp2f(t), e = __builtin_fmaf(e0 * 0.693147181f, lo, e0);
-    const float q = t0 > 126.f ? 0.f : __builtin_amdgcn_rcpf(1.f + e);
-    return g * q * u;
+/* silu(g) * u = g u / (1 + 2^t), t = -g log2 e held as t0 + lo; the exponential and the reciprocal are the hardware's (1 ulp each), and with
+ * the roundings of 1 + e and of the two products the result is within 2^-21 of its value. Below -126 there is no lo to add, and t0, which g of
+ * 2^127 and more make infinite, gives none.
+ * FAR: t0 beyond 126 too, where 1 + 2^t is 2^t to fp32 and its reciprocal may be below fp32's normal values though the product with a large
+ * u is not: g 2^-t u, with 2^-t as 2^(n - t) in (1/2, 1], which cannot overflow g, and half of 2^-n to each factor. From n = 512 on that
+ * is 0 for all finite g and u (2^128 2^-256 each); g of -infinity stays infinite, or NaN. */
+constexpr float kLog2e = 1.44269502f, kLn2 = 0.693147181f;
+template <bool FAR> static __device__ __forceinline__ float silu_mul(float g, float u) {
+    const float t0 = -g * kLog2e, t = FAR ? fminf(t0, 126.f) : t0;
+    const float lo = fabsf(t0) <= (FAR ? 512.f : 126.f) ? __builtin_fmaf(-g, kLog2e, -t0) - g * 1.92596299e-8f : 0.f;
+    const float e0 = __builtin_amdgcn_exp2f(t), e = __builtin_fmaf(e0 * kLn2, lo, e0);
+    const float r = g * __builtin_amdgcn_rcpf(1.f + e) * u;
+    if (!FAR) return r;
+    const float c = fminf(t0, 512.f), n = floorf(c), f = __builtin_amdgcn_exp2f(n - c);
+    const int i = (int)n, h = i >> 1;
+    return t0 > 126.f ? __builtin_ldexpf(g * __builtin_fmaf(f * -kLn2, lo, f), -h) * __builtin_ldexpf(u, h - i) : r;
+}
+/* Eight of them; the far form, which hardly any gates need, apart: in the way of every call it cost 4096 x 4096 0.3 of 4.9 us. */
+static __device__ __forceinline__ void silu_mul_octet(float (&g)[8], const float (&u)[8]) {
+    float least = g[0];
+#pragma unroll
+    for (int k = 1; k < 8; k++) least = fminf(least, g[k]);
+    if (__builtin_expect(-least * kLog2e > 126.f, 0)) {
+#pragma unroll
+        for (int k = 0; k < 8; k++) g[k] = silu_mul<true>(g[k], u[k]);
+    } else {
+#pragma unroll
+        for (int k = 0; k < 8; k++) g[k] = silu_mul<false>(g[k], u[k]);
+    }
 }
 static __device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc(const void *p, unsigned n) { return __builtin_amdgcn_make_buffer_rsrc((void *)p, 0, n, 0x00027000); }
 /* LDS writes of this wave's lanes are seen by its later reads (no other wave touches them). */
@@ -209,8 +229,7 @@ template <int XTY, bool SW, int T, int P, int STY, int SUB, bool VEC, bool MP> _
             if constexpr (SW) {
                 float u[8];
                 xn.u[0].up(u);
-#pragma unroll
-                for (int k = 0; k < 8; k++) f[k] = silu_mul(f[k], u[k]);
+                silu_mul_octet(f, u);
             }
             const bool in = x_col(pass, 0) < a.cols;
 #pragma unroll
@@ -413,8 +432,7 @@ template <int XTY, bool SW, int P, int SUB> __device__ __forceinline__ void g4x_
     if constexpr (SW) {
         float u[8];
         uo.up(u);
-#pragma unroll
-        for (int k = 0; k < 8; k++) f[k] = silu_mul(f[k], u[k]);
+        silu_mul_octet(f, u);
     }
     float big = 0.f;
 #pragma unroll

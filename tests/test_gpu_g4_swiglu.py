@@ -2,7 +2,7 @@
 import pytest
 
 import lastengine_amd as le
-from tests.test_gpu_g4 import torch_type
+from tests.test_gpu_g4 import run, torch_type
 
 pytestmark = pytest.mark.gpu
 
@@ -39,3 +39,20 @@ def test_sixteen_bit_products_are_rounded(engine, ty):
     bound = (1 + 1 / 16 + 0.27) * 2.0 ** -16 * a0 + torch.finfo(dt).eps / 2 * want.abs()
     assert (want.abs() <= 2.0 ** -8 * a0 * 1.01).all()
     assert (err <= bound).all(), float((err / bound).max())
+
+
+@pytest.mark.parametrize("ty", [le.F32, le.BF16])
+@pytest.mark.parametrize("m", [1, 3, 20])
+@pytest.mark.parametrize("gate", [-86.0, -87.5, -88.5, -92.0, -99.0, -104.0])
+def test_far_gates_and_large_ups(engine, ty, m, gate):
+    """Gates whose exponential fp32 does not hold, or not in full, beside ups so large that the product is an ordinary number.
+
+    Activations lie between 2e38 and 3e38 times silu(gate +- 0.25), so all count alike. Their error, 2^-21 and 2^-16 or 2^-22 of the value, is
+    below the bound's (cols + 8) 2^-24 times 47 of them; a product taken as 0 is off by all of it."""
+    import torch
+    cols = 256
+    gen = torch.Generator().manual_seed(610)
+    g = gate + torch.rand(m, cols, generator=gen) * 0.5 - 0.25
+    u = (torch.rand(m, cols, generator=gen) * 1e38 + 2e38) * torch.where(torch.rand(m, cols, generator=gen) < 0.5, -1.0, 1.0)
+    x = torch.cat([g, u], 1).to(torch_type(ty))
+    run(engine, ty, le.F16, 1, 40, cols, 64, m, 1, 1, None, True, True, 611, x=x, rms=False)
