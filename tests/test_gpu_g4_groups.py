@@ -96,3 +96,26 @@ def test_several_row_groups_a_block(engine, case):
             check(got[s], (act @ wf).cpu(), (act.abs() @ mag).cpu(), ty, cols)
     for s in range(slots):
         assert sel[s] >= 0 or (got[s] == 0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", [c for c in CASES if c[0][:6] in ("le_g4t", "le_g4m")][::2] + CASES[:2], ids=lambda c: c[0])
+def test_same_bits_whatever_the_workspace_held(engine, case):
+    """Sums in a fixed order: equal bits from call to call, with nothing read from the workspace that the call has not written, on blocks of
+    several row groups and K in one segment or several."""
+    import torch
+    name, ty, stype, zeros, rows, cols, group, m, slots, share, swiglu = case
+    print(case, flush=True)
+    codes, scales, z = make(N_MAT, rows, cols, group, stype, zeros, 720 + rows)
+    w = le.G4(codes.cuda(), scales.cuda(), z.cuda() if zeros else None, rows, cols, group, n_mat=N_MAT)
+    x = torch.randn(-(-slots // share) * m, cols * (1 + swiglu), generator=torch.Generator().manual_seed(721)).to(torch_type(ty)).cuda()
+    sel = torch.tensor(selection(slots), dtype=torch.int32).cuda()
+    need = engine.mv_g4_workspace_size(ty, w, m, slots, share, swiglu)
+    outs = []
+    for fill in (0x00, 0xFF, 0x7C, 0x3F):  # zeros, NaN, fp16 and fp32 of ordinary and large size
+        ws = torch.full((need,), fill, dtype=torch.uint8, device="cuda") if need else None
+        out = torch.full((slots, m, rows), float("nan"), dtype=torch_type(ty), device="cuda")
+        engine.mv_g4(ty, w, x, out, m=m, slots=slots, share=share, sel=sel, swiglu=swiglu, ws=ws)
+        outs.append(out)
+    torch.cuda.synchronize()
+    assert torch.isfinite(outs[0]).all() and all(torch.equal(o, outs[0]) for o in outs[1:])
