@@ -301,11 +301,15 @@ typedef struct le_g4 {
  * xstride values apart (0: one row for all). x and y are of type xtype; with swiglu 0, a is x's row of cols values, with
  * swiglu 1 a[c] = silu(row[c]) * row[cols + c] for a row of 2 * cols (gate | up), silu(g) = g / (1 + exp(-g)).
  * Activations are held to 2^-22 of their value (fp16 and bf16 without SwiGLU exactly, SwiGLU's of 16-bit types to 2^-16) or to 2^-39 of
- * the largest of their 128 columns, whichever is more, SwiGLU's beside the 2^-21 (or fp32's least values) to which it is formed; products with codes are exact, sums are fp32, and the result is rounded
- * once to xtype. A row's activations, finite, may be of any magnitude whose sums fp32 holds; one that is not finite makes
- * its token's outputs infinite or NaN. Limits: m <= 64, slots <= 65535, cols <= 2^24, slots * m * rows <= 2^31,
- * a matrix's codes and its scales each below 4 GiB; x 16-byte aligned, xstride a multiple of 16 bytes. y may not overlap an
- * input.
+ * the largest of their 128 columns, whichever is more; SwiGLU's besides to the 2^-21 (or fp32's least values) to which it is formed.
+ * Sums are fp32, of (16 + code) * a and of a for the zero points: products with codes are exact, and the sums' rounding is that of terms
+ * |scale| (47 + |zero|) |a|, not |w| |a|. That shows where activations far above the others meet weights near 0: with eight channels of
+ * 1000 among 4096 of size 1, their weights 0, an output is off by 2e-5 of its value (without such channels by 2e-7 to 6e-7; dequantized
+ * weights summed in fp32 give 6e-7 either way). The result is rounded once to xtype. Finite activations may be of any magnitude for which 31 times the sum of
+ * |a| over 128 columns, and the result, are below 2^128; one that is not finite makes its token's outputs infinite or NaN.
+ * Limits: m <= 64, slots <= 65535, cols <= 2^24, slots * m * rows <= 2^31, and, where a workspace is needed, rows of x (slots / share, rounded
+ * up, times m) <= 65535; a matrix's codes and its scales each below 4 GiB; x 16-byte aligned, xstride a multiple of 16 bytes. y may
+ * not overlap an input.
  * ws: le_matvec_g4_workspace_size bytes (16-byte aligned; NULL where that is 0: one token, and without SwiGLU two in fp16
  * and up to four in bf16), which every call writes anew; calls that may overlap need workspaces of their own. */
 size_t le_matvec_g4_workspace_size(const le_g4 *w, int xtype, int m, int slots, int share, int swiglu);
