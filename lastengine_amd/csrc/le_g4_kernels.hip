@@ -407,7 +407,7 @@ LE_G4_SUBS(LE_G4Q1, bf16t4, 30, false, 4, 1)
 
 /* ---- more tokens: activations laid out by a launch of their own ----
  *
- * le_g4x_*: the activations as MFMA fragments in the workspace, 16 bytes a lane: up to 16 virtual rows (tokens times pieces, a.na sets of
+ * le_g4x_*: the activations as MFMA fragments in the workspace, 16 bytes a lane: up to 12 virtual rows (tokens times pieces, a.na sets of
  * four) as le_g4t_* takes them, [slice of 512 columns][MFMA j][set][lane]; more tokens as le_g4m_* does, tiles of 16,
  * [chunk of 128 columns][MFMA j][piece][lane group][token]. SwiGLU and the cut into pieces are thus done once a launch and not once a block. The pieces are
  * fp16 here, of the chunk's activations times the power of two that brings the largest to [2^14, 2^15): one piece holds bf16 and fp16, two hold
@@ -625,12 +625,12 @@ template <int NA, int P, int STY, int SUB, bool VEC> __device__ __forceinline__ 
 /* le_g4m_*: 16 tokens as the rows of v_mfma_f32_16x16x32_f16, 16 weight rows as its columns (codes as fp16 16 + code): lane (n, g) loads
  * 16 bytes of row n at 32 g of a chunk. A wave keeps the fragments of a slice of CS chunks in registers and goes over the block's row
  * groups with it, as above. Where K has more chunks than the waves of a block hold, it is cut into segments, each a block's own, whose
- * partial results le_g4s_* adds: with passes instead (as le_g4q_*), every block of a long K reads all fragments for its few
+ * partial results le_g4s adds: with passes instead (as le_g4q_*), every block of a long K reads all fragments for its few
  * rows, one pass's at a time (4096 x 14336, five tokens: 29 us). The scales of
  * an item are loaded once by the lane groups together and passed between them: loaded by each lane group they were a third of the
  * time (14336 x 4096 bf16, five tokens 18.4 us, 12.6 without those loads). 14336 x 4096 fp32, groups of 128: 16 tokens 17.0 us, 32 22.8, 64 34.7. */
 template <int P, int STY, int SUB, bool VEC, int CS> __device__ __forceinline__ void g4m_body(const G4Args &a) {
-    constexpr int SB = STY == 0 ? 4 : 2, BPC = 128 / SUB, NSUB = CS * BPC, NL = NSUB < 4 ? 1 : NSUB / 4; /* scale blocks of an item's row, of them a lane's to load */
+    constexpr int SB = STY == 0 ? 4 : 2, BPC = 128 / SUB, NL = CS * BPC / 4; /* NL: of an item's scale blocks, a lane's to load */
     struct Item {
         uint4 q[CS];
         Scales<STY, NL, VEC && (NL > 1)> s, z;
@@ -677,7 +677,7 @@ template <int P, int STY, int SUB, bool VEC, int CS> __device__ __forceinline__ 
         const int gr = (int)blockIdx.x + gi * a.gx;
         const bool there = gi < G;
         const auto rq = rsrc(w0, there ? bytes : 0), rs = rsrc(s0, there ? sbytes : 0), rz = rsrc(z0, there && a.zeros ? sbytes : 0);
-        const int b0 = c0 * BPC + (NSUB < 4 ? g % NSUB : g * NL);
+        const int b0 = c0 * BPC + g * NL;
         const unsigned row = (gr * 16 + n) * a.ng;
         it.s.load(rs, row, b0, SUB, a.cols, a.gshift, a.ng);
         it.z.load(rz, row, b0, SUB, a.cols, a.gshift, a.ng);
