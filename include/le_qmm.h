@@ -304,7 +304,7 @@ typedef struct le_g4 {
  * the largest of their 128 columns, whichever is more; SwiGLU's besides to the 2^-21 (or fp32's least values) to which it is formed.
  * Sums are fp32, of (16 + code) * a and of a for the zero points: products with codes are exact, and the sums' rounding is that of terms
  * |scale| (47 + |zero|) |a|, not |w| |a|. That shows where activations far above the others meet weights near 0: with eight channels of
- * 1000 among 4096 of size 1, their weights 0, an output is off by 2e-5 of its value (without such channels by 2e-7 to 6e-7; dequantized
+ * 1000 among 4096 of size 1, their weights 0, an output is off by 1e-5 to 3e-5 of its value (without such channels by 2e-7 to 6e-7; dequantized
  * weights summed in fp32 give 6e-7 either way). The result is rounded once to xtype. Finite activations may be of any magnitude for which 31 times the sum of
  * |a| over 128 columns, and the result, are below 2^128; one that is not finite makes its token's outputs infinite or NaN.
  * Limits: m <= 64, slots <= 65535, cols <= 2^24, slots * m * rows <= 2^31, and, where a workspace is needed, rows of x (slots / share, rounded

@@ -12,8 +12,9 @@ namespace {
 int type_bytes(int ty) { return ty == LE_F32 ? 4 : ty == LE_F16 || ty == LE_BF16 ? 2 : 0; }
 bool aligned(const void *p, unsigned n) { return ((uintptr_t)p & (n - 1)) == 0; }
 
-/* One launch: bf16 pieces that hold an activation: 24 bits of fp32 in three, 11 of fp16 in two. SwiGLU's fp32 result: three, or the 16
- * bits of two where the output is rounded to 11 or 8. */
+/* (Times in this file: graph replays over 700 MB of weights, which no cache holds.)
+ * One launch: bf16 pieces that hold an activation: 24 bits of fp32 in three, 11 of fp16 in two. SwiGLU's fp32 result: three, or the 16
+ * bits of two, rounded, where the output is rounded to 11 or 8. */
 int pieces(int xtype, int swiglu) { return xtype == LE_F32 ? 3 : xtype == LE_F16 || swiglu ? 2 : 1; }
 /* Columns that a scale is applied to at a time. */
 int scale_block(const le_g4 *w) { return w->group % 128 == 0 || w->group == w->cols ? 128 : w->group % 64 == 0 ? 64 : 32; }

@@ -32,9 +32,9 @@
  * Codes of the next two items are on their way while one is multiplied; loads of items that do not exist and of rows past the end
  * are cut off by the buffer's size and fetch nothing.
  *
- * One token, weights from HBM (a streaming read of as many bytes at this size): 28672 x 4096 bf16, groups of 128, 62 MB 13.1 us (11.8),
- * 14336 x 4096 fp32 31 MB 8.2 (6.9), groups of 32 37 MB 9.4, 4096 x 4096 4.7 (3.5), 1024 x 2048 3.15 (2.7), 4096 x 14336 SwiGLU
- * fp32, groups of 64, 33 MB 13.0 (7.3): there each of 256 blocks reads all of x, forms SwiGLU and goes over K twice for its
+ * One token, weights from HBM (graph replays over 700 MB of them; in brackets a streaming read of as many bytes): 28672 x 4096 bf16, groups of
+ * 128, 62 MB 13.1 us (11.8), 14336 x 4096 fp32 31 MB 8.2 (6.9), groups of 32 37 MB 9.4, 4096 x 4096 4.7 (3.5), 1024 x 2048 3.15 (2.7), 4096 x 14336
+ * SwiGLU fp32, groups of 64, 33 MB 13.0 (7.3): there each of 256 blocks reads all of x, forms SwiGLU and goes over K twice for its
  * 16 rows. What the types and groups choose is compiled in: as branches on arguments it cost 14336 x 4096 in groups of 32 5.6 us. */
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
