@@ -356,6 +356,67 @@ int le_moe_combine(le_ctx *ctx, int ty, const void *e, long long lde, int n_row,
 int le_moe_combine_bwd(le_ctx *ctx, int ty, const void *dout, long long ldt, const void *e, long long lde, int n_row,
                        const int *pos, const float *w, int n_tok, int k, int cols, void *de, float *dw, le_stream_t stream);
 
+/* ---- products of the routed experts over dense weights, with their gradients (no counterpart in the reference, whose experts
+ *      are GGUF blocks and are not trained; le_mm_grouped is the form for GGUF weights) ----
+ * w holds n_exp matrices of rows x cols, row-major and contiguous, matrix after matrix, of type ty (LE_F32, LE_F16, LE_BF16), as the
+ * rows of x, y, dx and dy. Expert e has the rows off[e] <= i < off[e + 1] (place order, as le_moe_sort and le_moe_permute leave them;
+ * off: n_exp + 1 device ints that do not fall). x and dx have rows of cols values, ldx values apart, y and dy rows of `rows` values, ldy
+ * apart; n_row is how many rows these buffers have, and rows of no expert (from off[n_exp] on) are not read and stay as they were.
+ *   le_mm_experts:    y[i] = W_e x[i]
+ *   le_mm_experts_dx: dx[i] = W_e^T dy[i], the gradient of x
+ *   le_mm_experts_dw: dW_e = sum over e's rows i of dy[i] x[i]^T, the gradient of w, of type dwtype (ty or LE_F32); zeros for an expert
+ *                     without rows
+ * Products are exact (fp32: rounded as in a fused multiply-add), sums fp32 in an order that the sizes, off and alignment decide (the same
+ * bits from call to call), the result is rounded once. Any rows, cols >= 1, any strides >= the row; sizes, strides and
+ * pointers that are multiples of 16 bytes are faster. A row that is not finite makes its own results infinite or NaN (in dw, its
+ * expert's), and no others.
+ * Limits: n_exp <= 1024, rows and cols <= 2^24, n_row <= 2^30. n_row may be 0. Outputs may not overlap inputs.
+ * ws of le_mm_experts_dw: le_mm_experts_dw_workspace_size bytes, 16-byte aligned (NULL where that is 0), which every call writes anew; calls that
+ * may overlap need workspaces of their own. */
+int le_mm_experts(le_ctx *ctx, int ty, const void *w, const int *off, int n_exp, const void *x, long long ldx, void *y,
+                  long long ldy, int n_row, int rows, int cols, le_stream_t stream);
+int le_mm_experts_dx(le_ctx *ctx, int ty, const void *w, const int *off, int n_exp, const void *dy, long long ldy, void *dx,
+                     long long ldx, int n_row, int rows, int cols, le_stream_t stream);
+size_t le_mm_experts_dw_workspace_size(int ty, int n_exp, int n_row, int rows, int cols);
+int le_mm_experts_dw(le_ctx *ctx, int ty, const void *dy, long long ldy, const void *x, long long ldx, const int *off, int n_exp,
+                     int dwtype, void *dw, int n_row, int rows, int cols, void *ws, size_t ws_bytes, le_stream_t stream);
+
+/* ---- low-rank adapters of many requests beside a shared projection (no counterpart in the reference) ----
+ * n_ad adapters of one shape: a (rank x cols each) and b (rows x rank each), row-major and contiguous, adapter after adapter, of type
+ * ltype (LE_F32, LE_F16, LE_BF16), and a factor each, scale (fp32; NULL stands for 1). Adapters of lower rank are filled up with
+ * zeros. */
+typedef struct le_adapters {
+    const void *a, *b;  /* device */
+    const float *scale; /* device, or NULL */
+    int n_ad, rank, rows, cols, ltype;
+} le_adapters;
+/* For token t < m, with i = idx[t]:  y[t] = base[t] + scale_i * B_i (A_i x[t]);  y[t] = base[t] where i lies outside 0 .. n_ad - 1.
+ * base is what the shared projection gave (le_gemm, le_matvec, le_matvec_g4), NULL stands for zeros; base may be y. x, base and y are
+ * of type xtype, x's rows of cols values ldx apart (0: one row for all), base's and y's of `rows` values ldb and ldy apart. Products
+ * with A are exact and summed in fp32, A_i x[t] and its product with scale_i are held in fp32, and so are the sums over the rank and with base; the
+ * result is rounded once. Tokens of one adapter need not follow one another, but for many tokens runs of 16 and more are faster.
+ * Limits: rank <= 256, rows and cols <= 2^24, m <= 2^20, n_ad >= 1; m may be 0. y may not overlap other inputs, nor base otherwise.
+ * ws: le_lora_workspace_size bytes, 16-byte aligned, which every call writes anew; calls that may overlap need workspaces of
+ * their own. */
+size_t le_lora_workspace_size(const le_adapters *ad, int xtype, int m);
+int le_lora(le_ctx *ctx, const le_adapters *ad, const int *idx, int xtype, const void *x, long long ldx, int m,
+            const void *base, long long ldb, void *y, long long ldy, void *ws, size_t ws_bytes, le_stream_t stream);
+
+/* ---- the residual's addition, RMS norm and int8 activations in one launch, for many tokens (the reference's add_rmsnorm,
+ *      src/cuda/kernels.cu:409-427, and rms_quant, src/cuda/dense.cu:33-56, as one; le_rms_quant is the form for one fp32 row) ----
+ * For row t < m of n values of type ty (LE_F32, LE_F16, LE_BF16):
+ *     h[t] = x[t] + res[t], rounded to ty (res NULL: x[t])
+ *     o[t][i] = (h[t][i] * r) * w[i] in fp32, r = 1 / sqrt(sum of h[t]^2 / n + eps), sum, r and the first product in 64 bits
+ *     xd[t][u] = max |o[t][32u ..]| / 127,  xq[t][i] = o[t][i] * (1 / xd) to the nearest even, within -127 .. 127 (0 where xd is 0),
+ *     xs[t][u] = sum of the unit's xq: the activations that le_matvec_q8 takes, from o before it is rounded to ty.
+ * w is fp32. The 64 bits make codes next to a border those of the formula, whatever order a sum is taken in. A row with a value that is not
+ * finite, or of zeros where eps is 0, has NaN in o and xd, and 0 in xq and xs. h, o and xs may be NULL; xq and xd may both be NULL (then n is any, else a
+ * multiple of 32). x, res, h and o have rows ldx, ldr, ldh and ldo values apart (>= n), xq rows of n, xd and xs of n / 32, back to back.
+ * h may be x or res (with its row stride); outputs may not overlap inputs otherwise. eps >= 0. Limits: n <= 2^24, m < 2^31; m may be 0. */
+int le_add_rms_quant(le_ctx *ctx, int ty, const void *x, long long ldx, const void *res, long long ldr, const float *w, void *h,
+                     long long ldh, void *o, long long ldo, int8_t *xq, float *xd, int32_t *xs, int m, int n, float eps,
+                     le_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

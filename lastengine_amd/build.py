@@ -27,12 +27,18 @@ PARTS["mt"] = []
 for _ty in (0, 1, 30):
     PARTS["g4s%d" % _ty] = ["-DLE_G4_STY=%d" % _ty]
 PARTS["rt"] = []
+for _ty in (0, 1, 30):
+    PARTS["ex%d" % _ty] = ["-DLE_EX_TY=%d" % _ty]
+    PARTS["lo%d" % _ty] = ["-DLE_LO_XTY=%d" % _ty]
+PARTS["nq"] = []
 PARTS["gq"] = ["-DLE_GQ_SET=1"]
 PARTS["gq2"] = ["-DLE_GQ_SET=2"]
 SOURCES = {"gm": "le_gemm_kernels.hip", "mt": "le_mt_kernels.hip", "gq": "le_gq_kernels.hip", "gq2": "le_gq_kernels.hip",
-           "g4s0": "le_g4_kernels.hip", "g4s1": "le_g4_kernels.hip", "g4s30": "le_g4_kernels.hip", "rt": "le_route_kernels.hip"}  # parts not listed here compile le_qmm_kernels.hip
+           "g4s0": "le_g4_kernels.hip", "g4s1": "le_g4_kernels.hip", "g4s30": "le_g4_kernels.hip", "rt": "le_route_kernels.hip",
+           "ex0": "le_experts_kernels.hip", "ex1": "le_experts_kernels.hip", "ex30": "le_experts_kernels.hip", "lo0": "le_lora_kernels.hip",
+           "lo1": "le_lora_kernels.hip", "lo30": "le_lora_kernels.hip", "nq": "le_norm_kernels.hip"}  # parts not listed here compile le_qmm_kernels.hip
 
-HOST_SOURCES = ["le_qmm.cpp", "le_g4.cpp", "le_route.cpp", "le_quant.cpp", "le_gguf.cpp"]
+HOST_SOURCES = ["le_qmm.cpp", "le_g4.cpp", "le_route.cpp", "le_experts.cpp", "le_lora.cpp", "le_norm.cpp", "le_quant.cpp", "le_gguf.cpp"]
 # Host sources that declare device memory (hipcc, host and device passes), linked into the library.
 HIP_HOST_SOURCES = ["le_noalloc.hip"]
 

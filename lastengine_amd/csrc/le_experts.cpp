@@ -1,0 +1,90 @@
+/* Host side of the routed experts' products (le_mm_experts and its gradients, include/le_qmm.h): argument checks and launch shapes. */
+#include <algorithm>
+#include <cstdio>
+
+#include "le_checks.h"
+#include "le_ctx.h"
+#include "le_experts_args.h"
+
+namespace {
+
+constexpr int kSide = 1 << 24, kExperts = 1024, kRows = 1 << 30;
+
+int check_sizes(le_ctx *c, int ty, int n_exp, int n_row, int rows, int cols, long long ldx, long long ldy) {
+    if (!le_type_bytes(ty)) return le_ctx_failf(c, LE_ERR_TYPE, "rows of type %d", ty);
+    if (n_exp <= 0 || n_exp > kExperts || n_row < 0 || n_row > kRows || rows <= 0 || cols <= 0 || rows > kSide || cols > kSide)
+        return le_ctx_failf(c, LE_ERR_SHAPE, "n_exp=%d (1..1024), n_row=%d (0..2^30), rows=%d, cols=%d (1..2^24)", n_exp, n_row, rows, cols);
+    if (ldx < cols || ldy < rows) return le_ctx_failf(c, LE_ERR_SHAPE, "row strides %lld and %lld of %d and %d values", ldx, ldy, cols, rows);
+    return LE_OK;
+}
+
+/* Blocks for `tiles` tiles: whole turns of the eight XCDs with `run` tiles each (le_experts_kernels.hip, tile_of), in a loop beyond 2^23 */
+unsigned blocks_for(long long tiles, int run) {
+    const long long turn = 8LL * run;
+    return (unsigned)std::min((tiles + turn - 1) / turn * turn, (1LL << 23) / turn * turn);
+}
+
+int launch(le_ctx *c, const char *what, ExpertArgs &a, long long row_tiles, le_stream_t stream) {
+    a.run = 1;
+    void *args[] = {&a};
+    return le_ctx_launch(c, what, dim3(blocks_for(row_tiles * a.nt, a.run)), 256, 0, (hipStream_t)stream, args);
+}
+
+}  // namespace
+
+extern "C" {
+
+int le_mm_experts(le_ctx *c, int ty, const void *w, const int *off, int n_exp, const void *x, long long ldx, void *y,
+                  long long ldy, int n_row, int rows, int cols, le_stream_t stream) {
+    if (!c) return LE_ERR_ARG;
+    if (int rc = check_sizes(c, ty, n_exp, n_row, rows, cols, ldx, ldy)) return rc;
+    if (n_row == 0) return LE_OK;
+    if (!w || !off || !x || !y) return le_ctx_fail(c, LE_ERR_ARG, "null pointer");
+    const int b = le_type_bytes(ty);
+    if (!le_aligned(w, b) || !le_aligned(x, b) || !le_aligned(y, b) || !le_aligned(off, 4))
+        return le_ctx_fail(c, LE_ERR_ALIGN, "pointers must be aligned to their types");
+    if (int rc = le_ctx_on_device(c)) return rc;
+    ExpertArgs a{x, w, y, off, ldx, cols, ldy, n_exp, n_row, n_row, rows, cols, 0, (rows + 127) / 128, 1};
+    char name[40];
+    snprintf(name, sizeof name, "le_ex_y_%d_any", ty);
+    return launch(c, name, a, n_row / 128 + std::min(n_exp, n_row), stream);
+}
+
+int le_mm_experts_dx(le_ctx *c, int ty, const void *w, const int *off, int n_exp, const void *dy, long long ldy, void *dx,
+                     long long ldx, int n_row, int rows, int cols, le_stream_t stream) {
+    if (!c) return LE_ERR_ARG;
+    if (int rc = check_sizes(c, ty, n_exp, n_row, rows, cols, ldx, ldy)) return rc;
+    if (n_row == 0) return LE_OK;
+    if (!w || !off || !dy || !dx) return le_ctx_fail(c, LE_ERR_ARG, "null pointer");
+    const int b = le_type_bytes(ty);
+    if (!le_aligned(w, b) || !le_aligned(dy, b) || !le_aligned(dx, b) || !le_aligned(off, 4))
+        return le_ctx_fail(c, LE_ERR_ALIGN, "pointers must be aligned to their types");
+    if (int rc = le_ctx_on_device(c)) return rc;
+    ExpertArgs a{dy, w, dx, off, ldy, cols, ldx, n_exp, n_row, n_row, cols, rows, 0, (cols + 127) / 128, 1};
+    char name[40];
+    snprintf(name, sizeof name, "le_ex_dx_%d_any", ty);
+    return launch(c, name, a, n_row / 128 + std::min(n_exp, n_row), stream);
+}
+
+size_t le_mm_experts_dw_workspace_size(int, int, int, int, int) { return 0; }
+
+int le_mm_experts_dw(le_ctx *c, int ty, const void *dy, long long ldy, const void *x, long long ldx, const int *off, int n_exp,
+                     int dwtype, void *dw, int n_row, int rows, int cols, void *ws, size_t ws_bytes, le_stream_t stream) {
+    if (!c) return LE_ERR_ARG;
+    if (int rc = check_sizes(c, ty, n_exp, n_row, rows, cols, ldx, ldy)) return rc;
+    if (dwtype != ty && dwtype != LE_F32) return le_ctx_failf(c, LE_ERR_TYPE, "dw of type %d for rows of type %d", dwtype, ty);
+    if (!off || !dw || (n_row && (!dy || !x))) return le_ctx_fail(c, LE_ERR_ARG, "null pointer");
+    const int b = le_type_bytes(ty);
+    if (!le_aligned(dy, b) || !le_aligned(x, b) || !le_aligned(dw, le_type_bytes(dwtype)) || !le_aligned(off, 4) || !le_aligned(ws, 16))
+        return le_ctx_fail(c, LE_ERR_ALIGN, "pointers must be aligned to their types, ws to 16 bytes");
+    const size_t need = le_mm_experts_dw_workspace_size(ty, n_exp, n_row, rows, cols);
+    if (need && (!ws || ws_bytes < need)) return le_ctx_failf(c, LE_ERR_WORKSPACE, "workspace needs %zu bytes", need);
+    ExpertArgs a{dy, x, dw, off, ldy, ldx, cols, n_exp, n_row, rows, cols, n_row, (rows + 127) / 128, (cols + 127) / 128, 1};
+    if ((long long)a.mt * a.nt * n_exp > 0x7FFFFFFFLL) return le_ctx_fail(c, LE_ERR_SHAPE, "more than 2^31 tiles of 128 x 128");
+    if (int rc = le_ctx_on_device(c)) return rc;
+    char name[40];
+    snprintf(name, sizeof name, "le_ex_dw%s_%d_any", dwtype == ty ? "" : "f", ty);
+    return launch(c, name, a, (long long)a.mt * n_exp, stream);
+}
+
+}  // extern "C"

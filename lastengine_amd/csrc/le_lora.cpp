@@ -1,0 +1,55 @@
+/* Host side of the low-rank adapters (le_lora, include/le_qmm.h): argument checks and launch shapes. */
+#include <algorithm>
+#include <cstdio>
+
+#include "le_checks.h"
+#include "le_ctx.h"
+#include "le_lora_args.h"
+
+namespace {
+
+constexpr int kRank = 256, kSide = 1 << 24, kTokens = 1 << 20;
+
+const char *shape_error(const le_adapters *ad, int m) {
+    if (ad->n_ad <= 0 || ad->rank <= 0 || ad->rank > kRank) return "n_ad below 1 or rank outside 1..256";
+    if (ad->rows <= 0 || ad->cols <= 0 || ad->rows > kSide || ad->cols > kSide) return "rows or cols outside 1..2^24";
+    if (m < 0 || m > kTokens) return "m outside 0..2^20";
+    return nullptr;
+}
+
+}  // namespace
+
+extern "C" size_t le_lora_workspace_size(const le_adapters *ad, int xtype, int m) {
+    if (!ad || !le_type_bytes(xtype) || !le_type_bytes(ad->ltype) || shape_error(ad, m)) return 0;
+    return (size_t)m * ad->rank * 4;
+}
+
+extern "C" int le_lora(le_ctx *c, const le_adapters *ad, const int *idx, int xtype, const void *x, long long ldx, int m,
+                       const void *base, long long ldb, void *y, long long ldy, void *ws, size_t ws_bytes, le_stream_t stream) {
+    if (!c) return LE_ERR_ARG;
+    if (!ad) return le_ctx_fail(c, LE_ERR_ARG, "null pointer");
+    const int xb = le_type_bytes(xtype), wb = le_type_bytes(ad->ltype);
+    if (!xb) return le_ctx_failf(c, LE_ERR_TYPE, "activations of type %d", xtype);
+    if (!wb) return le_ctx_failf(c, LE_ERR_TYPE, "adapters of type %d", ad->ltype);
+    if (const char *e = shape_error(ad, m))
+        return le_ctx_failf(c, LE_ERR_SHAPE, "%s (%d adapters of rank %d, %d x %d, %d tokens)", e, ad->n_ad, ad->rank, ad->rows, ad->cols, m);
+    if ((ldx && ldx < ad->cols) || (base && ldb < ad->rows) || ldy < ad->rows)
+        return le_ctx_failf(c, LE_ERR_SHAPE, "row strides %lld, %lld and %lld of %d and %d values", ldx, ldb, ldy, ad->cols, ad->rows);
+    if (m == 0) return LE_OK;
+    if (!ad->a || !ad->b || !idx || !x || !y) return le_ctx_fail(c, LE_ERR_ARG, "null pointer");
+    if (!le_aligned(ad->a, wb) || !le_aligned(ad->b, wb) || !le_aligned(ad->scale, 4) || !le_aligned(idx, 4) || !le_aligned(x, xb) ||
+        !le_aligned(base, xb) || !le_aligned(y, xb) || !le_aligned(ws, 16))
+        return le_ctx_fail(c, LE_ERR_ALIGN, "pointers must be aligned to their types, ws to 16 bytes");
+    if (base == y && ldb != ldy) return le_ctx_fail(c, LE_ERR_ARG, "y in place of base has its row stride");
+    const size_t need = le_lora_workspace_size(ad, xtype, m);
+    if (!ws || ws_bytes < need) return le_ctx_failf(c, LE_ERR_WORKSPACE, "workspace needs %zu bytes", need);
+    if (int rc = le_ctx_on_device(c)) return rc;
+    LoraArgs a{ad->a, ad->b, ad->scale, idx, x, base, y, (float *)ws, ldx, ldb, ldy, ad->n_ad, ad->rank, ad->rows, ad->cols, m};
+    void *args[] = {&a};
+    char name[40];
+    snprintf(name, sizeof name, "le_lo_down_%d_%d", xtype, ad->ltype);
+    const long long waves = (long long)m * ad->rank;
+    if (int rc = le_ctx_launch(c, name, dim3((unsigned)std::min((waves + 3) / 4, 1LL << 20)), 256, 0, (hipStream_t)stream, args)) return rc;
+    snprintf(name, sizeof name, "le_lo_up_%d_%d", xtype, ad->ltype);
+    return le_ctx_launch(c, name, dim3((unsigned)((ad->rows + 255) / 256), (unsigned)std::min(m, 65535)), 256, 0, (hipStream_t)stream, args);
+}

@@ -1,0 +1,32 @@
+/* Host side of le_add_rms_quant (include/le_qmm.h): argument checks and launch shape. */
+#include <algorithm>
+#include <cmath>
+#include <cstdio>
+
+#include "le_checks.h"
+#include "le_ctx.h"
+#include "le_norm_args.h"
+
+extern "C" int le_add_rms_quant(le_ctx *c, int ty, const void *x, long long ldx, const void *res, long long ldr, const float *w, void *h,
+                                long long ldh, void *o, long long ldo, int8_t *xq, float *xd, int32_t *xs, int m, int n, float eps,
+                                le_stream_t stream) {
+    if (!c) return LE_ERR_ARG;
+    const int b = le_type_bytes(ty);
+    if (!b) return le_ctx_failf(c, LE_ERR_TYPE, "rows of type %d", ty);
+    if (m < 0 || n <= 0 || n > 1 << 24 || (xq && n % 32)) return le_ctx_failf(c, LE_ERR_SHAPE, "m=%d, n=%d (1..2^24, with xq a multiple of 32)", m, n);
+    if (ldx < n || (res && ldr < n) || (h && ldh < n) || (o && ldo < n))
+        return le_ctx_failf(c, LE_ERR_SHAPE, "row strides %lld, %lld, %lld and %lld of %d values", ldx, ldr, ldh, ldo, n);
+    if (!(eps >= 0.f) || std::isinf(eps)) return le_ctx_failf(c, LE_ERR_ARG, "eps=%g", eps);
+    if (!xq != !xd || (xs && !xq)) return le_ctx_fail(c, LE_ERR_ARG, "xq and xd go together, and xs with them");
+    if (m == 0) return LE_OK;
+    if (!x || !w || (!h && !o && !xq)) return le_ctx_fail(c, LE_ERR_ARG, "null pointer");
+    if ((h == x && ldh != ldx) || (h && h == res && ldh != ldr)) return le_ctx_fail(c, LE_ERR_ARG, "h in place of x or res has its row stride");
+    if (!le_aligned(x, b) || !le_aligned(res, b) || !le_aligned(h, b) || !le_aligned(o, b) || !le_aligned(w, 4) || !le_aligned(xd, 4) || !le_aligned(xs, 4))
+        return le_ctx_fail(c, LE_ERR_ALIGN, "pointers must be aligned to their types");
+    if (int rc = le_ctx_on_device(c)) return rc;
+    NormArgs a{x, res, w, h, o, (signed char *)xq, xd, xs, ldx, ldr, ldh, ldo, m, n, eps};
+    void *args[] = {&a};
+    char name[40];
+    snprintf(name, sizeof name, "le_nq_%d", ty);
+    return le_ctx_launch(c, name, dim3((unsigned)std::min(m, 1 << 20)), 256, 0, (hipStream_t)stream, args);
+}

@@ -27,7 +27,8 @@
 namespace {
 
 const char *kParts[] = {"le_qmm_deq", "le_qmm_moe", "le_qmm_mv8", "le_qmm_mv12", "le_qmm_mv14", "le_qmm_mv16", "le_qmm_mv18", "le_qmm_gm",
-                        "le_qmm_gq", "le_qmm_gq2", "le_qmm_mt", "le_qmm_mv2", "le_qmm_mv11", "le_qmm_mv13", "le_qmm_mv22", "le_qmm_g4s0", "le_qmm_g4s1", "le_qmm_g4s30", "le_qmm_rt"};
+                        "le_qmm_gq", "le_qmm_gq2", "le_qmm_mt", "le_qmm_mv2", "le_qmm_mv11", "le_qmm_mv13", "le_qmm_mv22", "le_qmm_g4s0", "le_qmm_g4s1", "le_qmm_g4s30", "le_qmm_rt",
+                        "le_qmm_ex0", "le_qmm_ex1", "le_qmm_ex30", "le_qmm_lo0", "le_qmm_lo1", "le_qmm_lo30", "le_qmm_nq"};
 
 /* Kernel argument block of le_mv_* (mirrors MvArgs in le_qmm_kernels.hip). */
 struct MvArgs {

@@ -95,6 +95,13 @@ def lib():
         "le_moe_permute": (I, [P, I, P, LL, P, I, I, I, P, LL, I, P]),
         "le_moe_combine": (I, [P, I, P, LL, I, P, P, I, I, I, P, LL, P]),
         "le_moe_combine_bwd": (I, [P, I, P, LL, P, LL, I, P, P, I, I, I, P, P, P]),
+        "le_mm_experts": (I, [P, I, P, P, I, P, LL, P, LL, I, I, I, P]),
+        "le_mm_experts_dx": (I, [P, I, P, P, I, P, LL, P, LL, I, I, I, P]),
+        "le_mm_experts_dw_workspace_size": (S, [I, I, I, I, I]),
+        "le_mm_experts_dw": (I, [P, I, P, LL, P, LL, P, I, I, P, I, I, I, P, S, P]),
+        "le_lora_workspace_size": (S, [P, I, I]),
+        "le_lora": (I, [P, P, P, I, P, LL, I, P, LL, P, LL, P, S, P]),
+        "le_add_rms_quant": (I, [P, I, P, LL, P, LL, P, P, LL, P, LL, P, P, P, I, I, F, P]),
         "le_fill_normal": (None, [P, S, ctypes.c_uint64, ctypes.c_uint64, D, D, I]),
         "le_quantize_rows": (I, [I, P, P, S, S, I]),
         "le_f32_to_f16": (ctypes.c_uint16, [F]),
@@ -206,6 +213,31 @@ class G4:
         self.struct = _G4(_ptr(codes), _ptr(scales), _ptr(zeros), n_mat, rows, cols, group, scale_type)
         self.ref = ctypes.addressof(self.struct)
         self.cols = cols
+
+
+class _Adapters(ctypes.Structure):  # le_adapters of include/le_qmm.h
+    _fields_ = [("a", ctypes.c_void_p), ("b", ctypes.c_void_p), ("scale", ctypes.c_void_p), ("n_ad", ctypes.c_int), ("rank", ctypes.c_int),
+                ("rows", ctypes.c_int), ("cols", ctypes.c_int), ("ltype", ctypes.c_int)]
+
+
+class Adapters:
+    """n_ad low-rank adapters of one shape: a (n_ad, rank, cols), b (n_ad, rows, rank) of F32, F16 or BF16 (told by the tensor's dtype, or
+    ltype for raw addresses), scale (n_ad) fp32 or None for 1. Holds the tensors as long as it lives; nothing is copied."""
+
+    def __init__(self, a, b, scale, n_ad, rank, rows, cols, ltype=None):
+        if ltype is None:
+            ltype = dtype_id(a)
+        if hasattr(a, "dtype") and hasattr(b, "dtype") and a.dtype != b.dtype:
+            raise LeError(-2, "a and b of different types")
+        if hasattr(scale, "dtype") and dtype_id(scale) != F32:
+            raise LeError(-2, "scale of type %s" % scale.dtype)
+        for t, n in ((a, rank * cols), (b, rows * rank), (scale, 1)):
+            if hasattr(t, "numel") and (t.numel() != n * n_ad or not t.is_contiguous()):
+                raise LeError(-3, "a tensor of %d values where the %d adapters have %d, contiguous" % (t.numel(), n_ad, n * n_ad))
+        self.tensors = (a, b, scale)
+        self.struct = _Adapters(_ptr(a), _ptr(b), _ptr(scale), n_ad, rank, rows, cols, ltype)
+        self.ref = ctypes.addressof(self.struct)
+        self.rows, self.cols = rows, cols
 
 
 def dtype_id(t):
@@ -383,6 +415,48 @@ class Engine:
         """Gradient of moe_combine: drows[pos[p]] = w[p] * dout[t] and dw[p] = dout[t] . rows[pos[p]] (either may be None)."""
         self._check(self._L.le_moe_combine_bwd(self._ctx, ty, _ptr(dout), ldt or cols, _ptr(rows), lde or cols, n_row, _ptr(pos),
                                                _ptr(w), n_tok, k, cols, _ptr(drows), _ptr(dw), _stream(stream)))
+
+    def mm_experts(self, ty, w, off, x, y, n_exp, n_row, rows, cols, ldx=None, ldy=None, stream=None):
+        """y[i] = W_e x[i] for the rows i of each expert e (off[e] <= i < off[e + 1]); w: n_exp matrices of rows x cols."""
+        self._check(self._L.le_mm_experts(self._ctx, ty, _ptr(w), _ptr(off), n_exp, _ptr(x), ldx or cols, _ptr(y), ldy or rows, n_row,
+                                          rows, cols, _stream(stream)))
+
+    def mm_experts_dx(self, ty, w, off, dy, dx, n_exp, n_row, rows, cols, ldy=None, ldx=None, stream=None):
+        """Gradient of mm_experts' rows: dx[i] = W_e^T dy[i]."""
+        self._check(self._L.le_mm_experts_dx(self._ctx, ty, _ptr(w), _ptr(off), n_exp, _ptr(dy), ldy or rows, _ptr(dx), ldx or cols, n_row,
+                                             rows, cols, _stream(stream)))
+
+    def mm_experts_dw_workspace_size(self, ty, n_exp, n_row, rows, cols):
+        return int(self._L.le_mm_experts_dw_workspace_size(ty, n_exp, n_row, rows, cols))
+
+    def mm_experts_dw(self, ty, dy, x, off, dw, n_exp, n_row, rows, cols, dw_ty=None, ldy=None, ldx=None, ws=None, ws_bytes=None,
+                      stream=None):
+        """Gradient of mm_experts' weights: dW_e = sum of dy[i] x[i]^T over the expert's rows, of type dw_ty (default: ty)."""
+        if ws is None:
+            ws = _workspace(self.mm_experts_dw_workspace_size(ty, n_exp, n_row, rows, cols), stream)
+        if ws_bytes is None:
+            ws_bytes = ws.numel() if hasattr(ws, "numel") else 0
+        self._check(self._L.le_mm_experts_dw(self._ctx, ty, _ptr(dy), ldy or rows, _ptr(x), ldx or cols, _ptr(off), n_exp,
+                                             ty if dw_ty is None else dw_ty, _ptr(dw), n_row, rows, cols, _ptr(ws), ws_bytes, _stream(stream)))
+
+    def lora_workspace_size(self, ty, adapters, m):
+        return int(self._L.le_lora_workspace_size(adapters.ref, ty, m))
+
+    def lora(self, ty, adapters, idx, x, base, y, m, ldx=None, ldb=None, ldy=None, ws=None, ws_bytes=None, stream=None):
+        """y[t] = base[t] + scale_i B_i (A_i x[t]) with i = idx[t] (an Adapters' number; any other: y[t] = base[t]); base None: zeros.
+        ldx 0: one row of x for all tokens."""
+        if ws is None:
+            ws = _workspace(self.lora_workspace_size(ty, adapters, m), stream)
+        if ws_bytes is None:
+            ws_bytes = ws.numel() if hasattr(ws, "numel") else 0
+        self._check(self._L.le_lora(self._ctx, adapters.ref, _ptr(idx), ty, _ptr(x), adapters.cols if ldx is None else ldx, m, _ptr(base),
+                                    ldb or adapters.rows, _ptr(y), ldy or adapters.rows, _ptr(ws), ws_bytes, _stream(stream)))
+
+    def add_rms_quant(self, ty, x, res, w, h, o, xq, xd, xs, m, n, eps, ldx=None, ldr=None, ldh=None, ldo=None, stream=None):
+        """h = x + res, its RMS norm o and that in int8 (xq, xd, xs as le_quant_x gives them), for m rows of n values of type ty; res, h, o,
+        xs, or xq and xd together, may be None."""
+        self._check(self._L.le_add_rms_quant(self._ctx, ty, _ptr(x), ldx or n, _ptr(res), ldr or n, _ptr(w), _ptr(h), ldh or n, _ptr(o),
+                                             ldo or n, _ptr(xq), _ptr(xd), _ptr(xs), m, n, float(eps), _stream(stream)))
 
     def moe_check(self, ws, stream=None):
         """Raise LeError(-8) if a one-launch MoE layer on workspace ws gave up at its device-wide
