@@ -395,7 +395,7 @@ typedef struct le_adapters {
  * of type xtype, x's rows of cols values ldx apart (0: one row for all), base's and y's of `rows` values ldb and ldy apart. Products
  * with A are exact and summed in fp32, A_i x[t] and its product with scale_i are held in fp32, and so are the sums over the rank and with base; the
  * result is rounded once. Tokens of one adapter need not follow one another, but for many tokens runs of 16 and more are faster.
- * Limits: rank <= 256, rows and cols <= 2^24, m <= 2^20, n_ad >= 1; m may be 0. y may not overlap other inputs, nor base otherwise.
+ * Limits: rank <= 256, rows and cols <= 2^24, m <= 1048560, n_ad >= 1; m may be 0. y may not overlap other inputs, nor base otherwise.
  * ws: le_lora_workspace_size bytes, 16-byte aligned, which every call writes anew; calls that may overlap need workspaces of
  * their own. */
 size_t le_lora_workspace_size(const le_adapters *ad, int xtype, int m);

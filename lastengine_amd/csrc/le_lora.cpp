@@ -8,20 +8,35 @@
 
 namespace {
 
-constexpr int kRank = 256, kSide = 1 << 24, kTokens = 1 << 20;
+constexpr int kRank = 256, kSide = 1 << 24, kTokens = 16 * 65535;
 
 const char *shape_error(const le_adapters *ad, int m) {
     if (ad->n_ad <= 0 || ad->rank <= 0 || ad->rank > kRank) return "n_ad below 1 or rank outside 1..256";
     if (ad->rows <= 0 || ad->cols <= 0 || ad->rows > kSide || ad->cols > kSide) return "rows or cols outside 1..2^24";
-    if (m < 0 || m > kTokens) return "m outside 0..2^20";
+    if (m < 0 || m > kTokens) return "m outside 0..1048560";
     return nullptr;
 }
+
+/* How a call is cut up. */
+struct Shape {
+    int tiles, turns, segs, steps;
+    Shape(const le_adapters *ad, int m) {
+        tiles = (m + 15) / 16;
+        /* blocks that share a tile's adapters: one each while there are few tiles */
+        turns = std::min(std::min(m, 16), std::max(1, 1024 / tiles));
+        /* segments of the columns: about 1024 blocks in all, each at least a step for its four waves */
+        const int all = (ad->cols + 31) / 32, want = std::max(1, 1024 / (tiles * turns));
+        segs = std::max(1, std::min(std::min(want, 16), all / 4));
+        steps = (all + segs - 1) / segs;
+        segs = (all + steps - 1) / steps;
+    }
+};
 
 }  // namespace
 
 extern "C" size_t le_lora_workspace_size(const le_adapters *ad, int xtype, int m) {
     if (!ad || !le_type_bytes(xtype) || !le_type_bytes(ad->ltype) || shape_error(ad, m)) return 0;
-    return (size_t)m * ad->rank * 4;
+    return m ? (size_t)Shape(ad, m).segs * m * ad->rank * 4 : 0;
 }
 
 extern "C" int le_lora(le_ctx *c, const le_adapters *ad, const int *idx, int xtype, const void *x, long long ldx, int m,
@@ -44,12 +59,15 @@ extern "C" int le_lora(le_ctx *c, const le_adapters *ad, const int *idx, int xty
     const size_t need = le_lora_workspace_size(ad, xtype, m);
     if (!ws || ws_bytes < need) return le_ctx_failf(c, LE_ERR_WORKSPACE, "workspace needs %zu bytes", need);
     if (int rc = le_ctx_on_device(c)) return rc;
-    LoraArgs a{ad->a, ad->b, ad->scale, idx, x, base, y, (float *)ws, ldx, ldb, ldy, ad->n_ad, ad->rank, ad->rows, ad->cols, m};
+    const Shape sh(ad, m);
+    LoraArgs a{ad->a, ad->b, ad->scale, idx, x, base, y, (float *)ws, ldx, ldb, ldy, ad->n_ad, ad->rank, ad->rows, ad->cols, m, sh.segs, sh.steps};
     void *args[] = {&a};
     char name[40];
-    snprintf(name, sizeof name, "le_lo_down_%d_%d", xtype, ad->ltype);
-    const long long waves = (long long)m * ad->rank;
-    if (int rc = le_ctx_launch(c, name, dim3((unsigned)std::min((waves + 3) / 4, 1LL << 20)), 256, 0, (hipStream_t)stream, args)) return rc;
-    snprintf(name, sizeof name, "le_lo_up_%d_%d", xtype, ad->ltype);
-    return le_ctx_launch(c, name, dim3((unsigned)((ad->rows + 255) / 256), (unsigned)std::min(m, 65535)), 256, 0, (hipStream_t)stream, args);
+    snprintf(name, sizeof name, "le_lo_down%d_%d_%d", ad->rank <= 16 ? 1 : ad->rank <= 32 ? 2 : 4, xtype, ad->ltype);
+    if (int rc = le_ctx_launch(c, name, dim3((unsigned)sh.tiles, (unsigned)sh.turns, (unsigned)sh.segs), 256, 0, (hipStream_t)stream, args)) return rc;
+    const unsigned blocks = (unsigned)((ad->rows + 255) / 256);
+    const bool few = m <= 64;
+    snprintf(name, sizeof name, "le_lo_%s_%d_%d", few ? "upv" : "upm", xtype, ad->ltype);
+    return le_ctx_launch(c, name, dim3(blocks, (unsigned)sh.tiles, few ? (unsigned)sh.turns : 1u), 256, few ? (size_t)16 * ((ad->rank + 7) & ~7) * 4 : 0,
+                         (hipStream_t)stream, args);
 }

@@ -7,7 +7,8 @@ struct LoraArgs {
     const int *idx;
     const void *x, *base; /* base null: 0 */
     void *y;
-    float *u;             /* [token][rank]: scale * A x */
+    float *u;             /* [segment][token][rank]: A x over a segment of the columns */
     long long ldx, ldb, ldy;
     int n_ad, rank, rows, cols, m;
+    int segs, steps;      /* segments of cols, and the 32-column steps of each */
 };

@@ -121,7 +121,7 @@ def test_without_rows(call, ctx):
 
 @pytest.mark.parametrize("bad,code", [
     (dict(ad=False), -1), (dict(xtype=8), -2), (dict(ltype=12), -2), (dict(n_ad=0), -3), (dict(rank=0), -3), (dict(rank=257), -3), (dict(rows=0), -3), (dict(cols=-1), -3),
-    (dict(rows=2**24 + 1, ldb=2**25, ldy=2**25), -3), (dict(cols=2**24 + 1, ldx=2**25), -3), (dict(m=-1), -3), (dict(m=2**20 + 1), -3), (dict(ldx=63), -3),
+    (dict(rows=2**24 + 1, ldb=2**25, ldy=2**25), -3), (dict(cols=2**24 + 1, ldx=2**25), -3), (dict(m=-1), -3), (dict(m=1048561), -3), (dict(ldx=63), -3),
     (dict(ldx=-64), -3), (dict(ldb=31), -3), (dict(ldy=31), -3), (dict(a=None), -1), (dict(b=None), -1), (dict(idx=None), -1), (dict(x=None), -1), (dict(y=None), -1),
     (dict(a=A + 1), -4), (dict(b=A + 1), -4), (dict(ltype=0, a=A + 2), -4), (dict(scale=A + 2), -4), (dict(idx=A + 1), -4), (dict(x=A + 2), -4), (dict(base=A + 2), -4),
     (dict(y=A + 2), -4), (dict(ws=A + 8), -4), (dict(ws=None), -7), (dict(ws_bytes=5 * 16 * 4 - 1), -7), (dict(base=A, y=A, ldb=40), -1)])
@@ -131,7 +131,7 @@ def test_lora_refusals(call, ctx, bad, code):
 
 
 @pytest.mark.parametrize("good", [
-    dict(), dict(base=None, ldb=0), dict(scale=None), dict(ldx=0), dict(rank=1), dict(rank=256), dict(m=1), dict(m=2**20), dict(rows=1, cols=1), dict(y=2 * A, ldy=50),
+    dict(), dict(base=None, ldb=0), dict(scale=None), dict(ldx=0), dict(rank=1), dict(rank=256), dict(m=1), dict(m=1048560), dict(rows=1, cols=1), dict(y=2 * A, ldy=50),
     dict(rows=2**24, ldb=2**24, ldy=2**24), dict(cols=2**24, ldx=2**24), dict(n_ad=100000), dict(xtype=30, ltype=30, x=A + 2, a=A + 2, b=A + 2)])
 def test_lora_launches(call, ctx, good):
     assert call.lora(**good) == 0, ctx.err
