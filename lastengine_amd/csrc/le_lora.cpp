@@ -19,24 +19,29 @@ const char *shape_error(const le_adapters *ad, int m) {
 
 /* How a call is cut up. */
 struct Shape {
-    int tiles, turns, segs, steps;
-    Shape(const le_adapters *ad, int m) {
+    int tiles, turns, sets, waves, segs, steps;
+    size_t wave_lds;
+    Shape(const le_adapters *ad, int xtype, int m) {
         tiles = (m + 15) / 16;
         /* blocks that share a tile's adapters: one each while there are few tiles */
-        turns = std::min(std::min(m, 16), std::max(1, 1024 / tiles));
-        /* segments of the columns: about 1024 blocks in all, each at least a step for its four waves */
-        const int all = (ad->cols + 31) / 32, want = std::max(1, 1024 / (tiles * turns));
-        segs = std::max(1, std::min(std::min(want, 16), all / 4));
+        turns = m <= 64 ? std::min(m, 16) : 1;
+        sets = ad->rank <= 16 ? 1 : ad->rank <= 32 ? 2 : 4; /* of 16 rows of A at once */
+        /* the columns' steps of 64 over a block's waves (as many as leave LDS for two blocks), and over segments while that makes no more than 2048 waves */
+        const int all = (ad->cols + 63) / 64;
+        wave_lds = le_type_bytes(xtype) * 1024 + 256 + sets * (le_type_bytes(ad->ltype) * 1024 + 256);
+        waves = std::min(std::min(8, (int)(80 * 1024 / wave_lds)), all);
+        segs = std::max(1, std::min(std::min(8, 2048 / (tiles * std::min(m, 16) * waves)), all / waves));
         steps = (all + segs - 1) / segs;
         segs = (all + steps - 1) / steps;
     }
+    size_t workspace(const le_adapters *ad) const { return (size_t)segs * tiles * ((ad->rank + 31) / 32) * 2048; }
 };
 
 }  // namespace
 
 extern "C" size_t le_lora_workspace_size(const le_adapters *ad, int xtype, int m) {
     if (!ad || !le_type_bytes(xtype) || !le_type_bytes(ad->ltype) || shape_error(ad, m)) return 0;
-    return m ? (size_t)Shape(ad, m).segs * m * ad->rank * 4 : 0;
+    return m ? Shape(ad, xtype, m).workspace(ad) : 0;
 }
 
 extern "C" int le_lora(le_ctx *c, const le_adapters *ad, const int *idx, int xtype, const void *x, long long ldx, int m,
@@ -59,15 +64,21 @@ extern "C" int le_lora(le_ctx *c, const le_adapters *ad, const int *idx, int xty
     const size_t need = le_lora_workspace_size(ad, xtype, m);
     if (!ws || ws_bytes < need) return le_ctx_failf(c, LE_ERR_WORKSPACE, "workspace needs %zu bytes", need);
     if (int rc = le_ctx_on_device(c)) return rc;
-    const Shape sh(ad, m);
+    const Shape sh(ad, xtype, m);
     LoraArgs a{ad->a, ad->b, ad->scale, idx, x, base, y, (float *)ws, ldx, ldb, ldy, ad->n_ad, ad->rank, ad->rows, ad->cols, m, sh.segs, sh.steps};
     void *args[] = {&a};
     char name[40];
-    snprintf(name, sizeof name, "le_lo_down%d_%d_%d", ad->rank <= 16 ? 1 : ad->rank <= 32 ? 2 : 4, xtype, ad->ltype);
-    if (int rc = le_ctx_launch(c, name, dim3((unsigned)sh.tiles, (unsigned)sh.turns, (unsigned)sh.segs), 256, 0, (hipStream_t)stream, args)) return rc;
-    const unsigned blocks = (unsigned)((ad->rows + 255) / 256);
-    const bool few = m <= 64;
-    snprintf(name, sizeof name, "le_lo_%s_%d_%d", few ? "upv" : "upm", xtype, ad->ltype);
-    return le_ctx_launch(c, name, dim3(blocks, (unsigned)sh.tiles, few ? (unsigned)sh.turns : 1u), 256, few ? (size_t)16 * ((ad->rank + 7) & ~7) * 4 : 0,
-                         (hipStream_t)stream, args);
+    snprintf(name, sizeof name, "le_lo_down%d_%d_%d", sh.sets, xtype, ad->ltype);
+    if (int rc = le_ctx_launch(c, name, dim3((unsigned)sh.tiles, (unsigned)sh.turns, (unsigned)sh.segs), 64 * sh.waves,
+                               sh.waves * std::max(sh.wave_lds, (size_t)sh.sets * 1024), (hipStream_t)stream, args))
+        return rc;
+    if (m <= 64) {
+        /* four rows a lane where that leaves 1024 blocks */
+        const int R = (ad->rows + 1023LL) / 1024 * sh.tiles * sh.turns >= 1024 ? 4 : 1;
+        snprintf(name, sizeof name, "le_lo_upv%d_%d_%d", R, xtype, ad->ltype);
+        return le_ctx_launch(c, name, dim3((unsigned)((ad->rows + 256 * R - 1) / (256 * R)), (unsigned)sh.tiles, (unsigned)sh.turns), 256,
+                             (size_t)4 * ((ad->rank + 7) & ~7) * 4, (hipStream_t)stream, args);
+    }
+    snprintf(name, sizeof name, "le_lo_upm%d_%d_%d", ad->rank <= 32 ? 1 : ad->rank <= 64 ? 2 : 0, xtype, ad->ltype);
+    return le_ctx_launch(c, name, dim3((unsigned)((ad->rows + 255) / 256), (unsigned)((sh.tiles + 3) / 4)), 256, 0, (hipStream_t)stream, args);
 }

@@ -73,38 +73,74 @@ template <int TY> __device__ __forceinline__ unsigned pack(const float *v, int d
     else return XT<TY>::down(v[2 * d]) | (unsigned)XT<TY>::down(v[2 * d + 1]) << 16;
 }
 
-/* c += P Q^T over 32 of k: 16 rows of each, a lane's row l % 16 and its eight k from 8 (l / 16) on. Two operands of one 16-bit type
- * multiply as they are, others in fp32: either way the products are exact (fp32: a fused multiply-add's) and the sums fp32. */
-template <int P, int Q> __device__ __forceinline__ v4f multiply(const Eight<P> &p, const Eight<Q> &q, v4f c) {
-    if constexpr (P == 1 && Q == 1) {
-        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, p.v), __builtin_bit_cast(v8h, q.v), c, 0, 0, 0);
-    } else if constexpr (P == 30 && Q == 30) {
-        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8b, p.v), __builtin_bit_cast(v8b, q.v), c, 0, 0, 0);
+/* ---- products ----
+ * An operand of a matrix instruction over 32 of k: 16 rows, a lane's row l % 16 and its eight k from 8 (l / 16) on. Two operands of one 16-bit
+ * type multiply as they are. Otherwise values are cut into bf16 pieces that add up to them exactly (fp16: 2 of 8 bits or less, fp32: 3 of 8,
+ * cut off, not rounded) and every piece of one multiplies every piece of the other: five to two times faster than fp32 instructions, which are left for two
+ * fp32 operands. Either way the products are exact (fp32: a fused multiply-add's) and the sums fp32. */
+template <int TY, bool CUT> struct Operand;
+template <int TY> struct Operand<TY, false> {
+    Eight<TY> p[1];
+    static constexpr int N = 1;
+    __device__ __forceinline__ void set(const Eight<TY> &e) { p[0] = e; }
+};
+template <int TY> struct Operand<TY, true> {
+    static constexpr int N = TY == 0 ? 3 : 2;
+    v4u p[N];
+    __device__ __forceinline__ void set(const Eight<TY> &e) {
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = e.up(i);
+#pragma unroll
+        for (int n = 0; n < N; n++)
+#pragma unroll
+            for (int d = 0; d < 4; d++) {
+                const unsigned lo = __builtin_bit_cast(unsigned, v[2 * d]), hi = __builtin_bit_cast(unsigned, v[2 * d + 1]);
+                p[n][d] = __builtin_amdgcn_perm(hi, lo, 0x07060302);
+                if (n + 1 < N) {
+                    v[2 * d] -= __builtin_bit_cast(float, lo & 0xFFFF0000u);
+                    v[2 * d + 1] -= __builtin_bit_cast(float, hi & 0xFFFF0000u);
+                }
+            }
+    }
+};
+/* The first operand's form and the second's, for types P and Q. */
+template <int P, int Q> struct Pair {
+    static constexpr bool same = P == Q;
+    using A = Operand<P, !same && P != 30>;
+    using B = Operand<Q, !same && Q != 30>;
+};
+__device__ __forceinline__ v4u raw(const v4u &v) { return v; }
+template <int TY> __device__ __forceinline__ v4u raw(const Eight<TY> &v) { return v.v; }
+template <int P, int Q> __device__ __forceinline__ v4f multiply(const typename Pair<P, Q>::A &a, const typename Pair<P, Q>::B &b, v4f c) {
+    if constexpr (P == 0 && Q == 0) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.p[0].v[i], b.p[0].v[i], c, 0, 0, 0);
+    } else if constexpr (P == 1 && Q == 1) {
+        c = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, a.p[0].v), __builtin_bit_cast(v8h, b.p[0].v), c, 0, 0, 0);
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; i++) c = __builtin_amdgcn_mfma_f32_16x16x4f32(p.up(i), q.up(i), c, 0, 0, 0);
-        return c;
+        for (int i = 0; i < Pair<P, Q>::A::N; i++)
+#pragma unroll
+            for (int j = 0; j < Pair<P, Q>::B::N; j++)
+                c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8b, raw(a.p[i])), __builtin_bit_cast(v8b, raw(b.p[j])), c, 0, 0, 0);
     }
+    return c;
 }
-
-template <int N> struct Count { static constexpr int value = N; };
 
 /* ---- the adapters of a tile ---- */
 
+/* Adapter of token t; -1: none, or no token */
+__device__ __forceinline__ int adapter(const LoraArgs &a, int t) {
+    const int id = t < a.m ? ((const LE_GLOBAL int *)a.idx)[t] : -1;
+    return id < a.n_ad && id >= 0 ? id : -1;
+}
 struct Tile {
-    int t0;       /* first of its 16 tokens */
-    int id;       /* adapter of this lane's token t0 + l % 16; -1: none, or no token */
-    unsigned left; /* tokens whose adapter has not come yet */
+    int id;           /* adapter of this lane's token, its lane % 16th of the tile */
+    unsigned left;    /* tokens whose adapter has not come yet */
     int cur;
     unsigned members; /* tokens of adapter cur */
-    __device__ __forceinline__ Tile(const LoraArgs &a, int tile) {
-        const int l = threadIdx.x & 63;
-        t0 = tile * 16;
-        const int t = t0 + (l & 15);
-        id = t < a.m ? ((const LE_GLOBAL int *)a.idx)[t] : -1;
-        if (id >= a.n_ad || id < 0) id = -1;
-        left = (unsigned)__ballot(id >= 0) & 0xFFFF;
-    }
+    __device__ __forceinline__ Tile(int id) : id(id), left((unsigned)__ballot(id >= 0) & 0xFFFF) {}
     __device__ __forceinline__ bool next() {
         if (!left) return false;
         cur = __builtin_amdgcn_readlane(id, __ffs((int)left) - 1);
@@ -114,66 +150,131 @@ struct Tile {
     }
 };
 
+/* Where u of token i of a tile has rank j: in the order of a matrix instruction's operand (32 ranks of 16 tokens, two pieces of 16 bytes a lane), so
+ * that a wave reads whole lines; ranks are filled up with zeros to a multiple of 32. */
+__device__ __forceinline__ long long place(const LoraArgs &a, int seg, int tile, int i, int j) {
+    const int jb = (a.rank + 31) >> 5, lane = i + 16 * (j >> 3 & 3);
+    return ((((long long)seg * ((a.m + 15) >> 4) + tile) * jb + (j >> 5)) * 2 + (j >> 2 & 1)) * 256 + lane * 4 + (j & 3);
+}
+
 /* ---- down: u = A x ----
- * A block takes a tile, an adapter of it and a segment of the columns, its four waves 32 columns in turn; their sums meet in LDS. Rows of A
- * as the other operand, RF times 16 of them at once. Operands come straight from memory in the matrix instruction's layout, 64 (fp32:
- * 128) bytes in a row of each. */
+ * A block takes a tile, an adapter of it and a segment of the columns, its waves 64 columns in turn; their sums meet in LDS. Rows of A
+ * as the other operand, RF times 16 of them at once. A wave reads 128 (fp32: 256) bytes of a row at a time, in whole lines, and turns them to
+ * the matrix instruction's layout through LDS of its own (read in that layout from memory, 16 bytes in each of 16 rows side by side, the same
+ * kernel took twice the time), the next step's on their way meanwhile. */
+template <int TY> struct Rows { /* 16 rows of 64 values */
+    static constexpr int V = TY == 0 ? 4 : 8, LANES = 64 / V, N = 16 * LANES / 64, PITCH = 64 * (16 / V) + 16;
+    static constexpr int BYTES = 16 * PITCH;
+    v4u r[N];
+    __device__ __forceinline__ void load(const void *base, const long long *row, int k, bool whole, int cols) {
+        using T = typename XT<TY>::raw;
+        const int l = threadIdx.x & 63, at = k + l % LANES * V;
+#pragma unroll
+        for (int n = 0; n < N; n++) {
+            const LE_GLOBAL T *p = (const LE_GLOBAL T *)base + row[n] + at;
+            if (whole || at + V <= cols) {
+                r[n] = *(const LE_GLOBAL typename Any<sizeof(T)>::v *)p;
+            } else {
+                r[n] = v4u{0, 0, 0, 0};
+#pragma unroll
+                for (int e = 0; e < V; e++)
+                    if (at + e < cols) {
+                        const typename XT<TY>::raw v = p[e];
+                        if constexpr (V == 4) r[n][e] = __builtin_bit_cast(unsigned, v);
+                        else r[n][e >> 1] |= (unsigned)v << (e & 1) * 16;
+                    }
+            }
+        }
+    }
+    __device__ __forceinline__ void store(char *lds) const {
+        const int l = threadIdx.x & 63;
+#pragma unroll
+        for (int n = 0; n < N; n++) *(v4u *)(lds + (n * (64 / LANES) + l / LANES) * PITCH + l % LANES * 16) = r[n];
+    }
+    static __device__ __forceinline__ int row_of(int n) { return n * (64 / LANES) + (threadIdx.x & 63) / LANES; }
+    static __device__ __forceinline__ Eight<TY> read(const char *lds, int half) {
+        const int l = threadIdx.x & 63;
+        const char *p = lds + (l & 15) * PITCH + (32 * half + 8 * (l >> 4)) * (16 / V);
+        Eight<TY> e;
+        if constexpr (TY == 0) {
+            *(v4f *)&e.v[0] = *(const v4f *)p;
+            *(v4f *)&e.v[4] = *(const v4f *)(p + 16);
+        } else {
+            e.v = *(const v4u *)p;
+        }
+        return e;
+    }
+};
 template <int WTY, int RF> __device__ __forceinline__ void down_body(const LoraArgs &a) {
-    __shared__ float part[4][RF][256];
-    const int l = threadIdx.x & 63, wave = threadIdx.x >> 6, kl = (l >> 4) * 8;
-    Tile t(a, blockIdx.x);
-    const int s0 = blockIdx.z * a.steps, s1 = min(s0 + a.steps, (a.cols + 31) / 32), whole = min(s1, a.cols / 32);
-    const long long xrow = min(t.t0 + (l & 15), a.m - 1) * a.ldx;
+    using Mul = Pair<XTY, WTY>;
+    using XR = Rows<XTY>;
+    using WR = Rows<WTY>;
+    extern __shared__ __attribute__((aligned(16))) char lds[]; /* each wave's rows, then its sums: [wave][RF][256] */
+    const int l = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), nw = blockDim.x >> 6, t0 = blockIdx.x * 16;
+    char *mine = lds + wave * (XR::BYTES + RF * WR::BYTES);
+    Tile t(adapter(a, t0 + (l & 15)));
+    const int s0 = blockIdx.z * a.steps + wave, s1 = min((int)(blockIdx.z + 1) * a.steps, (a.cols + 63) / 64);
+    long long xrow[XR::N];
+#pragma unroll
+    for (int n = 0; n < XR::N; n++) xrow[n] = min(t0 + XR::row_of(n), a.m - 1) * a.ldx;
     for (int nth = 0; t.next(); nth++) {
         if (nth % gridDim.y != blockIdx.y) continue;
         for (int j0 = 0; j0 < a.rank; j0 += 16 * RF) {
             v4f c[RF];
-            long long arow[RF];
+            long long arow[RF][WR::N];
 #pragma unroll
             for (int f = 0; f < RF; f++) {
                 c[f] = v4f{0.f, 0.f, 0.f, 0.f};
-                arow[f] = ((long long)t.cur * a.rank + min(j0 + 16 * f + (l & 15), a.rank - 1)) * a.cols;
+#pragma unroll
+                for (int n = 0; n < WR::N; n++) arow[f][n] = ((long long)t.cur * a.rank + min(j0 + 16 * f + WR::row_of(n), a.rank - 1)) * a.cols;
             }
-            int s = s0 + wave;
-            auto some = [&](auto count) { /* so many of the wave's steps, their loads ahead of their products */
-                constexpr int U = decltype(count)::value;
-                Eight<XTY> x[U];
-                Eight<WTY> w[U][RF];
+            XR x;
+            WR w[RF];
+            auto load = [&](int s) {
+                const bool whole = 64 * s + 64 <= a.cols;
+                x.load(a.x, xrow, 64 * s, whole, a.cols);
 #pragma unroll
-                for (int i = 0; i < U; i++) {
-                    const int k = 32 * (s + 4 * i) + kl;
-                    x[i] = load8<XTY>(a.x, xrow + k, 8);
-#pragma unroll
-                    for (int f = 0; f < RF; f++) w[i][f] = load8<WTY>(a.a, arow[f] + k, 8);
-                }
-#pragma unroll
-                for (int i = 0; i < U; i++)
-#pragma unroll
-                    for (int f = 0; f < RF; f++) c[f] = multiply<XTY, WTY>(x[i], w[i][f], c[f]);
-                s += 4 * U;
+                for (int f = 0; f < RF; f++) w[f].load(a.a, arow[f], 64 * s, whole, a.cols);
             };
-            constexpr int U = RF == 4 ? 2 : 4;
-            while (s + 4 * (U - 1) < whole) some(Count<U>());
-            while (s < whole) some(Count<1>());
-            if (s < s1) { /* the row's end */
-                const int k = 32 * s + kl, n = a.cols - k;
-                const Eight<XTY> x = load8<XTY>(a.x, xrow + k, n);
+            if (s0 < s1) load(s0);
+            for (int s = s0; s < s1; s += nw) {
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); /* the reads of the step before */
+                __builtin_amdgcn_wave_barrier();
+                x.store(mine);
 #pragma unroll
-                for (int f = 0; f < RF; f++) c[f] = multiply<XTY, WTY>(x, load8<WTY>(a.a, arow[f] + k, n), c[f]);
+                for (int f = 0; f < RF; f++) w[f].store(mine + XR::BYTES + f * WR::BYTES);
+                if (s + nw < s1) load(s + nw);
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                __builtin_amdgcn_wave_barrier();
+#pragma unroll
+                for (int half = 0; half < 2; half++) {
+                    typename Mul::A p;
+                    p.set(XR::read(mine, half));
+#pragma unroll
+                    for (int f = 0; f < RF; f++) {
+                        typename Mul::B q;
+                        q.set(WR::read(mine + XR::BYTES + f * WR::BYTES, half));
+                        c[f] = multiply<XTY, WTY>(p, q, c[f]);
+                    }
+                }
             }
+            float *sums = (float *)lds;
             __syncthreads();
 #pragma unroll
             for (int f = 0; f < RF; f++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) part[wave][f][((l >> 4) * 4 + i) * 16 + (l & 15)] = c[f][i];
+                for (int e = 0; e < 4; e++) sums[(wave * RF + f) * 256 + ((l >> 4) * 4 + e) * 16 + (l & 15)] = c[f][e];
             __syncthreads();
-            const int row = threadIdx.x >> 4;
-#pragma unroll
-            for (int f = 0; f < RF; f++) {
-                const int j = j0 + 16 * f + (threadIdx.x & 15);
-                const float v = (part[0][f][threadIdx.x] + part[1][f][threadIdx.x]) + (part[2][f][threadIdx.x] + part[3][f][threadIdx.x]);
-                if (j < a.rank && (t.members >> row & 1)) ((LE_GLOBAL float *)a.u)[((long long)blockIdx.z * a.m + t.t0 + row) * a.rank + j] = v;
+            for (int id = threadIdx.x; id < 256 * RF; id += blockDim.x) {
+                const int row = id >> 4 & 15, j = j0 + (id >> 8) * 16 + (id & 15);
+                if (j < ((a.rank + 31) & ~31) && (t.members >> row & 1)) {
+                    float v = sums[id];
+                    for (int n = 1; n < nw; n++) v += sums[n * RF * 256 + id];
+                    ((LE_GLOBAL float *)a.u)[place(a, blockIdx.z, blockIdx.x, row, j)] = j < a.rank ? v : 0.f;
+                    if (RF == 1) ((LE_GLOBAL float *)a.u)[place(a, blockIdx.z, blockIdx.x, row, j + 16)] = 0.f; /* rank <= 16 here */
+                }
             }
+            __syncthreads();
         }
     }
 }
@@ -181,128 +282,202 @@ template <int WTY, int RF> __device__ __forceinline__ void down_body(const LoraA
 __device__ __forceinline__ float factor(const LoraArgs &a, int ad) { return a.scale ? ((const LE_GLOBAL float *)a.scale)[ad] : 1.f; }
 
 /* ---- up, few tokens ----
- * A lane an output row, whose rank values of B it reads once for all tokens of the adapter; u in LDS. */
-template <int WTY> __device__ __forceinline__ void upv_body(const LoraArgs &a) {
-    extern __shared__ float lu[]; /* [token][rank, rounded up to 8] */
-    const int rp = (a.rank + 7) & ~7, r = blockIdx.x * 256 + threadIdx.x, rc = min(r, a.rows - 1);
-    Tile t(a, blockIdx.y);
+ * A lane R output rows; their first 16 values of B are read once for all tokens of the adapter (on their way while u comes to LDS), which are
+ * taken four at a time. */
+template <int WTY, int R> __device__ __forceinline__ void upv_body(const LoraArgs &a) {
+    extern __shared__ float lu[]; /* [4 tokens][rank, rounded up to 8] */
+    const int rp = (a.rank + 7) & ~7, t0 = blockIdx.y * 16, r0 = blockIdx.x * (256 * R) + threadIdx.x;
+    Tile t(adapter(a, t0 + (threadIdx.x & 15)));
     const LE_GLOBAL X *base = (const LE_GLOBAL X *)a.base;
-    if (blockIdx.z == 0 && r < a.rows) { /* tokens of no adapter */
+    if (blockIdx.z == 0) { /* tokens of no adapter */
         for (unsigned none = ~t.left & 0xFFFF; none; none &= none - 1) {
-            const int k = t.t0 + __ffs((int)none) - 1;
+            const int k = t0 + __ffs((int)none) - 1;
             if (k >= a.m) break;
-            ((LE_GLOBAL X *)a.y)[k * a.ldy + r] = a.base ? base[k * a.ldb + r] : X(0);
+#pragma unroll
+            for (int q = 0; q < R; q++)
+                if (r0 + 256 * q < a.rows) ((LE_GLOBAL X *)a.y)[k * a.ldy + r0 + 256 * q] = a.base ? base[k * a.ldb + r0 + 256 * q] : X(0);
         }
     }
     for (int nth = 0; t.next(); nth++) {
         if (nth % gridDim.z != blockIdx.z) continue;
-        float b[16];
+        long long row[R];
+        Eight<WTY> w[R][2];
 #pragma unroll
-        for (int i = 0; i < 16; i++) b[i] = (t.members >> i & 1) && a.base ? XT<XTY>::up(base[(t.t0 + i) * a.ldb + rc]) : 0.f;
+        for (int q = 0; q < R; q++) {
+            row[q] = ((long long)t.cur * a.rows + min(r0 + 256 * q, a.rows - 1)) * a.rank;
+            w[q][0] = load8<WTY>(a.b, row[q], a.rank);
+            w[q][1] = load8<WTY>(a.b, row[q] + 8, a.rank - 8);
+        }
         const float f = factor(a, t.cur);
-        __syncthreads();
-        for (int id = threadIdx.x; id < 16 * rp; id += 256) {
-            const int i = id / rp, j = id - i * rp;
-            float v = 0.f;
-            if ((t.members >> i & 1) && j < a.rank)
-                for (int s = 0; s < a.segs; s++) v += ((const LE_GLOBAL float *)a.u)[((long long)s * a.m + t.t0 + i) * a.rank + j];
-            lu[id] = f * v;
-        }
-        __syncthreads();
-        float acc[16];
+        for (unsigned todo = t.members; todo;) {
+            int k[4]; /* tokens; the last one again where fewer are left */
 #pragma unroll
-        for (int i = 0; i < 16; i++) acc[i] = 0.f;
-        const long long row = ((long long)t.cur * a.rows + rc) * a.rank;
-        for (int j = 0; j < a.rank; j += 8) {
-            const Eight<WTY> w = load8<WTY>(a.b, row + j, a.rank - j);
+            for (int i = 0; i < 4; i++) {
+                k[i] = todo ? t0 + __ffs((int)todo) - 1 : k[i > 0 ? i - 1 : 0];
+                todo &= todo - 1;
+            }
+            float b[4][R], acc[4][R];
 #pragma unroll
-            for (int i = 0; i < 16; i++)
-                if (t.members >> i & 1) {
-                    const float *u = lu + i * rp + j;
+            for (int i = 0; i < 4; i++)
 #pragma unroll
-                    for (int k = 0; k < 8; k++) acc[i] = fmaf(w.up(k), u[k], acc[i]);
+                for (int q = 0; q < R; q++) {
+                    b[i][q] = 0.f;
+                    if (a.base && (i == 0 || k[i] != k[i - 1])) b[i][q] = XT<XTY>::up(base[k[i] * a.ldb + min(r0 + 256 * q, a.rows - 1)]);
+                    acc[i][q] = 0.f;
                 }
-        }
-        if (r < a.rows) {
+            __syncthreads();
+            for (int id = threadIdx.x; id < 4 * rp; id += 256) {
+                const int i = id / rp, j = id - i * rp;
+                const LE_GLOBAL float *u = (const LE_GLOBAL float *)a.u + place(a, 0, blockIdx.y, (i == 0 ? k[0] : i == 1 ? k[1] : i == 2 ? k[2] : k[3]) - t0, j);
+                const long long seg = place(a, 1, 0, 0, 0);
+                float v = 0.f;
+#pragma unroll 8
+                for (int s = 0; s < a.segs; s++) v += u[s * seg];
+                lu[id] = f * v;
+            }
+            __syncthreads();
+            auto eight = [&](const Eight<WTY> &v, int q, int j) {
 #pragma unroll
-            for (int i = 0; i < 16; i++)
-                if (t.members >> i & 1) ((LE_GLOBAL X *)a.y)[(t.t0 + i) * a.ldy + r] = XT<XTY>::down(b[i] + acc[i]);
+                for (int i = 0; i < 4; i++)
+                    if (i == 0 || k[i] != k[i - 1]) {
+#pragma unroll
+                        for (int e = 0; e < 8; e++) acc[i][q] = fmaf(v.up(e), lu[i * rp + j + e], acc[i][q]);
+                    }
+            };
+#pragma unroll
+            for (int q = 0; q < R; q++) {
+                eight(w[q][0], q, 0);
+                if (a.rank > 8) eight(w[q][1], q, 8);
+            }
+            for (int j = 16; j < a.rank; j += 8) {
+                Eight<WTY> v[R];
+#pragma unroll
+                for (int q = 0; q < R; q++) v[q] = load8<WTY>(a.b, row[q] + j, a.rank - j);
+#pragma unroll
+                for (int q = 0; q < R; q++) eight(v[q], q, j);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int q = 0; q < R; q++)
+                    if ((i == 0 || k[i] != k[i - 1]) && r0 + 256 * q < a.rows)
+                        ((LE_GLOBAL X *)a.y)[k[i] * a.ldy + r0 + 256 * q] = XT<XTY>::down(b[i][q] + acc[i][q]);
         }
     }
 }
 
 /* ---- up, many tokens ----
- * A wave 64 output rows by 16 tokens. Of the 16 x 16 results of a matrix instruction a lane has four rows of its token; which rows of B are
- * its operand is free, and they are dealt so that four instructions leave 16 consecutive outputs in a lane. */
-template <int WTY> __device__ __forceinline__ void upm_body(const LoraArgs &a) {
+ * A wave 64 output rows by up to 64 tokens, 16 at a time. A matrix instruction leaves four rows of 16 tokens in a lane; they change places through LDS, so
+ * that base is read and y written in whole rows of 64 (128 or 256 bytes). B stays in registers while the adapter does, up to a rank of
+ * 32 J (J = 0: read for each tile). */
+template <int WTY, int J> __device__ __forceinline__ void upm_body(const LoraArgs &a) {
+    using v4u_any = Any<sizeof(X)>::v;
+    using Mul = Pair<WTY, 0>;
+    constexpr int E = 16 / sizeof(X), LANES = 64 / E, PIECES = 16 / E; /* values of a piece, lanes of a row of 64, pieces of a lane */
+    constexpr int PITCH = 68;
+    __shared__ __attribute__((aligned(16))) float turn[4][16 * PITCH];
+    float *mine = turn[threadIdx.x >> 6];
     const int l = threadIdx.x & 63, g = l >> 4, c16 = l & 15, r0 = (blockIdx.x * 4 + (threadIdx.x >> 6)) * 64;
     if (r0 >= a.rows) return;
-    Tile t(a, blockIdx.y);
-    const int tok = t.t0 + c16, tc = min(tok, a.m - 1), mine = r0 + 16 * g;
-    using v4u_any = Any<sizeof(X)>::v;
-    constexpr int PIECES = sizeof(X), E = 16 / sizeof(X); /* 16-byte pieces of 16 outputs, values of each */
-    float out[16];
-    const LE_GLOBAL X *base = (const LE_GLOBAL X *)a.base + tc * a.ldb + mine;
+    const int row = r0 + l % LANES * E; /* first of this lane's piece */
+    const bool whole = row + E <= a.rows;
+    const int ids = adapter(a, blockIdx.y * 64 + l);
+    int held = -1; /* whose B the registers hold */
+    typename Mul::A w[J > 0 ? J : 1][4];
+    auto get = [&](int ad, int j, typename Mul::A *q) {
 #pragma unroll
-    for (int i = 0; i < 16; i++) out[i] = 0.f;
-    if (a.base) {
+        for (int f = 0; f < 4; f++)
+            q[f].set(load8<WTY>(a.b, ((long long)ad * a.rows + min(r0 + 16 * f + c16, a.rows - 1)) * a.rank + j + 8 * g, a.rank - j - 8 * g));
+    };
 #pragma unroll
-        for (int p = 0; p < PIECES; p++) {
-            if (mine + 16 <= a.rows) {
-                const v4u v = *(const LE_GLOBAL v4u_any *)(base + p * E);
+    for (int n = 0; n < 4; n++) {
+        const int t0 = blockIdx.y * 64 + 16 * n, tok = t0 + c16;
+        if (t0 >= a.m) break;
+        v4u base[PIECES];
 #pragma unroll
-                for (int e = 0; e < E; e++) out[p * E + e] = unpack<XTY>(v, e);
-            } else {
-#pragma unroll
-                for (int e = 0; e < E; e++)
-                    if (mine + p * E + e < a.rows) out[p * E + e] = XT<XTY>::up(base[p * E + e]);
-            }
-        }
-    }
-    while (t.next()) {
-        v4f c[4];
-        long long brow[4];
-#pragma unroll
-        for (int f = 0; f < 4; f++) {
-            c[f] = v4f{0.f, 0.f, 0.f, 0.f};
-            brow[f] = ((long long)t.cur * a.rows + min(r0 + (c16 >> 2) * 16 + f * 4 + (c16 & 3), a.rows - 1)) * a.rank;
-        }
-        const float s = factor(a, t.cur);
-        for (int j = 8 * g; j - 8 * g < a.rank; j += 32) {
+        for (int p = 0; p < PIECES; p++)
+            if (a.base && whole) base[p] = *(const LE_GLOBAL v4u_any *)((const LE_GLOBAL X *)a.base + min(t0 + p * E + l / LANES, a.m - 1) * a.ldb + row);
+        Tile t(__builtin_amdgcn_ds_bpermute((16 * n + c16) * 4, ids));
+        const float s = t.id >= 0 ? factor(a, t.id) : 0.f;
+        /* scale u of this lane's token, zeros where it has no adapter */
+        auto low = [&](int j) {
             Eight<0> u;
 #pragma unroll
             for (int i = 0; i < 8; i++) u.v[i] = 0.f;
-            if (t.id == t.cur)
+            if (t.id >= 0)
                 for (int seg = 0; seg < a.segs; seg++) {
-                    const Eight<0> p = load8<0>(a.u, ((long long)seg * a.m + tok) * a.rank + j, a.rank - j);
+                    const LE_GLOBAL float *from = (const LE_GLOBAL float *)a.u + place(a, seg, t0 >> 4, c16, j + 8 * g);
+                    const v4f lo = *(const LE_GLOBAL v4f *)from, hi = *(const LE_GLOBAL v4f *)(from + 256);
 #pragma unroll
-                    for (int i = 0; i < 8; i++) u.v[i] += p.v[i];
+                    for (int i = 0; i < 4; i++) u.v[i] += lo[i], u.v[4 + i] += hi[i];
                 }
 #pragma unroll
             for (int i = 0; i < 8; i++) u.v[i] *= s;
+            return u;
+        };
+        typename Mul::B u[J > 0 ? J : 1];
+        if constexpr (J > 0) {
 #pragma unroll
-            for (int f = 0; f < 4; f++) c[f] = multiply<WTY, 0>(load8<WTY>(a.b, brow[f] + j, a.rank - j), u, c[f]);
+            for (int j = 0; j < J; j++) u[j].set(low(32 * j));
         }
-        if (t.id == t.cur) {
+        v4f out[4];
 #pragma unroll
-            for (int f = 0; f < 4; f++)
+        for (int f = 0; f < 4; f++) out[f] = v4f{0.f, 0.f, 0.f, 0.f};
+        while (t.next()) {
+            v4f c[4];
 #pragma unroll
-                for (int i = 0; i < 4; i++) out[4 * f + i] += c[f][i];
+            for (int f = 0; f < 4; f++) c[f] = v4f{0.f, 0.f, 0.f, 0.f};
+            if constexpr (J > 0) {
+                if (t.cur != held) {
+#pragma unroll
+                    for (int j = 0; j < J; j++) get(t.cur, 32 * j, w[j]);
+                    held = t.cur;
+                }
+#pragma unroll
+                for (int j = 0; j < J; j++)
+#pragma unroll
+                    for (int f = 0; f < 4; f++) c[f] = multiply<WTY, 0>(w[j][f], u[j], c[f]);
+            } else {
+                for (int j = 0; j < a.rank; j += 32) {
+                    u[0].set(low(j));
+                    get(t.cur, j, w[0]);
+#pragma unroll
+                    for (int f = 0; f < 4; f++) c[f] = multiply<WTY, 0>(w[0][f], u[0], c[f]);
+                }
+            }
+            if (t.id == t.cur) {
+#pragma unroll
+                for (int f = 0; f < 4; f++) out[f] = c[f];
+            }
         }
-    }
-    if (tok >= a.m) return;
-    LE_GLOBAL X *y = (LE_GLOBAL X *)a.y + tok * a.ldy + mine;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); /* the wave's reads of the tile before */
+        __builtin_amdgcn_wave_barrier();
 #pragma unroll
-    for (int p = 0; p < PIECES; p++) {
-        if (mine + 16 <= a.rows) {
-            v4u v;
+        for (int f = 0; f < 4; f++) *(v4f *)&mine[c16 * PITCH + 16 * f + 4 * g] = out[f];
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
 #pragma unroll
-            for (int d = 0; d < 4; d++) v[d] = pack<XTY>(out + p * E, d);
-            *(LE_GLOBAL v4u_any *)(y + p * E) = v;
-        } else {
+        for (int p = 0; p < PIECES; p++) {
+            const int i = p * E + l / LANES, k = t0 + i;
+            float v[E];
 #pragma unroll
-            for (int e = 0; e < E; e++)
-                if (mine + p * E + e < a.rows) y[p * E + e] = XT<XTY>::down(out[p * E + e]);
+            for (int e = 0; e < E; e += 4) *(v4f *)&v[e] = *(const v4f *)&mine[i * PITCH + l % LANES * E + e];
+            if (k >= a.m) continue;
+            LE_GLOBAL X *y = (LE_GLOBAL X *)a.y + k * a.ldy + row;
+            if (whole) {
+                if (a.base) {
+#pragma unroll
+                    for (int e = 0; e < E; e++) v[e] += unpack<XTY>(base[p], e);
+                }
+                v4u q;
+#pragma unroll
+                for (int d = 0; d < 4; d++) q[d] = pack<XTY>(v, d);
+                *(LE_GLOBAL v4u_any *)y = q;
+            } else {
+#pragma unroll
+                for (int e = 0; e < E; e++)
+                    if (row + e < a.rows) y[e] = XT<XTY>::down(a.base ? XT<XTY>::up(((const LE_GLOBAL X *)a.base)[k * a.ldb + row + e]) + v[e] : v[e]);
+            }
         }
     }
 }
@@ -311,12 +486,15 @@ template <int WTY> __device__ __forceinline__ void upm_body(const LoraArgs &a) {
 
 #define LE_LO_NAME2(WHAT, X, W) le_lo_##WHAT##_##X##_##W
 #define LE_LO_NAME(WHAT, X, W) LE_LO_NAME2(WHAT, X, W)
-#define LE_LO(W)                                                                                                              \
-    extern "C" __global__ void __launch_bounds__(256) LE_LO_NAME(down1, LE_LO_XTY, W)(LoraArgs a) { down_body<W, 1>(a); } \
-    extern "C" __global__ void __launch_bounds__(256) LE_LO_NAME(down2, LE_LO_XTY, W)(LoraArgs a) { down_body<W, 2>(a); } \
-    extern "C" __global__ void __launch_bounds__(256) LE_LO_NAME(down4, LE_LO_XTY, W)(LoraArgs a) { down_body<W, 4>(a); } \
-    extern "C" __global__ void __launch_bounds__(256) LE_LO_NAME(upv, LE_LO_XTY, W)(LoraArgs a) { upv_body<W>(a); }       \
-    extern "C" __global__ void __launch_bounds__(256) LE_LO_NAME(upm, LE_LO_XTY, W)(LoraArgs a) { upm_body<W>(a); }
+#define LE_LO(W)                                                                                                             \
+    extern "C" __global__ void __launch_bounds__(512) LE_LO_NAME(down1, LE_LO_XTY, W)(LoraArgs a) { down_body<W, 1>(a); } \
+    extern "C" __global__ void __launch_bounds__(512) LE_LO_NAME(down2, LE_LO_XTY, W)(LoraArgs a) { down_body<W, 2>(a); } \
+    extern "C" __global__ void __launch_bounds__(512) LE_LO_NAME(down4, LE_LO_XTY, W)(LoraArgs a) { down_body<W, 4>(a); } \
+    extern "C" __global__ void __launch_bounds__(256) LE_LO_NAME(upv1, LE_LO_XTY, W)(LoraArgs a) { upv_body<W, 1>(a); }    \
+    extern "C" __global__ void __launch_bounds__(256) LE_LO_NAME(upv4, LE_LO_XTY, W)(LoraArgs a) { upv_body<W, 4>(a); }    \
+    extern "C" __global__ void __launch_bounds__(256) LE_LO_NAME(upm0, LE_LO_XTY, W)(LoraArgs a) { upm_body<W, 0>(a); }    \
+    extern "C" __global__ void __launch_bounds__(256) LE_LO_NAME(upm1, LE_LO_XTY, W)(LoraArgs a) { upm_body<W, 1>(a); }    \
+    extern "C" __global__ void __launch_bounds__(256) LE_LO_NAME(upm2, LE_LO_XTY, W)(LoraArgs a) { upm_body<W, 2>(a); }
 LE_LO(0)
 LE_LO(1)
 LE_LO(30)

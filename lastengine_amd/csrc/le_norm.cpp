@@ -26,7 +26,17 @@ extern "C" int le_add_rms_quant(le_ctx *c, int ty, const void *x, long long ldx,
     if (int rc = le_ctx_on_device(c)) return rc;
     NormArgs a{x, res, w, h, o, (signed char *)xq, xd, xs, ldx, ldr, ldh, ldo, m, n, eps};
     void *args[] = {&a};
+    const int V = 16 / b, pieces = (n + V - 1) / V;
     char name[40];
-    snprintf(name, sizeof name, "le_nq_%d", ty);
-    return le_ctx_launch(c, name, dim3((unsigned)std::min(m, 1 << 20)), 256, 0, (hipStream_t)stream, args);
+    if (n % V || pieces > 4096) {
+        const int L = pieces <= 1024 ? 256 : 1024;
+        snprintf(name, sizeof name, "le_nq_%d_any%d", ty, L);
+        return le_ctx_launch(c, name, dim3((unsigned)std::min(m, 1 << 20)), L, 0, (hipStream_t)stream, args);
+    }
+    /* lanes a row: the fewest with four pieces or less each; more while the rows do not fill the chip */
+    int L = pieces <= 256 ? 64 : pieces <= 1024 ? 256 : 1024, nc = 1;
+    while (L < 1024 && pieces > L && (long long)m * L < 256LL * le_ctx_cus(c)) L *= 4;
+    while (nc * L < pieces) nc *= 2;
+    snprintf(name, sizeof name, "le_nq_%d_l%d_c%d", ty, L, nc);
+    return le_ctx_launch(c, name, dim3((unsigned)std::min(L == 64 ? (m + 3LL) / 4 : m, 1LL << 20)), L == 64 ? 256 : L, 0, (hipStream_t)stream, args);
 }
