@@ -72,13 +72,13 @@ extern "C" int le_lora(le_ctx *c, const le_adapters *ad, const int *idx, int xty
     if (int rc = le_ctx_launch(c, name, dim3((unsigned)sh.tiles, (unsigned)sh.turns, (unsigned)sh.segs), 64 * sh.waves,
                                sh.waves * std::max(sh.wave_lds, (size_t)sh.sets * 1024), (hipStream_t)stream, args))
         return rc;
+    const unsigned blocks = (unsigned)((ad->rows + 255) / 256);
     if (m <= 64) {
-        /* four rows a lane where that leaves 1024 blocks */
-        const int R = (ad->rows + 1023LL) / 1024 * sh.tiles * sh.turns >= 1024 ? 4 : 1;
-        snprintf(name, sizeof name, "le_lo_upv%d_%d_%d", R, xtype, ad->ltype);
-        return le_ctx_launch(c, name, dim3((unsigned)((ad->rows + 256 * R - 1) / (256 * R)), (unsigned)sh.tiles, (unsigned)sh.turns), 256,
-                             (size_t)4 * ((ad->rank + 7) & ~7) * 4, (hipStream_t)stream, args);
+        int G = 1; /* lanes a row of B */
+        while (8 * G < ad->rank) G *= 2;
+        snprintf(name, sizeof name, "le_lo_upv%d_%d_%d", G, xtype, ad->ltype);
+        return le_ctx_launch(c, name, dim3(std::min(blocks, (unsigned)std::max(1, 2048 / (sh.tiles * sh.turns))), (unsigned)sh.tiles, (unsigned)sh.turns), 256, 0, (hipStream_t)stream, args);
     }
     snprintf(name, sizeof name, "le_lo_upm%d_%d_%d", ad->rank <= 32 ? 1 : ad->rank <= 64 ? 2 : 0, xtype, ad->ltype);
-    return le_ctx_launch(c, name, dim3((unsigned)((ad->rows + 255) / 256), (unsigned)((sh.tiles + 3) / 4)), 256, 0, (hipStream_t)stream, args);
+    return le_ctx_launch(c, name, dim3(blocks, (unsigned)((sh.tiles + 3) / 4)), 256, 0, (hipStream_t)stream, args);
 }

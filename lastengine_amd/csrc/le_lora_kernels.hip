@@ -5,6 +5,7 @@
 #include <hip/hip_runtime.h>
 
 #include "le_f32_types.h"
+#include "le_lanes.h"
 #include "le_lora_args.h"
 
 #define LE_GLOBAL __attribute__((address_space(1)))
@@ -282,86 +283,109 @@ template <int WTY, int RF> __device__ __forceinline__ void down_body(const LoraA
 __device__ __forceinline__ float factor(const LoraArgs &a, int ad) { return a.scale ? ((const LE_GLOBAL float *)a.scale)[ad] : 1.f; }
 
 /* ---- up, few tokens ----
- * A lane R output rows; their first 16 values of B are read once for all tokens of the adapter (on their way while u comes to LDS), which are
- * taken four at a time. */
-template <int WTY, int R> __device__ __forceinline__ void upv_body(const LoraArgs &a) {
-    extern __shared__ float lu[]; /* [4 tokens][rank, rounded up to 8] */
-    const int rp = (a.rank + 7) & ~7, t0 = blockIdx.y * 16, r0 = blockIdx.x * (256 * R) + threadIdx.x;
-    Tile t(adapter(a, t0 + (threadIdx.x & 15)));
+ * A wave 64 output rows, G lanes with eight values each a row of B (so that a wave's loads are whole lines), G turns for all of them; after
+ * each the group's sum stays with the lane whose row it is. Lane l ends with row l. B is read once for all tokens of the adapter up to
+ * a rank of 64, and the tokens are taken four at a time. u of the whole tile is fetched beside the adapters' numbers, not after them, and
+ * the next 64 rows' operands during these' sums. */
+template <int WTY, int G> __device__ __forceinline__ void upv_body(const LoraArgs &a) {
+    constexpr int RP = 8 * G, TURNS = G < 8 ? G : 8; /* turns whose B is in registers at once */
+    __shared__ __attribute__((aligned(16))) float lu[16][RP]; /* A x of the tile's tokens; of those without an adapter nothing that is used */
+    const int l = threadIdx.x & 63, t0 = blockIdx.y * 16;
+    const int id = adapter(a, t0 + (l & 15));
+    const long long seg = place(a, 1, 0, 0, 0);
+    for (int i = threadIdx.x; i < 16 * RP; i += 256) {
+        const int j = i & (RP - 1);
+        const LE_GLOBAL float *u = (const LE_GLOBAL float *)a.u + place(a, 0, blockIdx.y, i / RP, j);
+        float v = 0.f;
+        if (j < a.rank)
+#pragma unroll 8
+            for (int s = 0; s < a.segs; s++) v += u[s * seg];
+        lu[0][i] = v;
+    }
+    __syncthreads();
+    Tile t(id);
     const LE_GLOBAL X *base = (const LE_GLOBAL X *)a.base;
+    LE_GLOBAL X *y = (LE_GLOBAL X *)a.y;
+    const int step = gridDim.x * 256, first = (blockIdx.x * 4 + (threadIdx.x >> 6)) * 64, part = l & (G - 1);
     if (blockIdx.z == 0) { /* tokens of no adapter */
         for (unsigned none = ~t.left & 0xFFFF; none; none &= none - 1) {
             const int k = t0 + __ffs((int)none) - 1;
             if (k >= a.m) break;
-#pragma unroll
-            for (int q = 0; q < R; q++)
-                if (r0 + 256 * q < a.rows) ((LE_GLOBAL X *)a.y)[k * a.ldy + r0 + 256 * q] = a.base ? base[k * a.ldb + r0 + 256 * q] : X(0);
+            for (int r = first + l; r < a.rows; r += step) y[k * a.ldy + r] = a.base ? base[k * a.ldb + r] : X(0);
         }
     }
     for (int nth = 0; t.next(); nth++) {
         if (nth % gridDim.z != blockIdx.z) continue;
-        long long row[R];
-        Eight<WTY> w[R][2];
-#pragma unroll
-        for (int q = 0; q < R; q++) {
-            row[q] = ((long long)t.cur * a.rows + min(r0 + 256 * q, a.rows - 1)) * a.rank;
-            w[q][0] = load8<WTY>(a.b, row[q], a.rank);
-            w[q][1] = load8<WTY>(a.b, row[q] + 8, a.rank - 8);
-        }
-        const float f = factor(a, t.cur);
-        for (unsigned todo = t.members; todo;) {
+        struct Four {
             int k[4]; /* tokens; the last one again where fewer are left */
+            __device__ __forceinline__ Four(unsigned &todo) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    k[i] = todo ? __ffs((int)todo) - 1 : k[i > 0 ? i - 1 : 0];
+                    todo &= todo - 1;
+                }
+            }
+            __device__ __forceinline__ bool is(int i) const { return i == 0 || k[i] != k[i - 1]; }
+        };
+        struct Ahead { /* what the first four tokens' results of 64 rows are made of */
+            Eight<WTY> w[TURNS];
+            float b[4];
+        } now, next;
+        auto load = [&](Eight<WTY> *w, int r0, int turn) {
+#pragma unroll
+            for (int p = 0; p < TURNS; p++)
+                w[p] = load8<WTY>(a.b, ((long long)t.cur * a.rows + min(r0 + l - part + turn + p, a.rows - 1)) * a.rank + 8 * part, a.rank - 8 * part);
+        };
+        auto bases = [&](const Four &q, float *b, int r0) {
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                k[i] = todo ? t0 + __ffs((int)todo) - 1 : k[i > 0 ? i - 1 : 0];
-                todo &= todo - 1;
+                b[i] = 0.f;
+                if (a.base && q.is(i)) b[i] = XT<XTY>::up(base[(t0 + q.k[i]) * a.ldb + min(r0 + l, a.rows - 1)]);
             }
-            float b[4][R], acc[4][R];
+        };
+        unsigned others = t.members;
+        const Four four(others);
+        if (first < a.rows) load(now.w, first, 0), bases(four, now.b, first);
+        const float f = factor(a, t.cur);
+        for (int r0 = first; r0 < a.rows; r0 += step, now = next) {
+            if (r0 + step < a.rows) load(next.w, r0 + step, 0), bases(four, next.b, r0 + step);
+            auto take = [&](const Four &q, const float *b) {
+                float acc[4], u[4][8];
 #pragma unroll
-            for (int i = 0; i < 4; i++)
-#pragma unroll
-                for (int q = 0; q < R; q++) {
-                    b[i][q] = 0.f;
-                    if (a.base && (i == 0 || k[i] != k[i - 1])) b[i][q] = XT<XTY>::up(base[k[i] * a.ldb + min(r0 + 256 * q, a.rows - 1)]);
-                    acc[i][q] = 0.f;
+                for (int i = 0; i < 4; i++) {
+                    acc[i] = 0.f;
+                    if (q.is(i)) {
+                        *(v4f *)&u[i][0] = *(const v4f *)&lu[q.k[i]][8 * part];
+                        *(v4f *)&u[i][4] = *(const v4f *)&lu[q.k[i]][8 * part + 4];
+                    }
                 }
-            __syncthreads();
-            for (int id = threadIdx.x; id < 4 * rp; id += 256) {
-                const int i = id / rp, j = id - i * rp;
-                const LE_GLOBAL float *u = (const LE_GLOBAL float *)a.u + place(a, 0, blockIdx.y, (i == 0 ? k[0] : i == 1 ? k[1] : i == 2 ? k[2] : k[3]) - t0, j);
-                const long long seg = place(a, 1, 0, 0, 0);
-                float v = 0.f;
-#pragma unroll 8
-                for (int s = 0; s < a.segs; s++) v += u[s * seg];
-                lu[id] = f * v;
-            }
-            __syncthreads();
-            auto eight = [&](const Eight<WTY> &v, int q, int j) {
+#pragma unroll 1
+                for (int turn = 0; turn < G; turn += TURNS) {
+                    if (G > 8) load(now.w, r0, turn);
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        if (q.is(i)) {
+#pragma unroll
+                            for (int p = 0; p < TURNS; p++) {
+                                float s = now.w[p].up(0) * u[i][0];
+#pragma unroll
+                                for (int e = 1; e < 8; e++) s = fmaf(now.w[p].up(e), u[i][e], s);
+                                s = lanes_sum<G>(s);
+                                if (part == turn + p) acc[i] = s;
+                            }
+                        }
+                }
 #pragma unroll
                 for (int i = 0; i < 4; i++)
-                    if (i == 0 || k[i] != k[i - 1]) {
-#pragma unroll
-                        for (int e = 0; e < 8; e++) acc[i][q] = fmaf(v.up(e), lu[i * rp + j + e], acc[i][q]);
-                    }
+                    if (q.is(i) && r0 + l < a.rows) y[(t0 + q.k[i]) * a.ldy + r0 + l] = XT<XTY>::down(fmaf(f, acc[i], b[i]));
             };
-#pragma unroll
-            for (int q = 0; q < R; q++) {
-                eight(w[q][0], q, 0);
-                if (a.rank > 8) eight(w[q][1], q, 8);
+            take(four, now.b);
+            for (unsigned todo = others; todo;) {
+                const Four q(todo);
+                float b[4];
+                bases(q, b, r0);
+                take(q, b);
             }
-            for (int j = 16; j < a.rank; j += 8) {
-                Eight<WTY> v[R];
-#pragma unroll
-                for (int q = 0; q < R; q++) v[q] = load8<WTY>(a.b, row[q] + j, a.rank - j);
-#pragma unroll
-                for (int q = 0; q < R; q++) eight(v[q], q, j);
-            }
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-#pragma unroll
-                for (int q = 0; q < R; q++)
-                    if ((i == 0 || k[i] != k[i - 1]) && r0 + 256 * q < a.rows)
-                        ((LE_GLOBAL X *)a.y)[k[i] * a.ldy + r0 + 256 * q] = XT<XTY>::down(b[i][q] + acc[i][q]);
         }
     }
 }
@@ -490,8 +514,12 @@ template <int WTY, int J> __device__ __forceinline__ void upm_body(const LoraArg
     extern "C" __global__ void __launch_bounds__(512) LE_LO_NAME(down1, LE_LO_XTY, W)(LoraArgs a) { down_body<W, 1>(a); } \
     extern "C" __global__ void __launch_bounds__(512) LE_LO_NAME(down2, LE_LO_XTY, W)(LoraArgs a) { down_body<W, 2>(a); } \
     extern "C" __global__ void __launch_bounds__(512) LE_LO_NAME(down4, LE_LO_XTY, W)(LoraArgs a) { down_body<W, 4>(a); } \
-    extern "C" __global__ void __launch_bounds__(256) LE_LO_NAME(upv1, LE_LO_XTY, W)(LoraArgs a) { upv_body<W, 1>(a); }    \
-    extern "C" __global__ void __launch_bounds__(256) LE_LO_NAME(upv4, LE_LO_XTY, W)(LoraArgs a) { upv_body<W, 4>(a); }    \
+    extern "C" __global__ void __launch_bounds__(256) LE_LO_NAME(upv1, LE_LO_XTY, W)(LoraArgs a) { upv_body<W, 1>(a); } \
+    extern "C" __global__ void __launch_bounds__(256) LE_LO_NAME(upv2, LE_LO_XTY, W)(LoraArgs a) { upv_body<W, 2>(a); } \
+    extern "C" __global__ void __launch_bounds__(256) LE_LO_NAME(upv4, LE_LO_XTY, W)(LoraArgs a) { upv_body<W, 4>(a); } \
+    extern "C" __global__ void __launch_bounds__(256) LE_LO_NAME(upv8, LE_LO_XTY, W)(LoraArgs a) { upv_body<W, 8>(a); } \
+    extern "C" __global__ void __launch_bounds__(256) LE_LO_NAME(upv16, LE_LO_XTY, W)(LoraArgs a) { upv_body<W, 16>(a); } \
+    extern "C" __global__ void __launch_bounds__(256) LE_LO_NAME(upv32, LE_LO_XTY, W)(LoraArgs a) { upv_body<W, 32>(a); } \
     extern "C" __global__ void __launch_bounds__(256) LE_LO_NAME(upm0, LE_LO_XTY, W)(LoraArgs a) { upm_body<W, 0>(a); }    \
     extern "C" __global__ void __launch_bounds__(256) LE_LO_NAME(upm1, LE_LO_XTY, W)(LoraArgs a) { upm_body<W, 1>(a); }    \
     extern "C" __global__ void __launch_bounds__(256) LE_LO_NAME(upm2, LE_LO_XTY, W)(LoraArgs a) { upm_body<W, 2>(a); }

@@ -8,6 +8,7 @@
 #include <hip/hip_runtime.h>
 
 #include "le_f32_types.h"
+#include "le_lanes.h"
 #include "le_norm_args.h"
 
 #define LE_GLOBAL __attribute__((address_space(1)))
@@ -19,19 +20,6 @@ typedef unsigned v4u __attribute__((ext_vector_type(4)));
 template <int S> struct Any;
 template <> struct Any<2> { typedef v4u __attribute__((aligned(2))) v; };
 template <> struct Any<4> { typedef v4u __attribute__((aligned(4))) v; };
-
-/* Value of the lane across in the quad (1, 2) or in the other quad of eight lanes, where all of a quad hold the same (4) */
-template <int D> __device__ __forceinline__ int across(int v) {
-    return __builtin_amdgcn_mov_dpp(v, D == 1 ? 0xB1 : D == 2 ? 0x4E : 0x141, 0xf, 0xf, true);
-}
-template <int N, int D = 1> __device__ __forceinline__ float lanes_max(float v) {
-    if constexpr (D < N) return lanes_max<N, 2 * D>(fmaxf(v, __builtin_bit_cast(float, across<D>(__builtin_bit_cast(int, v)))));
-    else return v;
-}
-template <int N, int D = 1> __device__ __forceinline__ int lanes_sum(int v) {
-    if constexpr (D < N) return lanes_sum<N, 2 * D>(v + across<D>(v));
-    else return v;
-}
 
 /* A piece's values: all, or the n that there are (zeros behind them); TAIL: n may also lie between.
  * ONCE: read by nobody else (not kept in the caches: 4096 x 4096, x, res and o of fp32 82 -> 63 us, of bf16 48 -> 38). */
