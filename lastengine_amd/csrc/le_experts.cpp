@@ -24,10 +24,22 @@ unsigned blocks_for(long long tiles, int run) {
     return (unsigned)std::min((tiles + turn - 1) / turn * turn, (1LL << 23) / turn * turn);
 }
 
-int launch(le_ctx *c, const char *what, ExpertArgs &a, long long row_tiles, le_stream_t stream) {
-    a.run = 1;
+/* The kernel of `what`_type for tiles of 128 rows. whole: every row of the operands is whole 16-byte chunks. */
+int launch(le_ctx *c, const char *what, int ty, ExpertArgs &a, bool whole, long long row_tiles, le_stream_t stream) {
+    const int bn = whole && a.n > 128 ? 256 : 128;
+    a.nt = (a.n + bn - 1) / bn;
+    const long long tiles = row_tiles * a.nt;
+    if (tiles > 0x7FFFFFFFLL) return le_ctx_fail(c, LE_ERR_SHAPE, "more than 2^31 tiles");
+    a.run = (int)std::max(1LL, std::min(tiles / a.n_exp, tiles / 64));
+    char name[40];
+    if (whole) snprintf(name, sizeof name, "le_ex_%s_%d_n%d", what, ty, bn);
+    else snprintf(name, sizeof name, "le_ex_%s_%d_any", what, ty);
     void *args[] = {&a};
-    return le_ctx_launch(c, what, dim3(blocks_for(row_tiles * a.nt, a.run)), 256, 0, (hipStream_t)stream, args);
+    return le_ctx_launch(c, name, dim3(blocks_for(tiles, a.run)), 256, whole ? (size_t)3 * (128 + bn) * 64 : 0, (hipStream_t)stream, args);
+}
+bool whole_rows(int ty, const void *p, const void *q, long long ld1, long long ld2, int rows, int cols) {
+    const int n = 16 / le_type_bytes(ty);
+    return le_aligned(p, 16) && le_aligned(q, 16) && ld1 % n == 0 && ld2 % n == 0 && rows % n == 0 && cols % n == 0;
 }
 
 }  // namespace
@@ -44,10 +56,8 @@ int le_mm_experts(le_ctx *c, int ty, const void *w, const int *off, int n_exp, c
     if (!le_aligned(w, b) || !le_aligned(x, b) || !le_aligned(y, b) || !le_aligned(off, 4))
         return le_ctx_fail(c, LE_ERR_ALIGN, "pointers must be aligned to their types");
     if (int rc = le_ctx_on_device(c)) return rc;
-    ExpertArgs a{x, w, y, off, ldx, cols, ldy, n_exp, n_row, n_row, rows, cols, 0, (rows + 127) / 128, 1};
-    char name[40];
-    snprintf(name, sizeof name, "le_ex_y_%d_any", ty);
-    return launch(c, name, a, n_row / 128 + std::min(n_exp, n_row), stream);
+    ExpertArgs a{x, w, y, off, ldx, cols, ldy, n_exp, n_row, n_row, rows, cols, 0, 0, 1};
+    return launch(c, "y", ty, a, whole_rows(ty, x, w, ldx, 0, rows, cols), n_row / 128 + std::min(n_exp, n_row), stream);
 }
 
 int le_mm_experts_dx(le_ctx *c, int ty, const void *w, const int *off, int n_exp, const void *dy, long long ldy, void *dx,
@@ -60,10 +70,8 @@ int le_mm_experts_dx(le_ctx *c, int ty, const void *w, const int *off, int n_exp
     if (!le_aligned(w, b) || !le_aligned(dy, b) || !le_aligned(dx, b) || !le_aligned(off, 4))
         return le_ctx_fail(c, LE_ERR_ALIGN, "pointers must be aligned to their types");
     if (int rc = le_ctx_on_device(c)) return rc;
-    ExpertArgs a{dy, w, dx, off, ldy, cols, ldx, n_exp, n_row, n_row, cols, rows, 0, (cols + 127) / 128, 1};
-    char name[40];
-    snprintf(name, sizeof name, "le_ex_dx_%d_any", ty);
-    return launch(c, name, a, n_row / 128 + std::min(n_exp, n_row), stream);
+    ExpertArgs a{dy, w, dx, off, ldy, cols, ldx, n_exp, n_row, n_row, cols, rows, 0, 0, 1};
+    return launch(c, "dx", ty, a, whole_rows(ty, dy, w, ldy, 0, rows, cols), n_row / 128 + std::min(n_exp, n_row), stream);
 }
 
 size_t le_mm_experts_dw_workspace_size(int, int, int, int, int) { return 0; }
@@ -79,12 +87,9 @@ int le_mm_experts_dw(le_ctx *c, int ty, const void *dy, long long ldy, const voi
         return le_ctx_fail(c, LE_ERR_ALIGN, "pointers must be aligned to their types, ws to 16 bytes");
     const size_t need = le_mm_experts_dw_workspace_size(ty, n_exp, n_row, rows, cols);
     if (need && (!ws || ws_bytes < need)) return le_ctx_failf(c, LE_ERR_WORKSPACE, "workspace needs %zu bytes", need);
-    ExpertArgs a{dy, x, dw, off, ldy, ldx, cols, n_exp, n_row, rows, cols, n_row, (rows + 127) / 128, (cols + 127) / 128, 1};
-    if ((long long)a.mt * a.nt * n_exp > 0x7FFFFFFFLL) return le_ctx_fail(c, LE_ERR_SHAPE, "more than 2^31 tiles of 128 x 128");
+    ExpertArgs a{dy, x, dw, off, ldy, ldx, cols, n_exp, n_row, rows, cols, n_row, (rows + 127) / 128, 0, 1};
     if (int rc = le_ctx_on_device(c)) return rc;
-    char name[40];
-    snprintf(name, sizeof name, "le_ex_dw%s_%d_any", dwtype == ty ? "" : "f", ty);
-    return launch(c, name, a, (long long)a.mt * n_exp, stream);
+    return launch(c, dwtype == ty ? "dw" : "dwf", ty, a, whole_rows(ty, dy, x, ldy, ldx, rows, cols), (long long)a.mt * n_exp, stream);
 }
 
 }  // extern "C"

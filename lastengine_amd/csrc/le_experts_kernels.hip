@@ -188,15 +188,65 @@ template <bool DOWN, int R> struct Loader {
 };
 
 enum Kind { Y, DX, DW };
+template <int N> struct Count { static constexpr int value = N; };
 
-template <int YTY> __device__ __forceinline__ void put(void *y, long long at, float v) {
-    ((LE_GLOBAL typename XT<YTY>::raw *)y)[at] = XT<YTY>::down(v);
-}
+/* ---- results ----
+ * The operands go into the matrix instruction as (B, A): a lane then holds row l % 32 of the tile's 32 and 16 of 32 columns, four in a row. NF such
+ * fragments side by side are rounded and change places through LDS of the wave's own, so that whole lines are written. */
+template <int YTY, int NF> struct Out {
+    using U = typename XT<YTY>::raw;
+    static constexpr int E = 16 / sizeof(U), LANES = 32 * NF / E, PITCH = 32 * NF * sizeof(U) + 16, BYTES = 32 * PITCH;
+    /* rows of them there are, at y, ld apart; cols of them there are, from this wave's first on */
+    static __device__ __forceinline__ void put(LE_LDS char *mine, const v16f *c, void *y, long long ld, int rows, int cols) {
+        typedef v4u __attribute__((aligned(4))) v4u_a4;
+        typedef v4u __attribute__((aligned(2))) v4u_a2;
+        const int l = threadIdx.x & 63;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); /* the reads of the rows before */
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int n = 0; n < NF; n++)
+#pragma unroll
+            for (int q = 0; q < 4; q++) { /* columns 8 q + 4 (l / 32) and on */
+                LE_LDS char *p = mine + (l & 31) * PITCH + (32 * n + 8 * q + 4 * (l >> 5)) * (int)sizeof(U);
+                const float v0 = c[n][4 * q], v1 = c[n][4 * q + 1], v2 = c[n][4 * q + 2], v3 = c[n][4 * q + 3];
+                if constexpr (sizeof(U) == 4) {
+                    *(LE_LDS v4f *)p = v4f{v0, v1, v2, v3};
+                } else {
+                    typedef unsigned v2u __attribute__((ext_vector_type(2)));
+                    *(LE_LDS v2u *)p = v2u{XT<YTY>::down(v0) | (unsigned)XT<YTY>::down(v1) << 16, XT<YTY>::down(v2) | (unsigned)XT<YTY>::down(v3) << 16};
+                }
+            }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        const int col = l % LANES * E;
+#pragma unroll
+        for (int i = 0; i < 32; i += 64 / LANES) {
+            const int r = i + l / LANES;
+            const v4u v = *(LE_LDS const v4u *)(mine + r * PITCH + col * (int)sizeof(U));
+            LE_GLOBAL U *to = (LE_GLOBAL U *)y + r * ld + col;
+            if (r < rows) {
+                if (col + E <= cols) {
+                    if constexpr (sizeof(U) == 4) *(LE_GLOBAL v4u_a4 *)to = v;
+                    else *(LE_GLOBAL v4u_a2 *)to = v;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < E - 1; e++)
+                        if (col + e < cols) {
+                            const unsigned w = v[sizeof(U) == 4 ? e : e >> 1];
+                            if constexpr (sizeof(U) == 4) to[e] = __builtin_bit_cast(float, w);
+                            else to[e] = (U)(w >> (e & 1) * 16);
+                        }
+                }
+            }
+        }
+    }
+};
 
 template <Kind KIND, int YTY> __device__ __forceinline__ void any_body(const ExpertArgs &a) {
     constexpr int BM = 128, BN = 128, MF = BM / 32;
     constexpr bool AD = KIND == DW, BD = KIND != Y;
-    __shared__ __attribute__((aligned(16))) char smem[(BM + BN) * 64];
+    constexpr int TILES = (BM + BN) * 64, OUT = 4 * Out<YTY, 1>::BYTES;
+    __shared__ __attribute__((aligned(16))) char smem[TILES > OUT ? TILES : OUT];
     LE_LDS char *ta = (LE_LDS char *)smem, *tb = ta + BM * 64;
     const int l = threadIdx.x & 63, wn = (threadIdx.x >> 6) * 32;
     for (long long b = blockIdx.x;; b += gridDim.x) {
@@ -228,19 +278,144 @@ template <Kind KIND, int YTY> __device__ __forceinline__ void any_body(const Exp
                 const Frag fb = frag<BD, BN>(tb, wn, s, l);
 #pragma unroll
                 for (int i = 0; i < MF; i++)
-                    if (i < mf) c[i] = mfma(frag<AD, BM>(ta, 32 * i, s, l), fb, c[i]);
+                    if (i < mf) c[i] = mfma(fb, frag<AD, BM>(ta, 32 * i, s, l), c[i]);
             }
         }
-        const int n = t.n0 + wn + (l & 31);
-        const long long row0 = KIND == DW ? (long long)t.e * a.m : t.lo;
-        if (n < a.n) {
+        __syncthreads();
+        const long long row0 = (KIND == DW ? (long long)t.e * a.m : t.lo) + t.m0;
 #pragma unroll
-            for (int i = 0; i < MF; i++)
+        for (int i = 0; i < MF; i++)
+            if (i < mf)
+                Out<YTY, 1>::put((LE_LDS char *)smem + (threadIdx.x >> 6) * Out<YTY, 1>::BYTES, &c[i],
+                                 (typename XT<YTY>::raw *)a.y + (row0 + 32 * i) * a.ldy + t.n0 + wn, a.ldy, A.rows - 32 * i, B.rows - wn);
+    }
+}
+
+/* ---- rows of whole 16-byte chunks ----
+ * 128 x BN tiles by four waves of 128 x BN / 4. Chunks go straight to LDS (lane l's 16 bytes to M0 + 16 l, so a wave's 64 land in a row; the
+ * permutation is in which chunk a lane asks for), three steps in a ring: while one is multiplied, the next one's are about to land and those of the one
+ * after it leave. One barrier a step: behind it a step's chunks are there for all waves, and the step before is read by all. Rows
+ * beyond an expert's last are asked for as its last (their results are dropped), k beyond the depth as zeros. */
+
+__device__ __attribute__((aligned(16))) const unsigned kZeros[4] = {0, 0, 0, 0};
+
+/* In assembly, so that the compiler does not wait for it before every LDS read; step_ready below does. */
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+__device__ __forceinline__ void chunk_to_lds(unsigned long long from, unsigned lds) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"(lds) : "memory", "m0");
+}
+#pragma clang diagnostic pop
+/* All but this wave's last N chunks have landed, its reads of LDS are done, and so for the other waves. */
+template <int N> __device__ __forceinline__ void step_ready() {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+}
+
+/* A wave's part of an operand's chunks: N of the 64 a time. */
+template <bool DOWN, int R> struct Stream {
+    static constexpr int N = R * 64 / 16 / 256;
+    unsigned long long at[N]; /* address of this lane's chunk of the next step */
+    int left[N];              /* depth that is left there */
+    unsigned long long step;
+    __device__ __forceinline__ void start(const void *base, long long ld, int rows, int depth) {
+        step = DOWN ? (unsigned long long)ld * (BK * ES) : 64;
 #pragma unroll
-                for (int j = 0; j < 16; j++) {
-                    const int r = t.m0 + 32 * i + 8 * (j >> 2) + 4 * (l >> 5) + (j & 3);
-                    if (r < m) put<YTY>(a.y, (row0 + r) * a.ldy + n, c[i][j]);
+        for (int j = 0; j < N; j++) {
+            const int id = threadIdx.x + 256 * j;
+            int r, k;
+            if constexpr (!DOWN) {
+                r = id >> 2;
+                k = ((id & 3) ^ ((r >> 2) & 3)) * EPC;
+                r = min(r, rows - 1);
+            } else {
+                constexpr int C = R / EPC;
+                k = id / C;
+                const int sw = ES == 2 ? (k & 3) << 2 : ((k >> 2) & 1) << 3;
+                r = min(((id % C) ^ (sw & (C - 1))) * EPC, rows - EPC);
+            }
+            left[j] = depth - k;
+            at[j] = (unsigned long long)base + (DOWN ? k * ld + r : r * ld + k) * ES;
+        }
+    }
+    /* The next step's chunks; whole: all of them lie within the depth. */
+    __device__ __forceinline__ void load(unsigned lds, bool whole) {
+        const unsigned wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+#pragma unroll
+        for (int j = 0; j < N; j++) {
+            chunk_to_lds(whole || left[j] > 0 ? at[j] : (unsigned long long)kZeros, lds + wave * 1024 + j * 4096);
+            at[j] += step;
+            left[j] -= BK;
+        }
+    }
+};
+
+template <Kind KIND, int YTY, int BN> __device__ __forceinline__ void pipe_body(const ExpertArgs &a) {
+    constexpr int BM = 128, MF = 4, NF = BN / 128, STEP = (BM + BN) * 64, CHUNKS = (BM + BN) / 64;
+    constexpr bool AD = KIND == DW, BD = KIND != Y;
+    extern __shared__ __attribute__((aligned(16))) char ring[];
+    LE_LDS char *const lds = (LE_LDS char *)ring;
+    const int l = threadIdx.x & 63, wn = (threadIdx.x >> 6) * (BN / 4);
+    for (long long b = blockIdx.x;; b += gridDim.x) {
+        Tile t;
+        if (!(KIND == DW ? find_weights<BM, BN>(a, tile_of(a, b), t) : find_rows<BM, BN>(a, tile_of(a, b), t))) return;
+        const int m = KIND == DW ? a.m : t.cnt, depth = KIND == DW ? t.cnt : a.k, rows = m - t.m0, cols = a.n - t.n0;
+        const long long wsize = (long long)a.n * a.k;
+        const int steps = (depth + BK - 1) / BK;
+        Stream<AD, BM> A;
+        Stream<BD, BN> B;
+        A.start((const T *)a.a + (KIND == DW ? t.lo * a.lda + t.m0 : (long long)(t.lo + t.m0) * a.lda), a.lda, rows, depth);
+        B.start((const T *)a.b + (KIND == DW ? t.lo * a.ldb + t.n0 : wsize * t.e + (KIND == Y ? (long long)t.n0 * a.ldb : t.n0)), a.ldb, cols, depth);
+        int slot = 0, to = 0, left = depth; /* places in the ring; depth that has not been asked for */
+        auto ask = [&] {
+            const unsigned at = (unsigned)(unsigned long long)lds + to;
+            A.load(at, left >= BK);
+            B.load(at + BM * 64, left >= BK);
+            left -= BK;
+            to = to == 2 * STEP ? 0 : to + STEP;
+        };
+        auto tile = [&](auto frags) {
+            constexpr int F = decltype(frags)::value;
+            v16f c[F][NF];
+#pragma unroll
+            for (int i = 0; i < F; i++)
+#pragma unroll
+                for (int n = 0; n < NF; n++)
+#pragma unroll
+                    for (int j = 0; j < 16; j++) c[i][n][j] = 0.f;
+            /* two steps are asked for ahead, also behind the last (zeros): the count of chunks on their way is then always the same */
+            ask();
+            ask();
+            for (int s = 0; s < steps; s++) {
+                step_ready<CHUNKS>();
+                ask();
+                LE_LDS const char *ta = lds + slot, *tb = ta + BM * 64;
+                slot = slot == 2 * STEP ? 0 : slot + STEP;
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    Frag fb[NF];
+#pragma unroll
+                    for (int n = 0; n < NF; n++) fb[n] = frag<BD, BN>(tb, wn + 32 * n, h, l);
+#pragma unroll
+                    for (int i = 0; i < F; i++) {
+                        const Frag fa = frag<AD, BM>(ta, 32 * i, h, l);
+#pragma unroll
+                        for (int n = 0; n < NF; n++) c[i][n] = mfma(fb[n], fa, c[i][n]);
+                    }
                 }
+            }
+            step_ready<0>(); /* the ring is free */
+            const long long row0 = (KIND == DW ? (long long)t.e * a.m : t.lo) + t.m0;
+#pragma unroll
+            for (int i = 0; i < F; i++)
+                Out<YTY, NF>::put(lds + (threadIdx.x >> 6) * Out<YTY, NF>::BYTES, c[i], (typename XT<YTY>::raw *)a.y + (row0 + 32 * i) * a.ldy + t.n0 + wn, a.ldy,
+                                  rows - 32 * i, cols - wn);
+            step_ready<0>();
+        };
+        switch (min(MF, (rows + 31) / 32)) {
+        case 1: tile(Count<1>()); break;
+        case 2: tile(Count<2>()); break;
+        case 3: tile(Count<3>()); break;
+        default: tile(Count<4>()); break;
         }
     }
 }
@@ -249,9 +424,13 @@ template <Kind KIND, int YTY> __device__ __forceinline__ void any_body(const Exp
 
 #define LE_EX_NAME2(WHAT, TY, TAIL) le_ex_##WHAT##_##TY##TAIL
 #define LE_EX_NAME(WHAT, TY, TAIL) LE_EX_NAME2(WHAT, TY, TAIL)
-extern "C" __global__ void __launch_bounds__(256) LE_EX_NAME(y, LE_EX_TY, _any)(ExpertArgs a) { any_body<Y, TY>(a); }
-extern "C" __global__ void __launch_bounds__(256) LE_EX_NAME(dx, LE_EX_TY, _any)(ExpertArgs a) { any_body<DX, TY>(a); }
-extern "C" __global__ void __launch_bounds__(256) LE_EX_NAME(dw, LE_EX_TY, _any)(ExpertArgs a) { any_body<DW, TY>(a); }
+#define LE_EX(WHAT, KIND, YTY)                                                                                                   \
+    extern "C" __global__ void __launch_bounds__(256) LE_EX_NAME(WHAT, LE_EX_TY, _any)(ExpertArgs a) { any_body<KIND, YTY>(a); } \
+    extern "C" __global__ void __launch_bounds__(256, 2) LE_EX_NAME(WHAT, LE_EX_TY, _n128)(ExpertArgs a) { pipe_body<KIND, YTY, 128>(a); } \
+    extern "C" __global__ void __launch_bounds__(256, 2) LE_EX_NAME(WHAT, LE_EX_TY, _n256)(ExpertArgs a) { pipe_body<KIND, YTY, 256>(a); }
+LE_EX(y, Y, TY)
+LE_EX(dx, DX, TY)
+LE_EX(dw, DW, TY)
 #if LE_EX_TY != 0
-extern "C" __global__ void __launch_bounds__(256) LE_EX_NAME(dwf, LE_EX_TY, _any)(ExpertArgs a) { any_body<DW, 0>(a); }
+LE_EX(dwf, DW, 0)
 #endif
