@@ -18,25 +18,42 @@ int check_sizes(le_ctx *c, int ty, int n_exp, int n_row, int rows, int cols, lon
     return LE_OK;
 }
 
-/* Blocks for `tiles` tiles: whole turns of the eight XCDs with `run` tiles each (le_experts_kernels.hip, tile_of), in a loop beyond 2^23 */
-unsigned blocks_for(long long tiles, int run) {
-    const long long turn = 8LL * run;
-    return (unsigned)std::min((tiles + turn - 1) / turn * turn, (1LL << 23) / turn * turn);
-}
-
-/* The kernel of `what`_type for tiles of 128 rows. whole: every row of the operands is whole 16-byte chunks. */
-int launch(le_ctx *c, const char *what, int ty, ExpertArgs &a, bool whole, long long row_tiles, le_stream_t stream) {
-    const int bn = whole && a.n > 128 ? 256 : 128;
+/* The kernel of `what`_type. whole: every row that is read is whole 16-byte chunks. */
+int launch(le_ctx *c, const char *what, int ty, ExpertArgs &a, bool whole, le_stream_t stream) {
+    const bool dw = what[1] == 'w';
+    int bm = 128, bn = 128, ring = 3;
+    if (!whole) {
+        /* rows through registers: tiles of 32 rows for few rows an expert */
+        if (!dw ? a.n_row < 48LL * a.n_exp : a.m <= 32) bm = 32;
+    } else if (a.n > 128) {
+        bn = 256;
+        if (dw) bm = 256;
+        /* few rows an expert: more blocks, each with more on its way (64 rows of 128 experts of 1536 x 2048 bf16 81 / 69 us, 512 rows 150 / 149) */
+        else if (what[0] == 'y' && a.n_row < 4LL * a.n_exp) bm = 64, bn = 128, ring = 4;
+    }
+    a.mt = (a.m + bm - 1) / bm;
     a.nt = (a.n + bn - 1) / bn;
-    const long long tiles = row_tiles * a.nt;
+    const long long tiles = (dw ? (long long)a.mt * a.n_exp : a.n_row / bm + std::min(a.n_exp, a.n_row)) * a.nt;
     if (tiles > 0x7FFFFFFFLL) return le_ctx_fail(c, LE_ERR_SHAPE, "more than 2^31 tiles");
-    a.run = (int)std::max(1LL, std::min(tiles / a.n_exp, tiles / 64));
     char name[40];
-    if (whole) snprintf(name, sizeof name, "le_ex_%s_%d_n%d", what, ty, bn);
-    else snprintf(name, sizeof name, "le_ex_%s_%d_any", what, ty);
+    if (whole) snprintf(name, sizeof name, "le_ex_%s_%d_m%d_n%d", what, ty, bm, bn);
+    else snprintf(name, sizeof name, "le_ex_%s_%d_any%d", what, ty, bm);
     void *args[] = {&a};
-    return le_ctx_launch(c, name, dim3(blocks_for(tiles, a.run)), 256, whole ? (size_t)3 * (128 + bn) * 64 : 0, (hipStream_t)stream, args);
+    if (bm == 256) {
+        /* a block a CU; the ring (three steps for fp32 results, whose rows take more of LDS, else four), the results of eight waves, off */
+        const bool f32 = ty == LE_F32 || what[2] == 'f';
+        const size_t lds = (size_t)(f32 ? 3 : 4) * 512 * 64 + 8 * 16 * (64 * (f32 ? 4 : 2) + 16) + (size_t)(a.n_exp + 1) * 4;
+        const int cus = std::max(8, le_ctx_cus(c));
+        for (a.run = 1; a.run * 2 <= tiles / 8 && cus / 8 % (a.run * 2) == 0;) a.run *= 2;
+        return le_ctx_launch(c, name, dim3((unsigned)(cus / (8 * a.run) * (8 * a.run))), 512, lds, (hipStream_t)stream, args);
+    }
+    /* tiles in whole turns of the eight XCDs, `run` in a row to each: an expert's, which share weights (18 in a row 351 us, 4 373, single ones 414) */
+    a.run = (int)std::max(1LL, std::min({tiles / a.n_exp, tiles / 64, 1LL << 16}));
+    const long long turn = 8LL * a.run;
+    return le_ctx_launch(c, name, dim3((unsigned)std::min((tiles + turn - 1) / turn * turn, (1LL << 23) / turn * turn)), 256, whole ? (size_t)ring * (bm + bn) * 64 : 0,
+                         (hipStream_t)stream, args);
 }
+/* Whether rows of `rows` and `cols` values, ld1 and ld2 apart, are whole 16-byte chunks. */
 bool whole_rows(int ty, const void *p, const void *q, long long ld1, long long ld2, int rows, int cols) {
     const int n = 16 / le_type_bytes(ty);
     return le_aligned(p, 16) && le_aligned(q, 16) && ld1 % n == 0 && ld2 % n == 0 && rows % n == 0 && cols % n == 0;
@@ -57,7 +74,7 @@ int le_mm_experts(le_ctx *c, int ty, const void *w, const int *off, int n_exp, c
         return le_ctx_fail(c, LE_ERR_ALIGN, "pointers must be aligned to their types");
     if (int rc = le_ctx_on_device(c)) return rc;
     ExpertArgs a{x, w, y, off, ldx, cols, ldy, n_exp, n_row, n_row, rows, cols, 0, 0, 1};
-    return launch(c, "y", ty, a, whole_rows(ty, x, w, ldx, 0, rows, cols), n_row / 128 + std::min(n_exp, n_row), stream);
+    return launch(c, "y", ty, a, whole_rows(ty, x, w, ldx, 0, cols, cols), stream);
 }
 
 int le_mm_experts_dx(le_ctx *c, int ty, const void *w, const int *off, int n_exp, const void *dy, long long ldy, void *dx,
@@ -71,7 +88,7 @@ int le_mm_experts_dx(le_ctx *c, int ty, const void *w, const int *off, int n_exp
         return le_ctx_fail(c, LE_ERR_ALIGN, "pointers must be aligned to their types");
     if (int rc = le_ctx_on_device(c)) return rc;
     ExpertArgs a{dy, w, dx, off, ldy, cols, ldx, n_exp, n_row, n_row, cols, rows, 0, 0, 1};
-    return launch(c, "dx", ty, a, whole_rows(ty, dy, w, ldy, 0, rows, cols), n_row / 128 + std::min(n_exp, n_row), stream);
+    return launch(c, "dx", ty, a, whole_rows(ty, dy, w, ldy, 0, rows, cols), stream);
 }
 
 size_t le_mm_experts_dw_workspace_size(int, int, int, int, int) { return 0; }
@@ -87,9 +104,9 @@ int le_mm_experts_dw(le_ctx *c, int ty, const void *dy, long long ldy, const voi
         return le_ctx_fail(c, LE_ERR_ALIGN, "pointers must be aligned to their types, ws to 16 bytes");
     const size_t need = le_mm_experts_dw_workspace_size(ty, n_exp, n_row, rows, cols);
     if (need && (!ws || ws_bytes < need)) return le_ctx_failf(c, LE_ERR_WORKSPACE, "workspace needs %zu bytes", need);
-    ExpertArgs a{dy, x, dw, off, ldy, ldx, cols, n_exp, n_row, rows, cols, n_row, (rows + 127) / 128, 0, 1};
+    ExpertArgs a{dy, x, dw, off, ldy, ldx, cols, n_exp, n_row, rows, cols, n_row, 0, 0, 1};
     if (int rc = le_ctx_on_device(c)) return rc;
-    return launch(c, dwtype == ty ? "dw" : "dwf", ty, a, whole_rows(ty, dy, x, ldy, ldx, rows, cols), (long long)a.mt * n_exp, stream);
+    return launch(c, dwtype == ty ? "dw" : "dwf", ty, a, whole_rows(ty, dy, x, ldy, ldx, rows, cols), stream);
 }
 
 }  // extern "C"
