@@ -10,4 +10,6 @@ struct ExpertArgs {
     int m, n, k;     /* outputs and depth; the one that counts an expert's rows is n_row here */
     int mt, nt;      /* tiles along M (weights' gradient) and N */
     int run;         /* tiles in a row that one XCD takes */
+    int segs;        /* weights' gradient: parts of an expert's rows, each with sums of its own */
+    int strip;       /* few rows: tiles of 32 outputs that a wave takes one after the other */
 };

@@ -35,9 +35,9 @@ typedef __bf16 v8b __attribute__((ext_vector_type(8)));
 
 /* ---- tiles in LDS ---- */
 
-/* W: bytes of k in a row of an `along` tile, 64 or 128. Sixteen rows' chunks of one k fill the 64 banks once. */
+/* W: bytes of k in a row of an `along` tile, 64, 128 or 256. Sixteen rows' chunks of one k fill the 64 banks once. */
 template <bool DOWN, int R, int W> __device__ __forceinline__ int swizzle(int row_or_k) {
-    if constexpr (!DOWN) return W == 64 ? (row_or_k >> 2) & 3 : (row_or_k >> 1) & 7;
+    if constexpr (!DOWN) return W == 64 ? (row_or_k >> 2) & 3 : W == 128 ? (row_or_k >> 1) & 7 : row_or_k & 15;
     else return (ES == 2 ? (row_or_k & 3) << 2 : ((row_or_k >> 2) & 1) << 3) & (R / EPC - 1);
 }
 template <bool DOWN, int R, int W = 64> __device__ __forceinline__ int lds_at(int row_or_k, int chunk) {
@@ -107,10 +107,12 @@ template <int BM, int BN> __device__ __forceinline__ void place(Tile &t, long lo
 /* Tile t of an expert's rows by outputs; every wave finds it by itself, 64 experts a turn. False: behind the last. */
 template <int BM, int BN, class OFF> __device__ __forceinline__ bool find_rows(const ExpertArgs &a, OFF off, long long q, Tile &t) {
     const int l = threadIdx.x & 63, u = (int)(q / a.nt); /* row tiles before this one, over all experts */
-    int before = 0;
+    int before = 0, lo1 = 0, cnt1 = 0;
+    if (l < a.n_exp) rows_of(a, off, l, lo1, cnt1);
     for (int e0 = 0; e0 < a.n_exp; e0 += 64) {
-        int lo = 0, cnt = 0;
-        if (e0 + l < a.n_exp) rows_of(a, off, e0 + l, lo, cnt);
+        const int lo = lo1, cnt = cnt1;
+        lo1 = cnt1 = 0;
+        if (e0 + 64 + l < a.n_exp) rows_of(a, off, e0 + 64 + l, lo1, cnt1); /* the next turn's meanwhile */
         const int mine = (int)(((long long)cnt + BM - 1) / BM);
         int sum = mine;
 #pragma unroll
@@ -134,9 +136,15 @@ template <int BM, int BN, class OFF> __device__ __forceinline__ bool find_rows(c
 }
 template <int BM, int BN, class OFF> __device__ __forceinline__ bool find_weights(const ExpertArgs &a, OFF off, long long q, Tile &t) {
     const long long per = (long long)a.mt * a.nt;
-    if (q >= per * a.n_exp) return false;
-    t.e = (int)(q / per);
-    rows_of(a, off, t.e, t.lo, t.cnt);
+    if (q >= per * a.n_exp * a.segs) return false;
+    t.e = (int)(q / per); /* its sums' place: behind those of the parts before */
+    const int seg = t.e / a.n_exp;
+    rows_of(a, off, t.e - seg * a.n_exp, t.lo, t.cnt);
+    if (a.segs > 1) {
+        const int part = ((t.cnt - 1) / a.segs & ~31) + 32, before = (int)min((long long)seg * part, (long long)t.cnt); /* whole steps */
+        t.lo += before;
+        t.cnt = min(part, t.cnt - before);
+    }
     place<BM, BN>(t, q - per * t.e, a.mt, a.nt);
     return true;
 }
@@ -485,6 +493,103 @@ template <Kind KIND, int YTY, int BM, int BN, int RING> __device__ __forceinline
     }
 }
 
+/* ---- few rows an expert ----
+ * y of at most 32 rows of an expert by 32 outputs, or a.strip times 32 one after the other, by one wave: nothing is shared, so there is no barrier,
+ * and a CU's four waves stream weights on their own. 256 bytes of a row of W at a time, since what comes from beyond the L2
+ * arrives the faster the longer its pieces are (64 bytes of each of many rows 4.4 TB/s, 128 5.3, 256 6.0); tiles begin at steps of
+ * their own, since rows lie a power of two apart as a rule and waves in the same place would ask the same channels (64 rows of 128 experts
+ * of 1536 x 2048 bf16 66 / 60 us). Of x only the rows that there are, in fours, so that the fewer they are, the more steps are on their way: 8 + X
+ * kB each. Where there are few tiles, a block's waves take steps in turn, and their sums meet in LDS. */
+constexpr int FEW_LDS = 40960; /* a wave's: the ring, then its results */
+template <int X> __device__ __forceinline__ void few_tile(const ExpertArgs &a, const Tile &t, LE_LDS char *lds, int wave, int nw) {
+    using O = Out<TY, 1, 16>;
+    constexpr int BKF = 256 / ES, STEP = (8 + X) * 1024, RING = (FEW_LDS - O::BYTES) / STEP;
+    const int l = threadIdx.x & 63, rows = t.cnt - t.m0, steps = (a.k + BKF - 1) / BKF, tiles = min(a.strip, (a.n - t.n0 + 31) / 32);
+    LE_LDS char *const mine = lds + wave * FEW_LDS;
+    auto row_of = [&](int j) { return 4 * j + (l >> 4); }; /* chunk j of x or W: four rows an instruction */
+    auto k_of = [&](int j) { return ((l & 15) ^ (row_of(j) & 15)) * EPC; };
+    const T *const w = (const T *)a.b + (long long)a.n * a.k * t.e;
+    unsigned long long xat[X], wat[8]; /* of this lane's chunks of a tile's step 0 */
+#pragma unroll
+    for (int j = 0; j < X; j++) xat[j] = (unsigned long long)((const T *)a.a + (long long)(t.lo + t.m0 + min(row_of(j), rows - 1)) * a.lda + k_of(j));
+    auto point = [&](int q) {
+#pragma unroll
+        for (int j = 0; j < 8; j++) wat[j] = (unsigned long long)(w + (long long)min(t.n0 + 32 * q + row_of(j), a.n - 1) * a.ldb + k_of(j));
+    };
+    auto begin = [&](int q) { return (t.n0 / 32 + q) % steps; };
+    int to = 0, asked = 0, next = wave, first = begin(0); /* tile and step to ask for */
+    point(0);
+    auto ask = [&] {
+        if (next >= steps && asked < tiles) {
+            next = wave;
+            if (++asked < tiles) point(asked), first = begin(asked);
+        }
+        const unsigned base = (unsigned)(unsigned long long)mine + to;
+        const int step = next + first >= steps ? next + first - steps : next + first, left = asked < tiles ? a.k - step * BKF : 0; /* 0: zeros */
+#pragma unroll
+        for (int j = 0; j < X; j++) chunk_to_lds(left >= BKF || k_of(j) < left ? xat[j] + step * 256LL : (unsigned long long)kZeros, base + j * 1024);
+#pragma unroll
+        for (int j = 0; j < 8; j++) chunk_to_lds(left >= BKF || k_of(j) < left ? wat[j] + step * 256LL : (unsigned long long)kZeros, base + (X + j) * 1024);
+        next += nw;
+        to = to == (RING - 1) * STEP ? 0 : to + STEP;
+    };
+#pragma unroll
+    for (int i = 0; i < RING - 1; i++) ask();
+    int slot = 0;
+    for (int q = 0; q < tiles; q++) {
+        v16f c[2];
+#pragma unroll
+        for (int j = 0; j < 16; j++) c[0][j] = 0.f, c[1][j] = 0.f;
+        for (int s = wave; s < steps; s += nw) {
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((RING - 2) * (8 + X)) : "memory");
+            ask();
+            LE_LDS const char *tx = mine + slot, *tw = tx + X * 1024;
+            slot = slot == (RING - 1) * STEP ? 0 : slot + STEP;
+#pragma unroll
+            for (int h = 0; h < 8; h++) { /* rows of x that are not there: the others once more */
+                const Frag fx = frag<false, 32, 256>(tx, 0, h, X == 8 ? l : (l & 32) | (l & (4 * X - 1))), fw = frag<false, 32, 256>(tw, 0, h, l);
+                c[h & 1] = mfma(fw, fx, c[h & 1]);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 16; j++) c[0][j] += c[1][j];
+        if (nw > 1) { /* one tile here; the waves' sums, in their order */
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory"); /* the ring is free */
+            if (wave)
+#pragma unroll
+                for (int j = 0; j < 4; j++) *(LE_LDS v4f *)(mine + (j * 64 + l) * 16) = v4f{c[0][4 * j], c[0][4 * j + 1], c[0][4 * j + 2], c[0][4 * j + 3]};
+            meet();
+            if (!wave)
+                for (int o = 1; o < nw; o++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        const v4f v = *(LE_LDS const v4f *)(lds + o * FEW_LDS + (j * 64 + l) * 16);
+#pragma unroll
+                        for (int e = 0; e < 4; e++) c[0][4 * j + e] += v[e];
+                    }
+        }
+        if (!wave)
+            O::put(mine + RING * STEP, c, (T *)a.y + (long long)(t.lo + t.m0) * a.ldy + t.n0 + 32 * q, a.ldy, rows, a.n - t.n0 - 32 * q);
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); /* nothing may land in LDS that is another tile's */
+}
+__device__ __forceinline__ void few_body(const ExpertArgs &a) {
+    extern __shared__ __attribute__((aligned(16))) char ring[];
+    LE_LDS char *const lds = (LE_LDS char *)ring;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), nw = blockDim.x >> 6;
+    for (long long b = blockIdx.x;; b += gridDim.x) {
+        Tile t;
+        if (!find<Y, 32, 1>(a, (const LE_GLOBAL int *)a.off, b, t)) return;
+        t.n0 *= 32 * a.strip;
+        const int rows = t.cnt - t.m0;
+        if (rows <= 4) few_tile<1>(a, t, lds, wave, nw);
+        else if (rows <= 8) few_tile<2>(a, t, lds, wave, nw);
+        else if (rows <= 16) few_tile<4>(a, t, lds, wave, nw);
+        else few_tile<8>(a, t, lds, wave, nw);
+        meet(); /* the reads of LDS */
+    }
+}
+
 /* ---- weights' gradient ----
  * An expert's rows make a short depth and a large result: 256 x 256 tiles by eight waves (2 x 4; a wave has every other 32 rows and 64 columns),
  * a block a CU, which takes tile after tile. What goes to LDS runs AHEAD steps ahead of what is multiplied, also from one tile into the
@@ -574,6 +679,16 @@ template <Kind KIND, int YTY, int RING> __device__ __forceinline__ void wide_bod
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); /* nothing may land in LDS that is no longer this block's */
 }
 
+/* ---- the sums of a weights' gradient's parts, in their order ---- */
+template <int YTY> __device__ __forceinline__ void sum_body(const float *parts, void *y, int n, int segs) {
+    const int i = blockIdx.x * 256 + threadIdx.x;
+    if (i >= n) return;
+    float v = 0.f;
+#pragma unroll 8
+    for (int s = 0; s < segs; s++) v += ((const LE_GLOBAL float *)parts)[(long long)s * n + i];
+    ((LE_GLOBAL typename XT<YTY>::raw *)y)[i] = XT<YTY>::down(v);
+}
+
 }  // namespace
 
 #define LE_EX_NAME2(WHAT, TY, TAIL) le_ex_##WHAT##_##TY##TAIL
@@ -587,10 +702,11 @@ template <Kind KIND, int YTY, int RING> __device__ __forceinline__ void wide_bod
     extern "C" __global__ void __launch_bounds__(256, 2) LE_EX_NAME(WHAT, LE_EX_TY, _m128_n256)(ExpertArgs a) { pipe_body<KIND, TY, 128, 256, 3>(a); }
 #define LE_EX_DW(WHAT, YTY)                                                                                                                 \
     LE_EX(WHAT, DW, YTY)                                                                                                                    \
-    extern "C" __global__ void __launch_bounds__(512) LE_EX_NAME(WHAT, LE_EX_TY, _m256_n256)(ExpertArgs a) { wide_body<DW, YTY, YTY == 0 ? 3 : 4>(a); }
+    extern "C" __global__ void __launch_bounds__(512) LE_EX_NAME(WHAT, LE_EX_TY, _m256_n256)(ExpertArgs a) { wide_body<DW, YTY, YTY == 0 ? 3 : 4>(a); }                             \
+    extern "C" __global__ void __launch_bounds__(256) LE_EX_NAME(WHAT, LE_EX_TY, _sum)(const float *parts, void *y, int n, int segs) { sum_body<YTY>(parts, y, n, segs); }
 LE_EX_ROWS(y, Y)
 LE_EX_ROWS(dx, DX)
-extern "C" __global__ void __launch_bounds__(256) LE_EX_NAME(y, LE_EX_TY, _m64_n128)(ExpertArgs a) { pipe_body<Y, TY, 64, 128, 4>(a); }
+extern "C" __global__ void __launch_bounds__(256, 1) LE_EX_NAME(y, LE_EX_TY, _few)(ExpertArgs a) { few_body(a); }
 LE_EX_DW(dw, TY)
 #if LE_EX_TY != 0
 LE_EX_DW(dwf, 0)

@@ -8,6 +8,7 @@
 
 namespace {
 
+constexpr int kFew = 256; /* tokens, for their own form of the second product */
 constexpr int kRank = 256, kSide = 1 << 24, kTokens = 16 * 65535;
 
 const char *shape_error(const le_adapters *ad, int m) {
@@ -23,14 +24,20 @@ struct Shape {
     size_t wave_lds;
     Shape(const le_adapters *ad, int xtype, int m) {
         tiles = (m + 15) / 16;
-        /* blocks that share a tile's adapters: one each while there are few tiles */
-        turns = m <= 64 ? std::min(m, 16) : 1;
-        sets = ad->rank <= 16 ? 1 : ad->rank <= 32 ? 2 : 4; /* of 16 rows of A at once */
-        /* the columns' steps of 64 over a block's waves (as many as leave LDS for two blocks), and over segments while that makes no more than 2048 waves */
+        /* blocks that share a tile's adapters: one each while there are few tiles (65 tokens with an adapter each 9 us, a block a tile 36); with
+         * many, two, since most tiles have one or two (4096 tokens of 4096 values in runs of 456, rank 64: one 51, two 34, four 33 us) */
+        turns = tiles <= 32 ? std::min(m, 16) : tiles <= 64 ? 4 : 2;
+        sets = ad->rank <= 16 ? 1 : ad->rank <= 32 || ad->ltype == LE_F32 ? 2 : 4; /* of 16 rows of A at once */
+        /* the columns' steps of 64 over a block's waves: eight, or as many as leave LDS for two blocks; four where every CU has a tile anyway (4 / 8
+         * waves, 4096 tokens in runs of 456: fp32 34 / 40 us, bf16 23 / 26, 16384 of 1024 columns 14 / 18; 2048 tokens: 61 / 45). And over segments
+         * while that makes no more than 2048 waves: up to eight for few tokens, each with an adapter of its own; for many, whose sums each of the second
+         * kernel's row blocks reads again, two up to 1024 waves (1 / 2 / 4 segments, both kernels: 300 tokens 30 / 27 / 29 us, 1024 35 / 32 / 39,
+         * 2048 45 / 53 / 54). */
         const int all = (ad->cols + 63) / 64;
         wave_lds = le_type_bytes(xtype) * 1024 + 256 + sets * (le_type_bytes(ad->ltype) * 1024 + 256);
-        waves = std::min(std::min(8, (int)(80 * 1024 / wave_lds)), all);
-        segs = std::max(1, std::min(std::min(8, 2048 / (tiles * std::min(m, 16) * waves)), all / waves));
+        waves = std::min(std::min(tiles < 256 ? 8 : 4, (int)(80 * 1024 / wave_lds)), all);
+        segs = m <= kFew ? std::min(8, 2048 / (tiles * turns * waves)) : std::min(2, 1024 / (tiles * waves));
+        segs = std::max(1, std::min(segs, all / waves));
         steps = (all + segs - 1) / segs;
         segs = (all + steps - 1) / steps;
     }
@@ -73,12 +80,14 @@ extern "C" int le_lora(le_ctx *c, const le_adapters *ad, const int *idx, int xty
                                sh.waves * std::max(sh.wave_lds, (size_t)sh.sets * 1024), (hipStream_t)stream, args))
         return rc;
     const unsigned blocks = (unsigned)((ad->rows + 255) / 256);
-    if (m <= 64) {
+    /* many tokens: a matrix instruction's 16 tokens at once, which pays where they have one adapter (4096 x 4096, rank 64 bf16, few / many form: 256
+     * tokens in runs of 100 22 / 11 us, of 8 19 / 20, of one 45 / 84; 512 tokens 40 / 12, 31 / 21, 67 / 88) */
+    if (m <= kFew) {
         int G = 1; /* lanes a row of B */
         while (8 * G < ad->rank) G *= 2;
         snprintf(name, sizeof name, "le_lo_upv%d_%d_%d", G, xtype, ad->ltype);
         return le_ctx_launch(c, name, dim3(std::min(blocks, (unsigned)std::max(1, 2048 / (sh.tiles * sh.turns))), (unsigned)sh.tiles, (unsigned)sh.turns), 256, 0, (hipStream_t)stream, args);
     }
-    snprintf(name, sizeof name, "le_lo_upm%d_%d_%d", ad->rank <= 32 ? 1 : ad->rank <= 64 ? 2 : 0, xtype, ad->ltype);
+    snprintf(name, sizeof name, "le_lo_upm%d_%d_%d", ad->rank % 8 || ad->rank > 64 ? 0 : ad->rank <= 32 ? 1 : 2, xtype, ad->ltype);
     return le_ctx_launch(c, name, dim3(blocks, (unsigned)((sh.tiles + 3) / 4)), 256, 0, (hipStream_t)stream, args);
 }

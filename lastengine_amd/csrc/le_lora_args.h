@@ -10,5 +10,5 @@ struct LoraArgs {
     float *u;             /* [segment][token][rank]: A x over a segment of the columns */
     long long ldx, ldb, ldy;
     int n_ad, rank, rows, cols, m;
-    int segs, steps;      /* segments of cols, and the 32-column steps of each */
+    int segs, steps; /* segments of cols, the 64-column steps of each */
 };

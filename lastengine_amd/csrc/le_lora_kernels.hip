@@ -63,6 +63,24 @@ template <int TY> __device__ __forceinline__ Eight<TY> load8(const void *base, l
     return r;
 }
 
+/* The eight values from p on, or zeros. */
+template <int TY> __device__ __forceinline__ Eight<TY> whole8(const void *base, long long at, bool there) {
+    using T = typename XT<TY>::raw;
+    const LE_GLOBAL T *p = (const LE_GLOBAL T *)base + at;
+    v4u lo = {0, 0, 0, 0}, hi = {0, 0, 0, 0};
+    if (there) {
+        lo = *(const LE_GLOBAL typename Any<sizeof(T)>::v *)p;
+        if constexpr (TY == 0) hi = *(const LE_GLOBAL typename Any<sizeof(T)>::v *)(p + 4);
+    }
+    Eight<TY> r;
+    if constexpr (TY == 0) {
+        *(v4u *)&r.v[0] = lo;
+        *(v4u *)&r.v[4] = hi;
+    } else {
+        r.v = lo;
+    }
+    return r;
+}
 /* Value e of a 16-byte piece, and word d of the piece of values v. */
 template <int TY> __device__ __forceinline__ float unpack(v4u v, int e) {
     const unsigned word = v[TY == 0 ? e : e >> 1];
@@ -211,7 +229,8 @@ template <int WTY, int RF> __device__ __forceinline__ void down_body(const LoraA
     using XR = Rows<XTY>;
     using WR = Rows<WTY>;
     extern __shared__ __attribute__((aligned(16))) char lds[]; /* each wave's rows, then its sums: [wave][RF][256] */
-    const int l = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), nw = blockDim.x >> 6, t0 = blockIdx.x * 16;
+    const int l = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), nw = blockDim.x >> 6;
+    const int tile = blockIdx.x, turn = blockIdx.y, turns = gridDim.y, t0 = tile * 16;
     char *mine = lds + wave * (XR::BYTES + RF * WR::BYTES);
     Tile t(adapter(a, t0 + (l & 15)));
     const int s0 = blockIdx.z * a.steps + wave, s1 = min((int)(blockIdx.z + 1) * a.steps, (a.cols + 63) / 64);
@@ -219,7 +238,7 @@ template <int WTY, int RF> __device__ __forceinline__ void down_body(const LoraA
 #pragma unroll
     for (int n = 0; n < XR::N; n++) xrow[n] = min(t0 + XR::row_of(n), a.m - 1) * a.ldx;
     for (int nth = 0; t.next(); nth++) {
-        if (nth % gridDim.y != blockIdx.y) continue;
+        if (nth % turns != turn) continue;
         for (int j0 = 0; j0 < a.rank; j0 += 16 * RF) {
             v4f c[RF];
             long long arow[RF][WR::N];
@@ -271,8 +290,8 @@ template <int WTY, int RF> __device__ __forceinline__ void down_body(const LoraA
                 if (j < ((a.rank + 31) & ~31) && (t.members >> row & 1)) {
                     float v = sums[id];
                     for (int n = 1; n < nw; n++) v += sums[n * RF * 256 + id];
-                    ((LE_GLOBAL float *)a.u)[place(a, blockIdx.z, blockIdx.x, row, j)] = j < a.rank ? v : 0.f;
-                    if (RF == 1) ((LE_GLOBAL float *)a.u)[place(a, blockIdx.z, blockIdx.x, row, j + 16)] = 0.f; /* rank <= 16 here */
+                    ((LE_GLOBAL float *)a.u)[place(a, blockIdx.z, tile, row, j)] = j < a.rank ? v : 0.f;
+                    if (RF == 1) ((LE_GLOBAL float *)a.u)[place(a, blockIdx.z, tile, row, j + 16)] = 0.f; /* rank <= 16 here */
                 }
             }
             __syncthreads();
@@ -392,8 +411,8 @@ template <int WTY, int G> __device__ __forceinline__ void upv_body(const LoraArg
 
 /* ---- up, many tokens ----
  * A wave 64 output rows by up to 64 tokens, 16 at a time. A matrix instruction leaves four rows of 16 tokens in a lane; they change places through LDS, so
- * that base is read and y written in whole rows of 64 (128 or 256 bytes). B stays in registers while the adapter does, up to a rank of
- * 32 J (J = 0: read for each tile). */
+ * that base is read and y written in whole rows of 64 (128 or 256 bytes). B stays in registers while the adapter does, for ranks that are
+ * multiples of 8 up to 32 J (J = 0, any other rank: read for each tile). */
 template <int WTY, int J> __device__ __forceinline__ void upm_body(const LoraArgs &a) {
     using v4u_any = Any<sizeof(X)>::v;
     using Mul = Pair<WTY, 0>;
@@ -410,8 +429,11 @@ template <int WTY, int J> __device__ __forceinline__ void upm_body(const LoraArg
     typename Mul::A w[J > 0 ? J : 1][4];
     auto get = [&](int ad, int j, typename Mul::A *q) {
 #pragma unroll
-        for (int f = 0; f < 4; f++)
-            q[f].set(load8<WTY>(a.b, ((long long)ad * a.rows + min(r0 + 16 * f + c16, a.rows - 1)) * a.rank + j + 8 * g, a.rank - j - 8 * g));
+        for (int f = 0; f < 4; f++) {
+            const long long at = ((long long)ad * a.rows + min(r0 + 16 * f + c16, a.rows - 1)) * a.rank + j + 8 * g;
+            if constexpr (J == 0) q[f].set(load8<WTY>(a.b, at, a.rank - j - 8 * g));
+            else q[f].set(whole8<WTY>(a.b, at, j + 8 * g < a.rank));
+        }
     };
 #pragma unroll
     for (int n = 0; n < 4; n++) {

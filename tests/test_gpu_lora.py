@@ -82,7 +82,7 @@ class Case:
 @pytest.mark.parametrize("wty", TYPES)
 @pytest.mark.parametrize("m,rows,cols,rank,n_ad,each", [
     (1, 256, 512, 16, 3, 1), (1, 1, 1, 1, 1, 1), (2, 33, 77, 5, 2, 1), (15, 200, 264, 12, 6, 5), (61, 520, 256, 16, 40, 1), (64, 64, 1032, 64, 4, 16), (70, 130, 96, 100, 3, 35),
-    (200, 96, 160, 8, 9, 1), (300, 264, 320, 32, 5, 70), (129, 72, 40, 256, 2, 64), (40, 50, 515, 31, 7, 3), (513, 140, 136, 4, 70, 2)])
+    (200, 96, 160, 8, 9, 1), (300, 264, 320, 32, 5, 70), (129, 72, 40, 256, 2, 64), (40, 50, 515, 31, 7, 3), (513, 140, 136, 4, 70, 2), (300, 264, 320, 64, 5, 40), (257, 130, 96, 100, 3, 35), (700, 200, 72, 24, 6, 1)])
 def test_whole_numbers(engine, xty, wty, m, rows, cols, rank, n_ad, each):
     c = Case(xty, wty, m, rows, cols, rank, n_ad, 1, each=each)
     c.run(engine)
@@ -90,7 +90,7 @@ def test_whole_numbers(engine, xty, wty, m, rows, cols, rank, n_ad, each):
 
 
 @pytest.mark.parametrize("xty", TYPES)
-@pytest.mark.parametrize("m", [1, 9, 100])
+@pytest.mark.parametrize("m", [1, 9, 100, 300])
 @pytest.mark.parametrize("kw", [dict(gap=8), dict(gap=3), dict(at=1), dict(gap=16, at=8), dict(base=False), dict(shared=True), dict(scale=False), dict(bare=1.0), dict(bare=0.0, each=1000)])
 def test_forms(engine, xty, m, kw):
     """Rows apart and at odd addresses, no base, one row of x for all, no factors, no token or every token of one adapter."""
@@ -101,7 +101,7 @@ def test_forms(engine, xty, m, kw):
 
 
 @pytest.mark.parametrize("xty", TYPES)
-@pytest.mark.parametrize("m", [1, 20, 90])
+@pytest.mark.parametrize("m", [1, 20, 90, 261])
 def test_in_place(engine, xty, m):
     c = Case(xty, xty, m, 200, 128, 8, 3, 3)
     c.run(engine, in_place=True)
@@ -125,7 +125,7 @@ def test_long_rows(engine):
 
 
 @pytest.mark.parametrize("xty", TYPES)
-@pytest.mark.parametrize("m", [3, 50, 140])
+@pytest.mark.parametrize("m", [3, 50, 140, 270])
 def test_what_is_not_finite_stays_with_its_token(engine, xty, m):
     """NaN in one adapter and infinity in one row of x: no token but theirs is touched, in a batch where the adapters alternate."""
     import torch
@@ -145,7 +145,7 @@ def test_what_is_not_finite_stays_with_its_token(engine, xty, m):
         assert not torch.isfinite(got[t]).any() if t % 3 == 1 else torch.equal(got[t], want[t]), t
 
 
-@pytest.mark.parametrize("m", [4, 80])
+@pytest.mark.parametrize("m", [4, 80, 260])
 def test_numbers_of_no_adapter(engine, m):
     import torch
     c = Case(le.F32, le.F16, m, 64, 128, 8, 3, 7)
@@ -173,7 +173,7 @@ def test_far_rows(engine):
     assert torch.equal(big[1].cpu(), want.bfloat16())
 
 
-@pytest.mark.parametrize("m", [1, 30, 150])
+@pytest.mark.parametrize("m", [1, 30, 150, 400])
 def test_same_bits_whatever_the_workspace_held(engine, m):
     import torch
     c = Case(le.F32, le.BF16, m, 300, 2048, 16, 5, 9, make=real)
