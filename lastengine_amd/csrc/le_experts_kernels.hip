@@ -107,12 +107,10 @@ template <int BM, int BN> __device__ __forceinline__ void place(Tile &t, long lo
 /* Tile t of an expert's rows by outputs; every wave finds it by itself, 64 experts a turn. False: behind the last. */
 template <int BM, int BN, class OFF> __device__ __forceinline__ bool find_rows(const ExpertArgs &a, OFF off, long long q, Tile &t) {
     const int l = threadIdx.x & 63, u = (int)(q / a.nt); /* row tiles before this one, over all experts */
-    int before = 0, lo1 = 0, cnt1 = 0;
-    if (l < a.n_exp) rows_of(a, off, l, lo1, cnt1);
+    int before = 0;
     for (int e0 = 0; e0 < a.n_exp; e0 += 64) {
-        const int lo = lo1, cnt = cnt1;
-        lo1 = cnt1 = 0;
-        if (e0 + 64 + l < a.n_exp) rows_of(a, off, e0 + 64 + l, lo1, cnt1); /* the next turn's meanwhile */
+        int lo = 0, cnt = 0;
+        if (e0 + l < a.n_exp) rows_of(a, off, e0 + l, lo, cnt);
         const int mine = (int)(((long long)cnt + BM - 1) / BM);
         int sum = mine;
 #pragma unroll
