@@ -30,25 +30,38 @@ int parts(int n_exp, int n_row, int rows, int cols) {
     return (int)std::max(1LL, std::min({2 * kCus / tiles, n_row / (256LL * n_exp), 64LL}));
 }
 
+/* Whether y is taken by a wave a tile: few rows an expert, fewer where a wave's work on them is short (us, so / in tiles of 128 x 256, 128 experts
+ * bf16: 1536 x 2048 64 rows 60 / 83, 128 rows 90 / 106, 512 rows 131 / 150; 2048 x 768 64 rows 33 / 37, 256 rows 67 / 62). */
+bool few_rows(const ExpertArgs &a, int ty, const char *what) {
+    return what[0] == 'y' && a.n_row < (a.k * (long long)le_type_bytes(ty) < 4096 ? 2LL : 4LL) * a.n_exp;
+}
+
 /* The kernel of `what`_type. whole: every row that is read is whole 16-byte chunks. */
 int launch(le_ctx *c, const char *what, int ty, ExpertArgs &a, bool whole, le_stream_t stream) {
     const bool dw = what[1] == 'w';
-    int bm = 128, bn = 128, ring = 3;
-    if (!whole) {
-        /* rows through registers: tiles of 32 rows for few rows an expert */
-        if (!dw ? a.n_row < 48LL * a.n_exp : a.m <= 32) bm = 32;
-    } else if (what[0] == 'y' && a.n_row < (a.k * (long long)le_type_bytes(ty) < 4096 ? 2LL : 4LL) * a.n_exp) {
-        /* few rows an expert, fewer where a wave's work on them is short (us, few / in tiles of 128 x 256, 128 experts bf16: 1536 x 2048 64 rows
-         * 60 / 83, 128 rows 90 / 106, 512 rows 131 / 150; 2048 x 768 64 rows 33 / 37, 256 rows 67 / 62) */
+    int bm = 128, bn = 128;
+    /* tiles of 128 x 128 and of 128 x 256 that there may be (times below: of this choice / of the other) */
+    const bool f32 = ty == LE_F32;
+    const long long row_tiles = a.n_row / 128 + std::min(a.n_exp, a.n_row), t128 = row_tiles * ((a.n + 127LL) / 128), t256 = row_tiles * ((a.n + 255LL) / 256);
+    if (!dw && (whole ? f32 && t128 <= 512 && !few_rows(a, ty, what) : a.n_row < 48LL * a.n_exp || t128 < 256 || (f32 && t128 < 2048))) {
+        /* tiles of 32 rows through registers for few rows an expert, or where larger tiles are too few (256 rows of 4 experts of 4096 x 4096
+         * bf16 43 / 56 us); fp32 is bound by the matrix instructions, which more waves keep busier (1351 rows of 7 experts of 1951 x 1024:
+         * dx 90 / 156, of 1952 x 1024 73 / 81; 16384 rows of 16 of 2048 x 1024 720 / 654) */
+        bm = 32;
+        whole = false;
+    } else if (!whole) {
+        if (dw && a.m <= 32) bm = 32;
+    } else if (few_rows(a, ty, what)) {
         bm = bn = 32;
-    } else if (a.n > 128) {
+    } else if (dw) {
+        /* a block a CU takes tile after tile of 256 x 256: not where CUs would stand idle for more than a fifth of the time (16384 rows of 8
+         * experts of 1024 x 1024 bf16 69 / 47 us, 8192 of one of 4096 x 4096 264 / 310) */
+        const long long wide = (a.m + 255LL) / 256 * ((a.n + 255LL) / 256) * a.n_exp, turns = (wide + kCus - 1) / kCus;
+        if (a.n > 128 && 5 * wide >= 4 * turns * kCus) bm = bn = 256;
+    } else if (!f32 && a.n > 128 && t256 >= 512) {
+        /* two blocks a CU (16384 rows of 8 experts of 1024 x 1024 bf16 45 / 63 us, 8192 39 / 38, 2048 23 / 17); not fp32 (32768 rows of 128 of
+         * 1536 x 2048 2198 / 2105) */
         bn = 256;
-        if (dw) {
-            /* a block a CU takes tile after tile of 256 x 256: not where CUs would stand idle for more than a fifth of the time */
-            const long long wide = (a.m + 255LL) / 256 * ((a.n + 255LL) / 256) * a.n_exp, turns = (wide + kCus - 1) / kCus;
-            if (5 * wide >= 4 * turns * kCus) bm = 256;
-            else bn = 128;
-        }
     }
     const bool few = bn == 32;
     int waves = 4;
@@ -72,8 +85,8 @@ int launch(le_ctx *c, const char *what, int ty, ExpertArgs &a, bool whole, le_st
     void *args[] = {&a};
     if (bm == 256) {
         /* a block a CU; the ring (three steps for fp32 results, whose rows take more of LDS, else four), the results of eight waves, off */
-        const bool f32 = ty == LE_F32 || what[2] == 'f';
-        const size_t lds = (size_t)(f32 ? 3 : 4) * 512 * 64 + 8 * 16 * (64 * (f32 ? 4 : 2) + 16) + (size_t)(a.n_exp + 1) * 4;
+        const bool wide32 = f32 || what[2] == 'f';
+        const size_t lds = (size_t)(wide32 ? 3 : 4) * 512 * 64 + 8 * 16 * (64 * (wide32 ? 4 : 2) + 16) + (size_t)(a.n_exp + 1) * 4;
         const int cus = std::max(8, le_ctx_cus(c));
         for (a.run = 1; a.run * 2 <= tiles / 8 && cus / 8 % (a.run * 2) == 0;) a.run *= 2;
         return le_ctx_launch(c, name, dim3((unsigned)(cus / (8 * a.run) * (8 * a.run))), 512, lds, (hipStream_t)stream, args);
@@ -81,7 +94,7 @@ int launch(le_ctx *c, const char *what, int ty, ExpertArgs &a, bool whole, le_st
     /* tiles in whole turns of the eight XCDs, `run` in a row to each: an expert's, which share weights (18 in a row 351 us, 4 373, single ones 414) */
     a.run = (int)std::max(1LL, std::min({tiles / (a.n_exp * (long long)a.segs), tiles / 64, 1LL << 16}));
     const long long turn = 8LL * a.run;
-    return le_ctx_launch(c, name, dim3((unsigned)std::min((tiles + turn - 1) / turn * turn, (1LL << 23) / turn * turn)), 64 * waves, few ? waves * 40960 : whole ? (size_t)ring * (bm + bn) * 64 : 0,
+    return le_ctx_launch(c, name, dim3((unsigned)std::min((tiles + turn - 1) / turn * turn, (1LL << 23) / turn * turn)), 64 * waves, few ? waves * 40960 : whole ? 3 * (bm + bn) * 64 : 0,
                          (hipStream_t)stream, args);
 }
 /* Whether rows of `rows` and `cols` values, ld1 and ld2 apart, are whole 16-byte chunks. */

@@ -695,17 +695,18 @@ template <int YTY> __device__ __forceinline__ void sum_body(const float *parts, 
     extern "C" __global__ void __launch_bounds__(256) LE_EX_NAME(WHAT, LE_EX_TY, _any32)(ExpertArgs a) { any_body<KIND, YTY, 32>(a); }   \
     extern "C" __global__ void __launch_bounds__(256, 2) LE_EX_NAME(WHAT, LE_EX_TY, _any128)(ExpertArgs a) { any_body<KIND, YTY, 128>(a); } \
     extern "C" __global__ void __launch_bounds__(256, 2) LE_EX_NAME(WHAT, LE_EX_TY, _m128_n128)(ExpertArgs a) { pipe_body<KIND, YTY, 128, 128, 3>(a); }
-#define LE_EX_ROWS(WHAT, KIND)                                                                                                              \
-    LE_EX(WHAT, KIND, TY)                                                                                                                   \
+#define LE_EX_ROWS(WHAT, KIND) \
     extern "C" __global__ void __launch_bounds__(256, 2) LE_EX_NAME(WHAT, LE_EX_TY, _m128_n256)(ExpertArgs a) { pipe_body<KIND, TY, 128, 256, 3>(a); }
 #define LE_EX_DW(WHAT, YTY)                                                                                                                 \
     LE_EX(WHAT, DW, YTY)                                                                                                                    \
     extern "C" __global__ void __launch_bounds__(512) LE_EX_NAME(WHAT, LE_EX_TY, _m256_n256)(ExpertArgs a) { wide_body<DW, YTY, YTY == 0 ? 3 : 4>(a); }                             \
     extern "C" __global__ void __launch_bounds__(256) LE_EX_NAME(WHAT, LE_EX_TY, _sum)(const float *parts, void *y, int n, int segs) { sum_body<YTY>(parts, y, n, segs); }
-LE_EX_ROWS(y, Y)
-LE_EX_ROWS(dx, DX)
+LE_EX(y, Y, TY)
+LE_EX(dx, DX, TY)
 extern "C" __global__ void __launch_bounds__(256, 1) LE_EX_NAME(y, LE_EX_TY, _few)(ExpertArgs a) { few_body(a); }
 LE_EX_DW(dw, TY)
 #if LE_EX_TY != 0
+LE_EX_ROWS(y, Y)
+LE_EX_ROWS(dx, DX)
 LE_EX_DW(dwf, 0)
 #endif

@@ -95,7 +95,7 @@ template <int TY> __device__ __forceinline__ unsigned pack(const float *v, int d
 /* ---- products ----
  * An operand of a matrix instruction over 32 of k: 16 rows, a lane's row l % 16 and its eight k from 8 (l / 16) on. Two operands of one 16-bit
  * type multiply as they are. Otherwise values are cut into bf16 pieces that add up to them exactly (fp16: 2 of 8 bits or less, fp32: 3 of 8,
- * cut off, not rounded) and every piece of one multiplies every piece of the other: five to two times faster than fp32 instructions, which are left for two
+ * cut off, not rounded) and every piece of one multiplies every piece of the other: two to five times faster than fp32 instructions, which are left for two
  * fp32 operands. Either way the products are exact (fp32: a fused multiply-add's) and the sums fp32. */
 template <int TY, bool CUT> struct Operand;
 template <int TY> struct Operand<TY, false> {

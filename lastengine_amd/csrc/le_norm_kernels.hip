@@ -175,7 +175,7 @@ template <int TY, int L> __device__ __forceinline__ void any_body(const NormArgs
 #define LE_NQ(TY, L, NC) \
     extern "C" __global__ void __launch_bounds__(L == 64 ? 256 : L) le_nq_##TY##_l##L##_c##NC(NormArgs a) { norm_body<TY, L, NC>(a); }
 #define LE_NQ_ALL(TY)                                                                                             \
-    LE_NQ(TY, 64, 1) LE_NQ(TY, 64, 2) LE_NQ(TY, 64, 4) LE_NQ(TY, 256, 1) LE_NQ(TY, 256, 2) LE_NQ(TY, 256, 4)      \
+    LE_NQ(TY, 64, 1) LE_NQ(TY, 64, 2) LE_NQ(TY, 256, 1) LE_NQ(TY, 256, 2) LE_NQ(TY, 256, 4)                        \
     LE_NQ(TY, 1024, 1) LE_NQ(TY, 1024, 2) LE_NQ(TY, 1024, 4)                                                      \
     extern "C" __global__ void __launch_bounds__(256) le_nq_##TY##_any256(NormArgs a) { any_body<TY, 256>(a); }   \
     extern "C" __global__ void __launch_bounds__(1024) le_nq_##TY##_any1024(NormArgs a) { any_body<TY, 1024>(a); }

@@ -118,7 +118,9 @@ SHAPES = [([1], 1, 1), ([1], 64, 64), ([0, 2, 0, 5, 0], 7, 5), ([3, 0, 1, 40], 3
           ([0, 0], 40, 24), ([5, 9, 7], 512, 1024), ([1] * 70, 48, 96), ([17] * 9, 264, 520), ([700], 256, 384), ([2500], 24, 40),
           ([1, 0, 3, 2, 0, 0, 1, 0], 264, 136), ([1, 1, 0, 0, 2], 1000, 520), ([130, 0, 5, 64, 33, 1, 0, 2], 1000, 4088), ([40, 300] * 8, 1016, 1000),
           ([3000, 0, 1], 130, 264), ([1, 0, 2000, 63], 33, 515), ([9000], 129, 130),
-          ([1] * 70, 1000, 136), ([2, 0, 1, 0] * 32, 2100, 72), ([6, 12, 31, 40] + [0] * 50, 200, 264), ([3, 20, 0, 7] + [0] * 20, 40, 2056)]
+          ([1] * 70, 1000, 136), ([2, 0, 1, 0] * 32, 2100, 72), ([6, 12, 31, 40] + [0] * 50, 200, 264), ([3, 20, 0, 7] + [0] * 20, 40, 2056),
+          ([5] * 63 + [160], 2056, 72), ([1, 9] * 31 + [140], 40, 2064), ([400, 410, 0, 500], 2049, 41), ([400, 410, 0, 500], 41, 2049), ([49] * 88, 2049, 41),
+          ([49] * 87 + [80], 41, 2049)]
 
 
 @pytest.mark.parametrize("ty", TYPES)
