@@ -27,7 +27,8 @@ struct Shape {
         /* blocks that share a tile's adapters: one each while there are few tiles (65 tokens with an adapter each 9 us, a block a tile 36); with
          * many, two, since most tiles have one or two (4096 tokens of 4096 values in runs of 456, rank 64: one 51, two 34, four 33 us) */
         turns = tiles <= 32 ? std::min(m, 16) : tiles <= 64 ? 4 : 2;
-        sets = ad->rank <= 16 ? 1 : ad->rank <= 32 || ad->ltype == LE_F32 ? 2 : 4; /* of 16 rows of A at once */
+        /* of 16 rows of A at once (rank 64, two / four: 4096 tokens bf16 31 / 23 us, 64 tokens 7 / 6, fp32 17 / 13) */
+        sets = ad->rank <= 16 ? 1 : ad->rank <= 32 ? 2 : 4;
         /* the columns' steps of 64 over a block's waves: eight, or as many as leave LDS for two blocks; four where every CU has a tile anyway (4 / 8
          * waves, 4096 tokens in runs of 456: fp32 34 / 40 us, bf16 23 / 26, 16384 of 1024 columns 14 / 18; 2048 tokens: 61 / 45). And over segments
          * while that makes no more than 2048 waves: up to eight for few tokens, each with an adapter of its own; for many, whose sums each of the second

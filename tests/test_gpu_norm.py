@@ -92,6 +92,14 @@ def test_bits(engine, ty, m, n, res):
 
 
 @pytest.mark.parametrize("ty", TYPES)
+@pytest.mark.parametrize("m,n", [(1100, 384), (1100, 544), (300, 1536), (300, 2080), (300, 4128), (3, 8224), (2, 12320)])
+def test_bits_of_every_shape_of_row(engine, ty, m, n):
+    c = Case(ty, m, n, 7, xs=False)
+    c.run(engine)
+    c.check()
+
+
+@pytest.mark.parametrize("ty", TYPES)
 @pytest.mark.parametrize("gap,at", [(8, 0), (3, 0), (0, 1), (32, 8), (5, 3)])
 @pytest.mark.parametrize("n", [64, 2080])
 def test_strides_and_alignment(engine, ty, gap, at, n):
