@@ -161,8 +161,10 @@ template <Kind KIND, int BM, int BN, class OFF> __device__ __forceinline__ bool 
 template <int YTY, int NF, int ROWS = 32> struct Out {
     using U = typename XT<YTY>::raw;
     static constexpr int E = 16 / sizeof(U), LANES = 32 * NF / E, PITCH = 32 * NF * sizeof(U) + 16, BYTES = ROWS * PITCH;
-    /* rows of them there are, at y, ld apart; cols of them there are, from this wave's first on */
-    static __device__ __forceinline__ void put(LE_LDS char *mine, const v16f *c, void *y, long long ld, int rows, int cols) {
+    static constexpr int STORES = 32 * LANES / 64; /* instructions of a put */
+    /* rows of them there are, at y, ld apart; cols of them there are, from this wave's first on. ALL: all 32 and 32 NF, in exactly STORES
+     * instructions (in assembly, as they are counted on). */
+    template <bool ALL = false> static __device__ __forceinline__ void put(LE_LDS char *mine, const v16f *c, void *y, long long ld, int rows, int cols) {
         typedef v4u __attribute__((aligned(4))) v4u_a4;
         typedef v4u __attribute__((aligned(2))) v4u_a2;
         const int l = threadIdx.x & 63, col = l % LANES * E;
@@ -192,7 +194,9 @@ template <int YTY, int NF, int ROWS = 32> struct Out {
             const int r = r0 + i + l / LANES;
             const v4u v = *(LE_LDS const v4u *)(mine + (r - r0) * PITCH + col * (int)sizeof(U));
             LE_GLOBAL U *to = (LE_GLOBAL U *)y + r * ld + col;
-            if (r < rows) {
+            if constexpr (ALL) {
+                asm volatile("global_store_dwordx4 %0, %1, off" ::"v"((unsigned long long)to), "v"(v) : "memory");
+            } else if (r < rows) {
                 if (col + E <= cols) {
                     if constexpr (sizeof(U) == 4) *(LE_GLOBAL v4u_a4 *)to = v;
                     else *(LE_GLOBAL v4u_a2 *)to = v;
@@ -592,8 +596,10 @@ __device__ __forceinline__ void few_body(const ExpertArgs &a) {
  * An expert's rows make a short depth and a large result: 256 x 256 tiles by eight waves (2 x 4; a wave has every other 32 rows and 64 columns),
  * a block a CU, which takes tile after tile. What goes to LDS runs AHEAD steps ahead of what is multiplied, also from one tile into the
  * next, so that nothing waits for a tile's first chunks and the results leave meanwhile. off lies in LDS, since a wait for a load from
- * memory would be one for the chunks as well. 128 experts of 1536 x 2048 bf16, 32768 rows: 345 us, in the tiles above 404; 8168 rows
- * of 2048 x 768 fp16 117 / 129. (The other two products gain nothing: 318 / 312 and 279 / 275.) */
+ * memory would be one for the chunks as well. 128 experts of 1536 x 2048 bf16, 32768 rows: 350 us (while the first steps waited for the stores
+ * before them 357), in the tiles above 404; 8168 rows of 2048 x 768 fp16 115 / 129. Without its stores it takes 262, without the
+ * matrix instructions 307, without both 144: loads and stores (1.16 GB, at a copy's rate 223) overlap in part only, since a tile's stores are
+ * waited for AHEAD steps later, and LDS holds no longer ring. (The other two products gain nothing: 318 / 312 and 279 / 275.) */
 template <Kind KIND, int YTY, int RING> __device__ __forceinline__ void wide_body(const ExpertArgs &a) {
     constexpr int BM = 256, BN = 256, NT = 512, STEP = (BM + BN) * 64, CHUNKS = (BM + BN) * 4 / NT, AHEAD = RING - 1;
     constexpr bool AD = KIND == DW, BD = KIND != Y;
@@ -628,7 +634,7 @@ template <Kind KIND, int YTY, int RING> __device__ __forceinline__ void wide_bod
     };
 #pragma unroll
     for (int i = 0; i < AHEAD; i++) ask();
-    int slot = 0;
+    int slot = 0, late = 0; /* steps to come that were asked for before a tile's results left */
     for (long long b = blockIdx.x;; b += gridDim.x) {
         Tile t;
         if (!find<KIND, BM, BN>(a, off, b, t)) break;
@@ -643,7 +649,8 @@ template <Kind KIND, int YTY, int RING> __device__ __forceinline__ void wide_bod
                 for (int j = 0; j < 16; j++) c[i][n][j] = 0.f;
         auto steps = [&](auto full) {
             for (int s = 0; s < depth; s += BK) {
-                step_ready<(AHEAD - 1) * CHUNKS>();
+                if (late > 0) step_ready<(AHEAD - 1) * CHUNKS + 4 * O::STORES>(), late--;
+                else step_ready<(AHEAD - 1) * CHUNKS>();
                 ask();
                 LE_LDS const char *ta = lds + slot, *tb = ta + BM * 64;
                 slot = slot == (RING - 1) * STEP ? 0 : slot + STEP;
@@ -669,10 +676,18 @@ template <Kind KIND, int YTY, int RING> __device__ __forceinline__ void wide_bod
         if (f == 4) steps(Count<1>());
         else steps(Count<0>());
         const long long row0 = (KIND == DW ? (long long)t.e * a.m : t.lo) + t.m0 + 32 * wm;
+        typename XT<YTY>::raw *const y = (typename XT<YTY>::raw *)a.y + row0 * a.ldy + t.n0 + wn;
+        LE_LDS char *const mine = lds + RING * STEP + wave * O::BYTES;
+        if (rows >= BM && cols >= BN) { /* the AHEAD steps that come next do not wait for these stores */
 #pragma unroll
-        for (int i = 0; i < 4; i++)
-            if (i < f)
-                O::put(lds + RING * STEP + wave * O::BYTES, c[i], (typename XT<YTY>::raw *)a.y + (row0 + 64 * i) * a.ldy + t.n0 + wn, a.ldy, rows - 64 * i - 32 * wm, cols - wn);
+            for (int i = 0; i < 4; i++) O::template put<true>(mine, c[i], y + 64 * i * a.ldy, a.ldy, 32, 64);
+            late = AHEAD;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if (i < f) O::put(mine, c[i], y + 64 * i * a.ldy, a.ldy, rows - 64 * i - 32 * wm, cols - wn);
+            late = 0;
+        }
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); /* nothing may land in LDS that is no longer this block's */
 }
