@@ -366,8 +366,8 @@ int le_moe_combine_bwd(le_ctx *ctx, int ty, const void *dout, long long ldt, con
  *   le_mm_experts_dx: dx[i] = W_e^T dy[i], the gradient of x
  *   le_mm_experts_dw: dW_e = sum over e's rows i of dy[i] x[i]^T, the gradient of w, of type dwtype (ty or LE_F32); zeros for an expert
  *                     without rows
- * Products are exact (fp32: rounded as in a fused multiply-add), sums fp32 in an order that the sizes, off and alignment decide (the same
- * bits from call to call), the result is rounded once. Any rows, cols >= 1, any strides >= the row; sizes, strides and
+ * Products are exact (fp32: rounded as in a fused multiply-add), sums fp32 in an order that the sizes, off, alignment and an expert's number decide (the
+ * same bits from call to call), the result is rounded once. Any rows, cols >= 1, any strides >= the row; sizes, strides and
  * pointers that are multiples of 16 bytes are faster. A row that is not finite makes its own results infinite or NaN (in dw, its
  * expert's), and no others.
  * Limits: n_exp <= 1024, rows and cols <= 2^24, n_row <= 2^30. n_row may be 0. Outputs may not overlap inputs.

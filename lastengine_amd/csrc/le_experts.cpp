@@ -30,10 +30,12 @@ int parts(int n_exp, int n_row, int rows, int cols) {
     return (int)std::max(1LL, std::min({2 * kCus / tiles, n_row / (256LL * n_exp), 64LL}));
 }
 
-/* Whether y is taken by a wave a tile: few rows an expert, fewer where a wave's work on them is short (us, so / in tiles of 128 x 256, 128 experts
- * bf16: 1536 x 2048 64 rows 60 / 83, 128 rows 90 / 106, 512 rows 131 / 150; 2048 x 768 64 rows 33 / 37, 256 rows 67 / 62). */
+/* Whether y is taken by a wave a tile: few rows an expert, fewer where a wave's work on them is short (us, so / in larger tiles, 128 experts bf16:
+ * 1536 x 2048 64 rows 60 / 65, 256 rows 110 / 119, 512 rows 130 / 127; 2048 x 768 64 rows 33 / 37, 128 rows 58 / 54; 8 of 14336 x 4096 16 rows
+ * 150 / 189); fp32, bound by the matrix instructions, where larger tiles are fewer than CUs (8 rows 43 / 88, 64 rows 209 / 145). */
 bool few_rows(const ExpertArgs &a, int ty, const char *what) {
-    return what[0] == 'y' && a.n_row < (a.k * (long long)le_type_bytes(ty) < 4096 ? 2LL : 4LL) * a.n_exp;
+    if (what[0] != 'y' || a.n_row >= (a.k * (long long)le_type_bytes(ty) < 4096 ? 1LL : 3LL) * a.n_exp) return false;
+    return ty != LE_F32 || std::min(a.n_exp, a.n_row) * ((a.n + 255LL) / 256) < kCus;
 }
 
 /* The kernel of `what`_type. whole: every row that is read is whole 16-byte chunks. */

@@ -406,6 +406,10 @@ template <bool DOWN, int R, int NT> struct Stream {
             }
         }
     }
+    __device__ __forceinline__ void skip(int steps) {
+#pragma unroll
+        for (int j = 0; j < N; j++) at[j] += (long long)steps * (long long)step;
+    }
     /* The next step's chunks; left: depth from its start on, zeros where that ends. */
     __device__ __forceinline__ void load(unsigned lds, int left) {
         const unsigned wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -417,8 +421,10 @@ template <bool DOWN, int R, int NT> struct Stream {
             }
         } else {
 #pragma unroll
-            for (int j = 0; j < N; j++)
+            for (int j = 0; j < N; j++) {
                 chunk_to_lds(k + (DOWN ? j * (NT / C) : 0) < left ? at[j] : (unsigned long long)kZeros, lds + wave * 1024 + j * NT * 16);
+                at[j] += step;
+            }
         }
     }
 };
@@ -439,12 +445,24 @@ template <Kind KIND, int YTY, int BM, int BN, int RING> __device__ __forceinline
         Stream<BD, BN, 256> B;
         A.start((const T *)a.a + (KIND == DW ? t.lo * a.lda + t.m0 : (long long)(t.lo + t.m0) * a.lda), a.lda, rows);
         B.start((const T *)a.b + (KIND == DW ? t.lo * a.ldb + t.n0 : wsize * t.e + (KIND == Y ? (long long)t.n0 * a.ldb : t.n0)), a.ldb, cols);
-        int slot = 0, to = 0, left = depth; /* places in the ring; depth that has not been asked for */
+        /* Rows of W and x lie a power of two apart as a rule, so that every tile's first steps would ask the same channels: experts begin at steps of
+         * their own (y of 1024 rows of 128 experts of 1536 x 2048 bf16 172 / 136 us, 8192 rows 208 / 190, 32768 321 / 325). */
+        int step = KIND == Y ? t.e * 5 % steps : 0, asked = 0;
+        A.skip(step);
+        B.skip(step);
+        int slot = 0, to = 0; /* places in the ring */
         auto ask = [&] {
             const unsigned at = (unsigned)(unsigned long long)lds + to;
+            const int left = asked < steps ? depth - step * BK : 0;
             A.load(at, left);
             B.load(at + BM * 64, left);
-            left -= BK;
+            asked++;
+            step++;
+            if (KIND == Y && step == steps) {
+                step = 0;
+                A.skip(-steps);
+                B.skip(-steps);
+            }
             to = to == (RING - 1) * STEP ? 0 : to + STEP;
         };
         auto tile = [&](auto frags) {
