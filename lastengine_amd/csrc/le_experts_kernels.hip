@@ -367,7 +367,7 @@ template <Kind KIND, int YTY, int BM> __device__ __forceinline__ void any_body(c
  * permutation is in which chunk a lane asks for), RING steps in a ring: while one is multiplied, the others are on their way. One barrier
  * a step: behind it a step's chunks are there for all waves, and the step before is read by all. Rows
  * beyond an expert's last are asked for as its last (their results are dropped), k beyond the depth as zeros.
- * 128 experts of 1536 x 2048 bf16, 32768 rows (206 GFLOP, 1.0 GB): y 312 us, dx 275; a copy of those bytes would take 200, the products at the
+ * 128 experts of 1536 x 2048 bf16, 32768 rows (206 GFLOP, 1.0 GB): y 293 to 325 us, dx 289 to 300; a copy of those bytes would take 200, the products at the
  * clock that they leave 150. What comes from beyond the L2 (1.3 GB, as an expert's second tile of rows finds its weights gone) moves at
  * what the fabric gives, 6 TB/s, for y less: its operands are read 64 bytes of a row at a time, which alone runs at 4.4 TB/s. Steps of 128
  * bytes leave LDS for one in flight: 332. */

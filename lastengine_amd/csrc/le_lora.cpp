@@ -29,14 +29,15 @@ struct Shape {
         turns = tiles <= 32 ? std::min(m, 16) : tiles <= 64 ? 4 : 2;
         /* of 16 rows of A at once (rank 64, two / four: 4096 tokens bf16 31 / 23 us, 64 tokens 7 / 6, fp32 17 / 13) */
         sets = ad->rank <= 16 ? 1 : ad->rank <= 32 ? 2 : 4;
-        /* the columns' steps of 64 over a block's waves: eight, or as many as leave LDS for two blocks; four where every CU has a tile anyway (4 / 8
+        /* the columns' steps of 64 over a block's waves: eight, or as many as leave LDS for two blocks (few tokens: one, where fp32 rows
+         * take most: 22 tokens of 20949 columns 21 / 31 us, 64 of 4096 11 / 13); four where every CU has a tile anyway (4 / 8
          * waves, 4096 tokens in runs of 456: fp32 34 / 40 us, bf16 23 / 26, 16384 of 1024 columns 14 / 18; 2048 tokens: 61 / 45). And over segments
          * while that makes no more than 2048 waves: up to eight for few tokens, each with an adapter of its own; for many, whose sums each of the second
          * kernel's row blocks reads again, two up to 1024 waves (1 / 2 / 4 segments, both kernels: 300 tokens 30 / 27 / 29 us, 1024 35 / 32 / 39,
          * 2048 45 / 53 / 54). */
         const int all = (ad->cols + 63) / 64;
         wave_lds = le_type_bytes(xtype) * 1024 + 256 + sets * (le_type_bytes(ad->ltype) * 1024 + 256);
-        waves = std::min(std::min(tiles < 256 ? 8 : 4, (int)(80 * 1024 / wave_lds)), all);
+        waves = std::min(std::min(tiles < 256 ? 8 : 4, (int)((m <= kFew ? 160 : 80) * 1024 / wave_lds)), all);
         segs = m <= kFew ? std::min(8, 2048 / (tiles * turns * waves)) : std::min(2, 1024 / (tiles * waves));
         segs = std::max(1, std::min(segs, all / waves));
         steps = (all + segs - 1) / segs;
