@@ -195,7 +195,8 @@ template <int YTY, int NF, int ROWS = 32> struct Out {
             const v4u v = *(LE_LDS const v4u *)(mine + (r - r0) * PITCH + col * (int)sizeof(U));
             LE_GLOBAL U *to = (LE_GLOBAL U *)y + r * ld + col;
             if constexpr (ALL) {
-                asm volatile("global_store_dwordx4 %0, %1, off" ::"v"((unsigned long long)to), "v"(v) : "memory");
+                /* its registers may not be written in the two wait states behind it, and the compiler does not see a store here */
+                asm volatile("global_store_dwordx4 %0, %1, off\n\ts_nop 1" ::"v"((unsigned long long)to), "v"(v) : "memory");
             } else if (r < rows) {
                 if (col + E <= cols) {
                     if constexpr (sizeof(U) == 4) *(LE_GLOBAL v4u_a4 *)to = v;
