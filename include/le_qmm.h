@@ -407,10 +407,12 @@ int le_lora(le_ctx *ctx, const le_adapters *ad, const int *idx, int xtype, const
  * For row t < m of n values of type ty (LE_F32, LE_F16, LE_BF16):
  *     h[t] = x[t] + res[t], rounded to ty (res NULL: x[t])
  *     o[t][i] = (h[t][i] * r) * w[i] in fp32, r = 1 / sqrt(sum of h[t]^2 / n + eps), sum, r and the first product in 64 bits
- *     xd[t][u] = max |o[t][32u ..]| / 127,  xq[t][i] = o[t][i] * (1 / xd) to the nearest even, within -127 .. 127 (0 where xd is 0),
+ *     xd[t][u] = max |o[t][32u ..]| / 127,  xq[t][i] = o[t][i] * (1 / xd) to the nearest even, within -127 .. 127 (0 where xd is 0;
+ *     where xd is below 2^-126, whose reciprocal may leave fp32, of o and xd 2^64 times as large),
  *     xs[t][u] = sum of the unit's xq: the activations that le_matvec_q8 takes, from o before it is rounded to ty.
  * w is fp32. The 64 bits make codes next to a border those of the formula, whatever order a sum is taken in. A row with a value that is not
- * finite, or of zeros where eps is 0, has NaN in o and xd, and 0 in xq and xs. h, o and xs may be NULL; xq and xd may both be NULL (then n is any, else a
+ * finite, or of zeros where eps is 0, has NaN in o and xd, and 0 in xq and xs; a unit with an o that is not finite (w that is not, a product
+ * beyond fp32) has what that makes of xd, infinity or NaN, and 0 in xq and xs. h, o and xs may be NULL; xq and xd may both be NULL (then n is any, else a
  * multiple of 32). x, res, h and o have rows ldx, ldr, ldh and ldo values apart (>= n), xq rows of n, xd and xs of n / 32, back to back.
  * h may be x or res (with its row stride); outputs may not overlap inputs otherwise. eps >= 0. Limits: n <= 2^24, m < 2^31; m may be 0. */
 int le_add_rms_quant(le_ctx *ctx, int ty, const void *x, long long ldx, const void *res, long long ldr, const float *w, void *h,

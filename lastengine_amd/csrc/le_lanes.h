@@ -24,7 +24,7 @@ template <int N, int D = 1> static __device__ __forceinline__ int lanes_sum(int 
     if constexpr (D < N) return lanes_sum<N, 2 * D>(v + lane_across<D>(v));
     else return v;
 }
-template <int N, int D = 1> static __device__ __forceinline__ float lanes_max(float v) {
-    if constexpr (D < N) return lanes_max<N, 2 * D>(fmaxf(v, __builtin_bit_cast(float, lane_across<D>(__builtin_bit_cast(int, v)))));
+template <int N, int D = 1> static __device__ __forceinline__ unsigned lanes_max(unsigned v) {
+    if constexpr (D < N) return lanes_max<N, 2 * D>(max(v, (unsigned)lane_across<D>((int)v)));
     else return v;
 }

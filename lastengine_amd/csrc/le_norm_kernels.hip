@@ -78,13 +78,14 @@ __device__ __forceinline__ double root(const NormArgs &a, double s) {
 /* The norm of a piece, and its codes */
 template <int TY, int V, bool TAIL> __device__ __forceinline__ void finish(const NormArgs &a, long long t, int i, const float *h, double r) {
     constexpr int UNIT = 32 / V; /* lanes of 32 values */
-    float w[V], o[V], am = 0.f;
+    float w[V], o[V];
+    unsigned am = 0; /* the largest |o| as bits, whose order is that of the values, NaN behind infinity */
     load<0, 4, TAIL, false>(a.w, i, a.n - i, w);
     if constexpr (V == 8) load<0, 4, TAIL, false>(a.w, i + 4, a.n - i - 4, w + 4);
 #pragma unroll
     for (int j = 0; j < V; j++) {
         o[j] = (float)((double)h[j] * r) * w[j];
-        am = fmaxf(am, fabsf(o[j]));
+        am = max(am, __builtin_bit_cast(unsigned, o[j]) & 0x7FFFFFFFu);
     }
     const int n = a.n - i;
     if (n > 0) {
@@ -92,13 +93,15 @@ template <int TY, int V, bool TAIL> __device__ __forceinline__ void finish(const
         if (a.o) store<TY, V, TAIL>(a.o, t * a.ldo + i, n, o);
     }
     if (a.xq) { /* n is a multiple of 32: whole units */
-        const bool fine = r == r;
-        const float d = lanes_max<UNIT>(am) / 127.0f, id = d > 0.f ? 1.0f / d : 0.f;
+        am = lanes_max<UNIT>(am);
+        const bool fine = am < 0x7F800000u;
+        /* 1 / d is infinite for d below 2^-128: both sides of such units are taken 2^64 times as large, which changes no bit of the others' product */
+        const float d = __builtin_bit_cast(float, am) / 127.0f, up = d < 0x1p-126f ? 0x1p64f : 1.0f, id = d > 0.f ? 1.0f / (d * up) : 0.f;
         int sum = 0;
         unsigned q[V / 4];
 #pragma unroll
         for (int j = 0; j < V; j++) {
-            const int c = fine ? (int)fminf(fmaxf(rintf(o[j] * id), -127.f), 127.f) : 0;
+            const int c = fine ? (int)fminf(fmaxf(rintf(o[j] * up * id), -127.f), 127.f) : 0;
             sum += c;
             q[j >> 2] = j & 3 ? q[j >> 2] | (c & 255) << 8 * (j & 3) : c & 255;
         }
@@ -110,7 +113,7 @@ template <int TY, int V, bool TAIL> __device__ __forceinline__ void finish(const
             if constexpr (V == 4) *(LE_GLOBAL word *)xq = q[0];
             else *(LE_GLOBAL words *)xq = q[0] | (unsigned long long)q[V / 4 - 1] << 32;
             if ((i & 31) == 0) {
-                ((LE_GLOBAL float *)a.xd)[(t * a.n + i) >> 5] = fine ? d : __builtin_nanf("");
+                ((LE_GLOBAL float *)a.xd)[(t * a.n + i) >> 5] = d;
                 if (a.xs) ((LE_GLOBAL int *)a.xs)[(t * a.n + i) >> 5] = sum;
             }
         }

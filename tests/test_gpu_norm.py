@@ -234,3 +234,61 @@ def test_on_given_streams_and_in_graphs(engine):
     torch.cuda.synchronize()
     cs[1].run(engine, streams[0])
     cs[1].check()
+
+
+def weights_of(c, w):
+    c.wrows.rows.copy_(w)
+    return c
+
+
+@pytest.mark.parametrize("ty", TYPES)
+@pytest.mark.parametrize("m,n", [(3, 64), (2, 2080), (5, 4096), (1, 40000)])
+@pytest.mark.parametrize("size", [1e-36, 1e-37, 3e-39, 1e-41, 1e-44])
+def test_units_whose_scale_has_no_reciprocal(engine, ty, m, n, size):
+    """The smallest fp32 weights: xd down to the last subnormal numbers and 0, with zeros in every unit and a unit of zeros."""
+    import torch
+    gen = torch.Generator().manual_seed(13)
+    w = ((torch.randn(1, n, generator=gen).double() + 3.0) * size).float()
+    w[0, ::5] = 0.0
+    w[0, 32:64] = 0.0
+    c = weights_of(Case(ty, m, n, 14), w)
+    c.run(engine)
+    h, o, _, d, _ = reference(c.x.rows.cpu(), c.res.rows.cpu(), w[0], ty, c.eps)
+    u, far = o.numpy().reshape(m, n // 32, 32), d.numpy() < np.float32(2.0 ** -126)
+    up = np.where(far, np.float32(2.0 ** 64), np.float32(1.0))
+    with np.errstate(divide="ignore"):
+        inv = np.where(d.numpy() > 0, np.float32(1.0) / (d.numpy() * up), np.float32(0.0)).astype(np.float32)
+    q = np.clip(np.rint((u * up[:, :, None]) * inv[:, :, None]), -127, 127)
+    # what the codes stand for: half a code from the quotient, a product and a reciprocal in 32 bits off by 2^-24 of up to 190 each (xd's own rounding, where it
+    # has few bits, makes a quotient of up to 190, which is cut to 127)
+    live = d.numpy() > 0
+    ratio = np.clip(u.astype(np.float64)[live] / d.double().numpy()[live][:, None], -127.0, 127.0)
+    assert (np.abs(q[live] - ratio) <= 0.5 + 190 * 2.0 ** -22).all() and (q[u == 0] == 0).all()
+    q = q.astype(np.int8)
+    c.check([h, o, torch.from_numpy(q.reshape(m, n)), d, torch.from_numpy(q.astype(np.int32).sum(2).astype(np.int32))])
+    if size < 1e-37:
+        assert far.all()
+
+
+@pytest.mark.parametrize("ty", TYPES)
+@pytest.mark.parametrize("m,n", [(3, 96), (2, 2080), (4, 4096), (1, 40000)])
+def test_units_that_are_not_finite(engine, ty, m, n):
+    """Weights that are not finite and products beyond fp32 reach their own units alone, which get no codes."""
+    import torch
+    gen = torch.Generator().manual_seed(15)
+    w = torch.randn(1, n, generator=gen) * 0.3 + 1.0
+    w[0, 5] = float("nan")
+    w[0, 33] = float("inf")
+    w[0, n - 1] = -3e38  # beyond fp32 for a norm of 1.2 and more, -infinity or infinity
+    w[0, n - 3] = float("-inf") if n > 96 else 1.0
+    c = weights_of(Case(ty, m, n, 16), w)
+    c.x.rows[:, n - 1], c.res.rows[:, n - 1] = 8.0, 8.0
+    c.run(engine)
+    h, o, q, d, s = reference(c.x.rows.cpu(), c.res.rows.cpu(), w[0], ty, c.eps)
+    torch.cuda.synchronize()
+    assert torch.isnan(d[:, 0]).all() and torch.isinf(d[:, 1]).all() and torch.isinf(d[:, -1]).all()
+    for u in (0, 1, -1):
+        assert (q.reshape(m, -1, 32)[:, u] == 0).all() and (s.reshape(m, -1)[:, u] == 0).all()
+    k = m * n
+    assert same(c.h.rows.cpu(), h) and same(c.o.rows.cpu(), o.to(dtype(ty))) and c.o.untouched(m, 77.0)
+    assert same(c.xd[:k // 32].cpu(), d.reshape(-1)) and torch.equal(c.xq[:k].cpu(), q.reshape(-1)) and torch.equal(c.xs[:k // 32].cpu(), s.reshape(-1))
