@@ -22,7 +22,8 @@ template <> struct Any<2> { typedef v4u __attribute__((aligned(2))) v; };
 template <> struct Any<4> { typedef v4u __attribute__((aligned(4))) v; };
 
 /* A piece's values: all, or the n that there are (zeros behind them); TAIL: n may also lie between.
- * ONCE: read by nobody else (not kept in the caches: 4096 x 4096, x, res and o of fp32 82 -> 63 us, of bf16 48 -> 38). */
+ * ONCE: read by nobody else after this (not kept in the caches: 4096 x 4096, x, res and o of fp32 82 -> 63 us, of bf16 48 -> 38; but a row's first
+ * reading of two keeps it: x, res, h and o of 4096 x 4097 fp32 90 -> 76 us, of 8192 x 1001 bf16 35 -> 28, 64 x 40000 fp32 with codes 28 -> 22). */
 template <int TY, int V, bool TAIL, bool ONCE> __device__ __forceinline__ void load(const void *p, long long at, int n, float *v) {
     using T = typename XT<TY>::raw;
     const LE_GLOBAL T *g = (const LE_GLOBAL T *)p + at;
@@ -58,12 +59,12 @@ template <int TY, int V, bool TAIL> __device__ __forceinline__ void store(void *
     }
 }
 
-/* h from here on, as it is stored */
-template <int TY, int V, bool TAIL> __device__ __forceinline__ void sum_with(const NormArgs &a, long long t, int i, float *v) {
-    load<TY, V, TAIL, true>(a.x, t * a.ldx + i, a.n - i, v);
+/* h from here on, as it is stored. ONCE: of load() */
+template <int TY, int V, bool TAIL, bool ONCE> __device__ __forceinline__ void sum_with(const NormArgs &a, long long t, int i, float *v) {
+    load<TY, V, TAIL, ONCE>(a.x, t * a.ldx + i, a.n - i, v);
     if (a.res) {
         float r[V];
-        load<TY, V, TAIL, true>(a.res, t * a.ldr + i, a.n - i, r);
+        load<TY, V, TAIL, ONCE>(a.res, t * a.ldr + i, a.n - i, r);
 #pragma unroll
         for (int j = 0; j < V; j++) v[j] = XT<TY>::up(XT<TY>::down(v[j] + r[j]));
     }
@@ -142,7 +143,7 @@ template <int TY, int L, int NC> __device__ __forceinline__ void norm_body(const
         float h[NC][V];
         double s = 0.0;
 #pragma unroll
-        for (int c = 0; c < NC; c++) sum_with<TY, V, false>(a, t, (l + L * c) * V, h[c]);
+        for (int c = 0; c < NC; c++) sum_with<TY, V, false, true>(a, t, (l + L * c) * V, h[c]);
 #pragma unroll
         for (int c = 0; c < NC; c++)
 #pragma unroll
@@ -159,7 +160,7 @@ template <int TY, int L> __device__ __forceinline__ void any_body(const NormArgs
         double s = 0.0;
         for (int i = threadIdx.x * V; i < a.n; i += L * V) {
             float h[V];
-            sum_with<TY, V, true>(a, t, i, h);
+            sum_with<TY, V, true, false>(a, t, i, h);
 #pragma unroll
             for (int j = 0; j < V; j++) s = fma((double)h[j], (double)h[j], s);
         }
@@ -167,7 +168,7 @@ template <int TY, int L> __device__ __forceinline__ void any_body(const NormArgs
         for (int i0 = 0; i0 < a.n; i0 += L * V) { /* all lanes go along: units lie across them */
             const int i = i0 + threadIdx.x * V;
             float h[V];
-            sum_with<TY, V, true>(a, t, i, h);
+            sum_with<TY, V, true, true>(a, t, i, h);
             finish<TY, V, true>(a, t, i, h, r);
         }
     }
