@@ -426,6 +426,7 @@ template <int WTY, int J> __device__ __forceinline__ void upm_body(const LoraArg
     const bool whole = row + E <= a.rows;
     const int ids = adapter(a, blockIdx.y * 64 + l);
     int held = -1; /* whose B the registers hold */
+    const float none = a.base ? -0.f : 0.f; /* what a token without an adapter adds: its base stays as it is, a zero of either sign too */
     typename Mul::A w[J > 0 ? J : 1][4];
     auto get = [&](int ad, int j, typename Mul::A *q) {
 #pragma unroll
@@ -468,7 +469,7 @@ template <int WTY, int J> __device__ __forceinline__ void upm_body(const LoraArg
         }
         v4f out[4];
 #pragma unroll
-        for (int f = 0; f < 4; f++) out[f] = v4f{0.f, 0.f, 0.f, 0.f};
+        for (int f = 0; f < 4; f++) out[f] = v4f{none, none, none, none};
         while (t.next()) {
             v4f c[4];
 #pragma unroll

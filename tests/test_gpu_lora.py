@@ -232,3 +232,25 @@ def test_beside_a_quantized_projection(engine, ty):
     c.base64 = y.cpu().double()
     c.run(engine)
     c.check_real()
+
+
+@pytest.mark.parametrize("ty", TYPES)
+@pytest.mark.parametrize("m", [1, 20, 256, 257, 700])
+def test_base_of_no_adapter_to_the_bit(engine, ty, m):
+    """Zeros of both signs, infinities and the smallest values of base where there is no adapter; without a base zeros."""
+    import torch
+    t = dtype(ty)
+    values = torch.tensor([-0.0, 0.0, float("inf"), -float("inf"), torch.finfo(t).smallest_normal / 4, -torch.finfo(t).max], dtype=t)
+    for rows in (96, 99):
+        c = Case(ty, ty, m, rows, 64, 8, 3, 13, bare=0.0)
+        c.idx[::3] = -1
+        c.dev_idx.copy_(c.idx)
+        base = values[torch.arange(m * rows).reshape(m, rows) % len(values)]
+        c.base.rows.copy_(base)
+        bits = torch.int32 if ty == le.F32 else torch.int16
+        for has_base in (True, False):
+            c.has_base = has_base
+            c.run(engine)
+            torch.cuda.synchronize()
+            want = base[::3] if has_base else torch.zeros_like(base[::3])
+            assert torch.equal(c.y.rows.cpu()[::3].contiguous().view(bits), want.contiguous().view(bits))
