@@ -1,5 +1,5 @@
 /* Low-rank adapters beside a shared projection (le_lora, include/le_qmm.h), compiled once per type of the activations (LE_LO_XTY).
- * Two launches: u[t] = A x[t] over the columns, then y[t] = base[t] + B (scale u[t]) over the rank. Tokens are taken 16 at a time, as they
+ * Two launches: u[t] = A x[t] over the columns, then y[t] = base[t] + scale (B u[t]) over the rank. Tokens are taken 16 at a time, as they
  * come; a tile of 16 with several adapters is done once for each of them, and what it gives for the others' tokens is dropped
  * (selected, so that nothing of one token or adapter reaches another). */
 #include <hip/hip_runtime.h>
@@ -446,7 +446,7 @@ template <int WTY, int J> __device__ __forceinline__ void upm_body(const LoraArg
             if (a.base && whole) base[p] = *(const LE_GLOBAL v4u_any *)((const LE_GLOBAL X *)a.base + min(t0 + p * E + l / LANES, a.m - 1) * a.ldb + row);
         Tile t(__builtin_amdgcn_ds_bpermute((16 * n + c16) * 4, ids));
         const float s = t.id >= 0 ? factor(a, t.id) : 0.f;
-        /* scale u of this lane's token, zeros where it has no adapter */
+        /* u of this lane's token, zeros where it has no adapter */
         auto low = [&](int j) {
             Eight<0> u;
 #pragma unroll
@@ -458,8 +458,6 @@ template <int WTY, int J> __device__ __forceinline__ void upm_body(const LoraArg
 #pragma unroll
                     for (int i = 0; i < 4; i++) u.v[i] += lo[i], u.v[4 + i] += hi[i];
                 }
-#pragma unroll
-            for (int i = 0; i < 8; i++) u.v[i] *= s;
             return u;
         };
         typename Mul::B u[J > 0 ? J : 1];
@@ -497,6 +495,8 @@ template <int WTY, int J> __device__ __forceinline__ void upm_body(const LoraArg
                 for (int f = 0; f < 4; f++) out[f] = c[f];
             }
         }
+#pragma unroll
+        for (int f = 0; f < 4; f++) out[f] *= s; /* behind the sum, as for few tokens: scale u may be out of fp32's range where y is not */
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); /* the wave's reads of the tile before */
         __builtin_amdgcn_wave_barrier();
 #pragma unroll

@@ -254,3 +254,29 @@ def test_base_of_no_adapter_to_the_bit(engine, ty, m):
             torch.cuda.synchronize()
             want = base[::3] if has_base else torch.zeros_like(base[::3])
             assert torch.equal(c.y.rows.cpu()[::3].contiguous().view(bits), want.contiguous().view(bits))
+
+
+@pytest.mark.parametrize("xty", [le.F32, le.BF16])
+@pytest.mark.parametrize("wty", TYPES)
+@pytest.mark.parametrize("m", [20, 256, 257, 400])
+@pytest.mark.parametrize("rank", [16, 64, 100])
+def test_far_factors(engine, xty, wty, m, rank):
+    """Factors whose products with A x alone would leave fp32, though y does not. Powers of two, one rank live: exact."""
+    import torch
+    for scale, xs, bs in ((2.0 ** 100, 2.0 ** 40, 2.0 ** -14), (2.0 ** -120, 2.0 ** -20, 2.0 ** 14)):
+        c = Case(xty, wty, m, 72, 64, rank, 3, 14, bare=0.0, base=False, scale=False)
+        c.x64 = torch.zeros(m, 64).double()
+        c.x64[:, 5] = xs * (1 + torch.arange(m) % 2)
+        c.a64 = torch.zeros(3, rank, 64).double()
+        c.a64[:, rank - 3] = 1.0
+        c.b64 = torch.zeros(3, 72, rank).double()
+        c.b64[:, :, rank - 3] = bs * (torch.arange(72) % 3 - 1).double()
+        c.s64 = torch.full((3,), scale).double()
+        c.x.rows.copy_(c.x64)
+        c.a.rows.copy_(c.a64.reshape(3, -1))
+        c.b.rows.copy_(c.b64.reshape(3, -1))
+        c.scale = c.s64.float().cuda()
+        c.ad = le.Adapters(c.a.ptr, c.b.ptr, c.scale, 3, rank, 72, 64, ltype=wty)
+        c.run(engine)
+        c.check_whole()
+        assert float(c.y.rows.abs().max()) == 2 * scale * xs * bs
