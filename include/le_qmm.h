@@ -393,8 +393,11 @@ typedef struct le_adapters {
 /* For token t < m, with i = idx[t]:  y[t] = base[t] + scale_i * B_i (A_i x[t]);  y[t] = base[t] where i lies outside 0 .. n_ad - 1.
  * base is what the shared projection gave (le_gemm, le_matvec, le_matvec_g4), NULL stands for zeros; base may be y. x, base and y are
  * of type xtype, x's rows of cols values ldx apart (0: one row for all), base's and y's of `rows` values ldb and ldy apart. Products
- * with A are exact and summed in fp32, A_i x[t] is held in fp32, and so are the sums over the rank, their product with scale_i and the sum with base; the
- * result is rounded once. Tokens of one adapter need not follow one another, but for many tokens runs of 16 and more are faster.
+ * with A are exact (two fp32 values: rounded as in a fused multiply-add) and summed in fp32, A_i x[t] is held in fp32, and so are the sums over the rank,
+ * their product with scale_i and the sum with base; the result is rounded once. Of an fp32 value beside 16-bit ones (x beside A, A beside x, for more
+ * than 256 tokens A_i x[t] beside B) what lies below 2^-133 is cut off. A value that is not finite, or A_i x[t] beyond fp32, makes the results that it has a part
+ * in infinite or NaN (not always the formula's one of the two), and no others. Tokens of one adapter need not follow one another, but for many tokens runs
+ * of 16 and more are faster: above 256 tokens every 16 neighbours are done once for each adapter among them.
  * Limits: rank <= 256, rows and cols <= 2^24, m <= 1048560, n_ad >= 1; m may be 0. y may not overlap other inputs, nor base otherwise.
  * ws: le_lora_workspace_size bytes, 16-byte aligned, which every call writes anew; calls that may overlap need workspaces of
  * their own. */

@@ -280,3 +280,60 @@ def test_far_factors(engine, xty, wty, m, rank):
         c.run(engine)
         c.check_whole()
         assert float(c.y.rows.abs().max()) == 2 * scale * xs * bs
+
+
+@pytest.mark.parametrize("xty,wty", [(x, w) for x in TYPES for w in TYPES if x != w])
+@pytest.mark.parametrize("m", [3, 50, 140, 270])
+def test_what_is_not_finite_stays_with_its_token_beside_another_type(engine, xty, wty, m):
+    import torch
+    c = Case(xty, wty, m, 72, 136, 8, 3, 15, bare=0.0)
+    c.idx = (torch.arange(m) % 3).to(torch.int32)
+    c.dev_idx.copy_(c.idx)
+    want = c.want().to(dtype(xty))
+    c.a.rows[1] = float("nan")
+    c.b.rows[1] = float("inf")
+    c.x.rows[2, 5] = float("inf")
+    c.a.rows[2] += 10.0  # no zeros, so that all of token 2 is infinite or NaN
+    c.b.rows[2, 3 * 8:] = 1.0
+    c.b.rows[2, :3 * 8] = 0.0
+    c.run(engine)
+    torch.cuda.synchronize()
+    got = c.y.rows.cpu()
+    for t in range(m):
+        if t == 2:
+            assert not torch.isfinite(got[t, 3:]).any()
+        elif t % 3 == 1:
+            assert not torch.isfinite(got[t]).any()
+        elif t % 3 == 0:
+            assert torch.equal(got[t], want[t]), t
+        else:
+            assert torch.isfinite(got[t]).all(), t
+
+
+@pytest.mark.parametrize("xty,wty", [(le.F32, le.F16), (le.F32, le.BF16), (le.F16, le.F32), (le.BF16, le.F32)])
+@pytest.mark.parametrize("m", [20, 300])
+@pytest.mark.parametrize("e", [-90, -108, -120, -128])
+def test_small_fp32_beside_16_bits(engine, xty, wty, m, e):
+    """The fp32 side's values around 2^e, the other's 2^up, brought near 1 by the second product and the factor: fp32 sums, and each value cut at 2^-133."""
+    import torch
+    gen = torch.Generator().manual_seed(16)
+    cols, up = 64, 14
+    c = Case(xty, wty, m, 40, cols, 16, 2, 17, bare=0.0, base=False)
+    tiny = lambda *shape: ((1 + torch.rand(*shape, generator=gen, dtype=torch.float64)) * 2.0 ** e).float().double()  # noqa: E731
+    c.x64 = tiny(m, cols) if xty == le.F32 else torch.full((m, cols), 2.0 ** up).double()
+    c.a64 = tiny(2, 16, cols) if wty == le.F32 else torch.full((2, 16, cols), 2.0 ** up).double()
+    c.b64 = torch.zeros(2, 40, 16).double()
+    c.b64[:, torch.arange(40), torch.arange(40) % 16] = 2.0 ** 14
+    c.s64 = torch.full((2,), 2.0 ** (-e - up - 14 - 6)).double()
+    c.x.rows.copy_(c.x64)
+    c.a.rows.copy_(c.a64.reshape(2, -1))
+    c.b.rows.copy_(c.b64.reshape(2, -1))
+    c.scale = c.s64.float().cuda()
+    c.ad = le.Adapters(c.a.ptr, c.b.ptr, c.scale, 2, 16, 40, cols, ltype=wty)
+    c.run(engine)
+    torch.cuda.synchronize()
+    want, total = c.want(), 2.0 ** (-e - up - 6)
+    # the sums over cols and rank (cols + 16 steps and the factor), what is cut of the cols values and of their sum, one rounding
+    bound = (cols + 20) * 2.0 ** -23 * want + (cols * 2.0 ** (-133 + up) + 2.0 ** -133) * total
+    bound = bound + half_step(xty) * (want + bound) + (2.0 ** -25 if xty == le.F16 else 1e-38)
+    assert float(want.min()) > 0.5 and ((c.y.rows.cpu().double() - want).abs() <= bound).all()
