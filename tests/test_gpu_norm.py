@@ -292,3 +292,24 @@ def test_units_that_are_not_finite(engine, ty, m, n):
     k = m * n
     assert same(c.h.rows.cpu(), h) and same(c.o.rows.cpu(), o.to(dtype(ty))) and c.o.untouched(m, 77.0)
     assert same(c.xd[:k // 32].cpu(), d.reshape(-1)) and torch.equal(c.xq[:k].cpu(), q.reshape(-1)) and torch.equal(c.xs[:k // 32].cpu(), s.reshape(-1))
+
+
+@pytest.mark.parametrize("ty", TYPES)
+@pytest.mark.parametrize("n,gap,at", [(256, 0, 0), (256, 8, 0), (4096, 3, 1), (33, 0, 0), (40000, 0, 0)])
+def test_rows_of_zeros_without_eps(engine, ty, n, gap, at):
+    """NaN in the row of zeros, every other value of o and what lies around it as it has to be."""
+    import torch
+    c = Case(ty, 5, n, 17, eps=0.0, gap=gap, at=at, q=n % 32 == 0)
+    for t in (1, 4):
+        c.x.rows[t], c.res.rows[t] = 0.0, -0.0
+    c.run(engine)
+    torch.cuda.synchronize()
+    wh, wo, wq, wd, ws = c.want()
+    assert torch.isnan(wo[[1, 4]]).all() and not torch.isnan(wo[[0, 2, 3]]).any()
+    assert same(c.o.rows.cpu(), wo.to(dtype(ty)))
+    assert c.o.untouched(c.m, 77.0) and c.h.untouched(c.m, 77.0)
+    assert same(c.h.rows.cpu(), wh)
+    if c.xq is not None:
+        wq[[1, 4]], ws[[1, 4]], wd[[1, 4]] = 0, 0, float("nan")
+        k = c.m * n
+        assert torch.equal(c.xq[:k].cpu(), wq.reshape(-1)) and torch.equal(c.xs[:k // 32].cpu(), ws.reshape(-1)) and same(c.xd[:k // 32].cpu(), wd.reshape(-1))
