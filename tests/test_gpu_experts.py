@@ -301,3 +301,19 @@ def test_on_given_streams_and_in_graphs(engine):
     torch.cuda.synchronize()
     cs[1].run(engine, streams[0])
     cs[1].check_whole()
+
+
+@pytest.mark.parametrize("ty", TYPES)
+@pytest.mark.parametrize("fp32", [False, True])
+@pytest.mark.parametrize("at", [1, 2, 3, 8])
+@pytest.mark.parametrize("counts,rows,cols", [([130, 0, 70, 3], 1000, 4088), ([33, 200, 0, 9], 1024, 4096), ([20, 260, 1], 520, 1000), ([1500], 64, 48), ([7, 3], 24, 40)])
+def test_weights_gradient_aligned_to_its_type_alone(engine, ty, fp32, at, counts, rows, cols):
+    """Rows of whole 16-byte pieces, so that the kernels of such rows run, and a result that begins anywhere."""
+    import torch
+    c = Case(ty, counts, rows, cols, 14, dw_ty=le.F32 if fp32 else None)
+    c.dw = Rows(c.dw_ty, c.e, rows * cols, None, at, 77.0)
+    c.run(engine)
+    torch.cuda.synchronize()
+    assert c.dw.untouched(c.e, 77.0)
+    want = c.want(c.x64, c.dy64, c.w64)[2]
+    assert torch.equal(c.dw.rows.cpu().reshape(want.shape), want.to(c.dw.rows.dtype))
