@@ -317,3 +317,53 @@ def test_weights_gradient_aligned_to_its_type_alone(engine, ty, fp32, at, counts
     assert c.dw.untouched(c.e, 77.0)
     want = c.want(c.x64, c.dy64, c.w64)[2]
     assert torch.equal(c.dw.rows.cpu().reshape(want.shape), want.to(c.dw.rows.dtype))
+
+
+def far_experts(ty, rows, cols, n_row, live, seed):
+    """Weights of 1024 experts of which only the last is filled and has rows; its first value lies past 2^32."""
+    import torch
+    gen, t = torch.Generator().manual_seed(seed), dtype(ty)
+    assert 1023 * rows * cols > 1 << 32
+    w = torch.empty(1024 * rows * cols, dtype=t, device="cuda")
+    wl, x, dy = whole(gen, rows, cols), whole(gen, live, cols), whole(gen, live, rows)
+    w[1023 * rows * cols:] = wl.reshape(-1).to(t).cuda()
+    off = torch.zeros(1025, dtype=torch.int32, device="cuda")
+    off[1024] = live
+    full = [torch.full((n_row, width), float("nan"), dtype=t, device="cuda") for width in (cols, rows)]
+    full[0][:live], full[1][:live] = x.to(t).cuda(), dy.to(t).cuda()
+    return w, off, full[0], full[1], wl, x, dy
+
+
+@pytest.mark.parametrize("ty", TYPES)
+@pytest.mark.parametrize("rows,cols,n_row,live", [(2048, 2064, 3, 3), (2048, 2064, 4000, 300), (128, 32816, 4000, 300), (2048, 2065, 4000, 70), (2048, 2065, 50000, 300)])
+def test_weights_past_32_bits(engine, ty, rows, cols, n_row, live):
+    """Every way that y and dx read weights: few rows an expert, whole rows in narrow and wide tiles, rows of any alignment in small and
+    large tiles."""
+    import torch
+    t = dtype(ty)
+    w, off, x, dy, w64, x64, dy64 = far_experts(ty, rows, cols, n_row, live, 15)
+    y, dx = (torch.full((n_row, width), 77.0, dtype=t, device="cuda") for width in (rows, cols))
+    engine.mm_experts(ty, w, off, x, y, 1024, n_row, rows, cols)
+    engine.mm_experts_dx(ty, w, off, dy, dx, 1024, n_row, rows, cols)
+    torch.cuda.synchronize()
+    assert torch.equal(y[:live].cpu(), (x64 @ w64.t()).to(t)) and (y[live:] == 77.0).all()
+    assert torch.equal(dx[:live].cpu(), (dy64 @ w64).to(t)) and (dx[live:] == 77.0).all()
+
+
+@pytest.mark.parametrize("ty", TYPES)
+@pytest.mark.parametrize("rows,cols", [(2048, 2064), (2048, 2065), (32816, 128), (24, 175001)])
+def test_weights_gradient_past_32_bits(engine, ty, rows, cols):
+    """Gradients of 1024 experts, zeros but for the first and the last, which begins past 2^32 values."""
+    import torch
+    gen, t, live = torch.Generator().manual_seed(18), dtype(ty), 45
+    assert 1023 * rows * cols > 1 << 32
+    x, dy = whole(gen, live, cols), whole(gen, live, rows)
+    off = torch.full((1025,), 5, dtype=torch.int32, device="cuda")
+    off[0], off[1024] = 0, live
+    dw = torch.full((1024, rows * cols), 77.0, dtype=t, device="cuda")
+    engine.mm_experts_dw(ty, dy.to(t).cuda(), x.to(t).cuda(), off, dw, 1024, live, rows, cols)
+    torch.cuda.synchronize()
+    for e, s in ((0, slice(0, 5)), (1023, slice(5, live))):
+        assert torch.equal(dw[e].cpu().reshape(rows, cols), (dy[s].t() @ x[s]).to(t)), e
+    for e in range(1, 1023, 73):
+        assert not dw[e:min(e + 73, 1023)].any(), e
