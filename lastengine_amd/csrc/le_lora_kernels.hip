@@ -426,7 +426,8 @@ template <int WTY, int J> __device__ __forceinline__ void upm_body(const LoraArg
     const bool whole = row + E <= a.rows;
     const int ids = adapter(a, blockIdx.y * 64 + l);
     int held = -1; /* whose B the registers hold */
-    const float none = a.base ? -0.f : 0.f; /* what a token without an adapter adds: its base stays as it is, a zero of either sign too */
+    const float none = a.base ? -0.f : 0.f; /* a token's factor without an adapter: what its zeros then add leaves base as it is, a zero of either sign too
+                                             * (sums that begin at that instead of 0 take 44 registers more) */
     typename Mul::A w[J > 0 ? J : 1][4];
     auto get = [&](int ad, int j, typename Mul::A *q) {
 #pragma unroll
@@ -445,7 +446,7 @@ template <int WTY, int J> __device__ __forceinline__ void upm_body(const LoraArg
         for (int p = 0; p < PIECES; p++)
             if (a.base && whole) base[p] = *(const LE_GLOBAL v4u_any *)((const LE_GLOBAL X *)a.base + min(t0 + p * E + l / LANES, a.m - 1) * a.ldb + row);
         Tile t(__builtin_amdgcn_ds_bpermute((16 * n + c16) * 4, ids));
-        const float s = t.id >= 0 ? factor(a, t.id) : 0.f;
+        const float s = t.id >= 0 ? factor(a, t.id) : none;
         /* u of this lane's token, zeros where it has no adapter */
         auto low = [&](int j) {
             Eight<0> u;
@@ -467,7 +468,7 @@ template <int WTY, int J> __device__ __forceinline__ void upm_body(const LoraArg
         }
         v4f out[4];
 #pragma unroll
-        for (int f = 0; f < 4; f++) out[f] = v4f{none, none, none, none};
+        for (int f = 0; f < 4; f++) out[f] = v4f{0.f, 0.f, 0.f, 0.f};
         while (t.next()) {
             v4f c[4];
 #pragma unroll
@@ -533,6 +534,8 @@ template <int WTY, int J> __device__ __forceinline__ void upm_body(const LoraArg
 
 #define LE_LO_NAME2(WHAT, X, W) le_lo_##WHAT##_##X##_##W
 #define LE_LO_NAME(WHAT, X, W) LE_LO_NAME2(WHAT, X, W)
+/* Waves a SIMD of upm0: four where 128 registers do without scratch (fp32 adapters of rank 37 beside fp16, 4096 tokens 59 us, with one register too many 66) */
+#define LE_LO_FOUR(W) (LE_LO_XTY != 0 && W != 1 ? 4 : 3)
 #define LE_LO(W)                                                                                                             \
     extern "C" __global__ void __launch_bounds__(512) LE_LO_NAME(down1, LE_LO_XTY, W)(LoraArgs a) { down_body<W, 1>(a); } \
     extern "C" __global__ void __launch_bounds__(512) LE_LO_NAME(down2, LE_LO_XTY, W)(LoraArgs a) { down_body<W, 2>(a); } \
@@ -543,7 +546,7 @@ template <int WTY, int J> __device__ __forceinline__ void upm_body(const LoraArg
     extern "C" __global__ void __launch_bounds__(256) LE_LO_NAME(upv8, LE_LO_XTY, W)(LoraArgs a) { upv_body<W, 8>(a); } \
     extern "C" __global__ void __launch_bounds__(256) LE_LO_NAME(upv16, LE_LO_XTY, W)(LoraArgs a) { upv_body<W, 16>(a); } \
     extern "C" __global__ void __launch_bounds__(256) LE_LO_NAME(upv32, LE_LO_XTY, W)(LoraArgs a) { upv_body<W, 32>(a); } \
-    extern "C" __global__ void __launch_bounds__(256) LE_LO_NAME(upm0, LE_LO_XTY, W)(LoraArgs a) { upm_body<W, 0>(a); }    \
+    extern "C" __global__ void __launch_bounds__(256, LE_LO_FOUR(W)) LE_LO_NAME(upm0, LE_LO_XTY, W)(LoraArgs a) { upm_body<W, 0>(a); }    \
     extern "C" __global__ void __launch_bounds__(256) LE_LO_NAME(upm1, LE_LO_XTY, W)(LoraArgs a) { upm_body<W, 1>(a); }    \
     extern "C" __global__ void __launch_bounds__(256) LE_LO_NAME(upm2, LE_LO_XTY, W)(LoraArgs a) { upm_body<W, 2>(a); }
 LE_LO(0)
