@@ -102,11 +102,13 @@ template <int TY, int V, bool TAIL> __device__ __forceinline__ void finish(const
         unsigned q[V / 4];
 #pragma unroll
         for (int j = 0; j < V; j++) {
-            const int c = fine ? (int)fminf(fmaxf(rintf(o[j] * up * id), -127.f), 127.f) : 0;
+            const int c = (int)fminf(fmaxf(rintf(o[j] * up * id), -127.f), 127.f);
             sum += c;
             q[j >> 2] = j & 3 ? q[j >> 2] | (c & 255) << 8 * (j & 3) : c & 255;
         }
-        sum = lanes_sum<UNIT>(sum);
+        sum = fine ? lanes_sum<UNIT>(sum) : 0;
+#pragma unroll
+        for (int j = 0; j < V / 4; j++) q[j] = fine ? q[j] : 0;
         if (n > 0) {
             typedef unsigned __attribute__((aligned(1))) word;
             typedef unsigned long long __attribute__((aligned(1))) words;
