@@ -618,7 +618,8 @@ __device__ __forceinline__ void few_body(const ExpertArgs &a) {
  * memory would be one for the chunks as well. 128 experts of 1536 x 2048 bf16, 32768 rows: 350 us (while the first steps waited for the stores
  * before them 357), in the tiles above 404; 8168 rows of 2048 x 768 fp16 115 / 129. Without its stores it takes 262, without the
  * matrix instructions 307, without both 144: loads and stores (1.16 GB, at a copy's rate 223) overlap in part only, since a tile's stores are
- * waited for AHEAD steps later, and LDS holds no longer ring. (The other two products gain nothing: 318 / 312 and 279 / 275.) */
+ * waited for AHEAD steps later, and LDS holds no longer ring. (The other two products gained nothing from such tiles before y's steps were
+ * staggered; not measured since.) */
 template <Kind KIND, int YTY, int RING> __device__ __forceinline__ void wide_body(const ExpertArgs &a) {
     constexpr int BM = 256, BN = 256, NT = 512, STEP = (BM + BN) * 64, CHUNKS = (BM + BN) * 4 / NT, AHEAD = RING - 1;
     constexpr bool AD = KIND == DW, BD = KIND != Y;

@@ -305,7 +305,7 @@ __device__ __forceinline__ float factor(const LoraArgs &a, int ad) { return a.sc
  * A wave 64 output rows, G lanes with eight values each a row of B (so that a wave's loads are whole lines), G turns for all of them; after
  * each the group's sum stays with the lane whose row it is. Lane l ends with row l. B is read once for all tokens of the adapter up to
  * a rank of 64, and the tokens are taken four at a time. u of the whole tile is fetched beside the adapters' numbers, not after them, and
- * the next 64 rows' operands during these' sums. */
+ * the next 64 rows' operands during these' sums (above a rank of 64 B does not fit and is fetched for every four tokens). */
 template <int WTY, int G> __device__ __forceinline__ void upv_body(const LoraArgs &a) {
     constexpr int RP = 8 * G, TURNS = G < 8 ? G : 8; /* turns whose B is in registers at once */
     __shared__ __attribute__((aligned(16))) float lu[16][RP]; /* A x of the tile's tokens; of those without an adapter nothing that is used */

@@ -3,7 +3,8 @@
  * A row is read once and stays in registers from the sum of its squares to its codes: L lanes a row (a wave, or a block of 256 or 1024),
  * NC pieces of 16 bytes a lane, a unit of 32 values in 8 (16-bit types: 4) lanes. Bound by memory for many rows. The sum, the root and the first
  * product are in 64 bits, which the memory's time covers: the codes are then those of the formula whatever L is, and the largest
- * fp32 values need no scaling. Rows of more than four pieces in each of 1024
+ * fp32 values need no scaling. 16-bit rows are held as fp32, for which four pieces in each of 1024 lanes (rows of 16385 to 32768 values) have 11
+ * registers too few (48 bytes of scratch a lane). Rows of more than four pieces in each of 1024
  * lanes, and rows that end inside a piece (no codes then), are read twice. */
 #include <hip/hip_runtime.h>
 
